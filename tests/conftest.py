@@ -25,6 +25,13 @@ def pytest_configure(config):
 def pytest_collection_modifyitems(config, items):
     import torch
 
+    # (an empty mount point is no source tree: what loads the reference's own modules is skipped as where there is none)
+    if not os.path.exists("/root/reference/models/matcher.py"):
+        absent = pytest.mark.skip(reason="needs the reference's source tree")
+        for item in items:
+            if item.path.name == "test_reference_criteria.py":
+                item.add_marker(absent)
+
     if torch.cuda.is_available():
         return
     skip = pytest.mark.skip(reason="no GPU in this process")
