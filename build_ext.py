@@ -18,7 +18,10 @@ SOURCES = ["cost_kernel.hip", "lap_kernel.hip", "pack_kernel.hip", "consumer_ker
 HEADERS = [os.path.join(CSRC, "dm_common.h"), os.path.join(CSRC, "cost_math.h"), os.path.join(ROOT, "include", "detr_match.h")]
 # -ffp-contract=off: every fp32 operation of the cost is rounded separately, as in the
 # reference's elementwise torch ops (hipcc would otherwise fuse a*b+c into an fma).
-FLAGS = ["--offload-arch=gfx950", "-O3", "-ffp-contract=off", "-fPIC", "-shared", "-std=c++17", "-Wno-pass-failed"]
+# -packed-fp32-ops: no v_pk_*_f32, which -O3 makes of ordinary float code by itself; some of their forms have given wrong
+# results now and then, with no error.
+FLAGS = ["--offload-arch=gfx950", "-O3", "-ffp-contract=off", "-fPIC", "-shared", "-std=c++17", "-Wno-pass-failed",
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def _stale():
