@@ -19,6 +19,8 @@ ABI_VERSION = 2
 MAX_SETS_PER_LAUNCH = 16
 NOALLOC_MAX_COST_FLOATS = 8 << 20
 CLS_LOSS_PARTIALS = 4096
+MAX_EXPERTS = 1024
+DTYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 OK, E_INVALID_ARG, E_LAUNCH, E_UNSUPPORTED = 0, -1, -2, -3
 NEED_BUFFERS = 1     # dm_match_targets_f32 without pack buffers: nothing launched
@@ -37,6 +39,11 @@ class DmIndexSet(ctypes.Structure):
                 ("out_off", ctypes.c_int64), ("Q", ctypes.c_int32), ("boxes_stride", ctypes.c_int32)]
 
 
+class DmRouterSet(ctypes.Structure):
+    _fields_ = [("logits", ctypes.c_void_p), ("mask", ctypes.c_void_p), ("experts", ctypes.c_void_p), ("grad", ctypes.c_void_p),
+                ("image_stride", ctypes.c_int64), ("Q", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
 class DmParams(ctypes.Structure):
     _fields_ = [("cls_mode", ctypes.c_int32), ("w_class", ctypes.c_float), ("w_bbox", ctypes.c_float),
                 ("w_giou", ctypes.c_float), ("focal_alpha", ctypes.c_float), ("focal_gamma", ctypes.c_float)]
@@ -49,6 +56,7 @@ EXPORTS = ["dm_pack_targets", "dm_abi_version", "dm_strerror", "dm_last_hip_erro
            "dm_debug_set_knob",
            "dm_pair_loss_f32", "dm_pair_loss_backward_f32", "dm_pair_list_loss_f32", "dm_pair_list_backward_f32", "dm_target_classes_i64",
            "dm_focal_loss_f32", "dm_cross_entropy_f32",
+           "dm_balance_workspace", "dm_balance_loss", "dm_balance_backward", "dm_expert_counts",
            "dm_atss_f32", "dm_frcnn_f32", "dm_frcnn_dense_i64"]
 
 
@@ -106,6 +114,15 @@ def _load():
                                       ctypes.c_int64, i32, vp, vp, vp, vp, vp]
     lib.dm_cross_entropy_f32.restype = ctypes.c_int
     lib.dm_cross_entropy_f32.argtypes = [vp, vp, vp, ctypes.c_int64, i32, ctypes.c_int64, vp, vp, vp, vp, vp]
+    i64 = ctypes.c_int64
+    lib.dm_balance_workspace.restype = i64
+    lib.dm_balance_workspace.argtypes = [setp, i32, i32, i32, i32]
+    lib.dm_balance_loss.restype = ctypes.c_int
+    lib.dm_balance_loss.argtypes = [setp, i32, i32, i32, i32, i32, i32, i32, vp, vp, vp, vp, vp, vp, vp, i64, vp, vp]
+    lib.dm_balance_backward.restype = ctypes.c_int
+    lib.dm_balance_backward.argtypes = [setp, i32, i32, i32, i32, i32, i32, vp, vp, vp, vp, vp]
+    lib.dm_expert_counts.restype = ctypes.c_int
+    lib.dm_expert_counts.argtypes = [setp, i32, i32, i32, i32, i32, i32, vp, vp, i64, vp, vp]
     lib.dm_atss_f32.restype = ctypes.c_int
     lib.dm_atss_f32.argtypes = [isetp, i32, i32, i32, i32, vp, vp, vp, vp, vp]
     lib.dm_frcnn_f32.restype = ctypes.c_int

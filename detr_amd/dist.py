@@ -165,3 +165,18 @@ def all_reduce_num_boxes(local_counts: Sequence[int], device, group=None) -> tor
     """[S] float32 tensor on ``device``: clamp(sum over ranks / world_size, min=1).
     `start_num_boxes_all_reduce(...).result()` in one call."""
     return start_num_boxes_all_reduce(local_counts, device, group).result()
+
+
+def all_reduce_expert_counts(counts: torch.Tensor, group=None) -> torch.Tensor:
+    """The per-expert counts of all ranks (`losses.expert_counts` summed over the group) for `losses.balance_losses(...,
+    counts=...)`: the shares then are those of the global batch, and the average of the ranks' gradients is the gradient of
+    the global balance loss when the ranks hold equally many rows.  `counts` itself is left as it is."""
+    total = counts.clone()
+    if dist.is_available() and dist.is_initialized() and dist.get_world_size(group) > 1:
+        if total.is_cuda and dist.get_backend(group) == "gloo":
+            host = total.cpu()          # (gloo takes host memory)
+            dist.all_reduce(host, op=dist.ReduceOp.SUM, group=group)
+            total.copy_(host)
+        else:
+            dist.all_reduce(total, op=dist.ReduceOp.SUM, group=group)
+    return total

@@ -23,8 +23,8 @@ forward and as many backward.
 is the body of a criterion's loop over its Hungarian-matched output sets (loss.py:164-176) on top of all of the above:
 one matching launch for the step, nothing synchronises.
 """
-import ctypes
-from typing import List, Optional, Sequence, Tuple
+import struct
+from typing import List, NamedTuple, Optional, Sequence, Tuple
 
 import torch
 
@@ -227,29 +227,35 @@ _cls_partials = {}       # (device index, stream handle) -> float64 workspace of
 _cls_status = {}         # device index -> int32 word the kernels OR their findings into
 
 
+def _status_word(device):
+    index = device.index if device.index is not None else torch.cuda.current_device()
+    status = _cls_status.get(index)
+    if status is None:
+        status = _cls_status[index] = torch.zeros(1, dtype=torch.int32, device=device)
+    return status
+
+
 def _cls_buffers(device):
     index = device.index if device.index is not None else torch.cuda.current_device()
     stream = torch.cuda.current_stream(device).cuda_stream
     partials = _cls_partials.get((index, stream))
     if partials is None:
         partials = _cls_partials[(index, stream)] = torch.empty(_lib.CLS_LOSS_PARTIALS, dtype=torch.float64, device=device)
-    status = _cls_status.get(index)
-    if status is None:
-        status = _cls_status[index] = torch.zeros(1, dtype=torch.int32, device=device)
-    return partials, status, stream
+    return partials, _status_word(device), stream
 
 
 def check_cls_status(device=None) -> None:
     """Raises RuntimeError when a `focal_loss` / `cross_entropy` call on `device` (default: the current one) since the
     last check met a class value outside the range the reference accepts (its `one_hot` / `cross_entropy` raise for
     such a value at once; here the row counts as ignored and the finding waits for this call), or a
-    `pair_list_box_loss_sums` call met an index outside its tensor.  Synchronises."""
+    `pair_list_box_loss_sums` call met an index outside its tensor, or a `balance_losses` call an expert's index outside
+    [-1, E).  Synchronises."""
     index = torch.cuda.current_device() if device is None else torch.device(device).index
     status = _cls_status.get(index)
     if status is not None and int(status.item()):
         status.zero_()
         raise RuntimeError("class values must lie in [0, number of classes] (the last one meaning no object), "
-                           "pair indices inside their tensors")
+                           "pair indices inside their tensors, experts' indices in [-1, number of experts)")
 
 
 def _checked(logits, target_cls):
@@ -403,6 +409,210 @@ class CrossEntropy(torch.nn.Module):
                 raise RuntimeError("detr_amd.losses.CrossEntropy: float32 GPU logits of [B, Q, C] or [B, C, Q] expected")
             return self.fallback(inputs, targets, num_boxes)
         return cross_entropy(x, targets, self.weight, self.ignore_index)
+
+
+# ---- the balance loss of expert routers ------------------------------------------------------------------------
+
+
+class BalanceLosses(NamedTuple):
+    """Of `balance_losses`: per set, or per set and image.  `z` is None with sigmoid scores."""
+    balance: torch.Tensor
+    z: Optional[torch.Tensor]
+    counts: torch.Tensor
+
+
+_ROUTER_SET = struct.Struct("=4Qq2i")          # DmRouterSet
+
+
+def _router_sets(tensors, masks, experts, grads=None) -> bytes:
+    """The DmRouterSet records of a call."""
+    return b"".join(
+        _ROUTER_SET.pack(x.data_ptr(), 0 if m is None else m.data_ptr(), 0 if e is None else e.data_ptr(),
+                         0 if g is None else g.data_ptr(), ops.image_stride(x), x.shape[1], 0)
+        for x, m, e, g in zip(tensors, masks, experts, grads or [None] * len(tensors)))
+
+
+def _per_set(value, n, what):
+    """`value` for each of n sets: None, one tensor for all of them, or a list of n."""
+    if value is None or isinstance(value, torch.Tensor):
+        return [value] * n
+    value = list(value)
+    if len(value) != n:
+        raise ValueError(f"{what}: one tensor, or one for each of the {n} sets")
+    return value
+
+
+def _checked_routers(router_logits, top_k, mask, experts):
+    """(logits, masks, experts) per set, as the kernels read them."""
+    logits = [router_logits] if isinstance(router_logits, torch.Tensor) else list(router_logits)
+    if not logits:
+        raise ValueError("no router logits")
+    first = logits[0]
+    if not first.is_cuda:
+        raise RuntimeError("detr_amd.losses: the balance loss runs on the GPU (there is no CPU path)")
+    if first.dtype not in _lib.DTYPE_CODES:
+        raise TypeError(f"router logits must be float32, bfloat16 or float16, got {first.dtype}")
+    if first.dim() != 3:
+        raise ValueError(f"router logits must be [B, Q, E], got {tuple(first.shape)}")
+    B, E = int(first.shape[0]), int(first.shape[2])
+    if E < 1:
+        raise ValueError("router logits for no expert")
+    if not isinstance(top_k, int) or top_k < 1 or (experts is None and top_k > E):
+        raise ValueError(f"top_k must be a whole number from 1 to the number of experts ({E}), got {top_k}")
+    masks, experts = _per_set(mask, len(logits), "mask"), _per_set(experts, len(logits), "experts")
+    for i, x in enumerate(logits):
+        if x.dtype != first.dtype or x.device != first.device:
+            raise TypeError("the router logits of a call must share their type and device")
+        if x.dim() != 3 or x.shape[0] != B or x.shape[2] != E:
+            raise ValueError("the router logits of a call must be [B, Q, E] with the same B and E")
+        x = x.detach()
+        logits[i] = x if ops.image_stride(x) is not None else x.contiguous()
+        m, e = masks[i], experts[i]
+        if m is not None:
+            if m.dtype != torch.bool or m.device != x.device:
+                raise TypeError("mask must be a bool tensor on the device of the router logits")
+            if tuple(m.shape) != (B, x.shape[1]):
+                raise ValueError(f"mask must be [B, Q] = {(B, int(x.shape[1]))}, got {tuple(m.shape)}")
+            masks[i] = m.contiguous()
+        if e is not None:
+            if e.dtype != torch.int64 or e.device != x.device:
+                raise TypeError("experts must be an int64 tensor on the device of the router logits")
+            if tuple(e.shape) != (B, x.shape[1], top_k):
+                raise ValueError(f"experts must be [B, Q, top_k] = {(B, int(x.shape[1]), top_k)}, got {tuple(e.shape)}")
+            experts[i] = e.contiguous()
+        elif i and experts[0] is not None:
+            raise ValueError("experts for all sets of the call or for none")
+    if experts[0] is None and any(e is not None for e in experts):
+        raise ValueError("experts for all sets of the call or for none")
+    return logits, masks, experts
+
+
+def _router_workspace(sets, S, B, E, per_image, device):
+    need = lib.dm_balance_workspace(sets, S, B, E, per_image)
+    if need < 0:
+        _lib.check(need, "dm_balance_workspace")
+    return torch.empty(need, dtype=torch.uint8, device=device)
+
+
+def _groups(S, B, per_image):
+    return (S, B) if per_image else (S,)
+
+
+class _BalanceLosses(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, checked, top_k, given_counts, sigmoid, per_image, *router_logits):
+        logits, masks, experts = checked
+        first = logits[0]
+        device, S, B, E = first.device, len(logits), int(first.shape[0]), int(first.shape[2])
+        groups = _groups(S, B, per_image)
+        n = S * B if per_image else S
+        dtype = _lib.DTYPE_CODES[first.dtype]
+        balance = torch.empty(groups, dtype=torch.float32, device=device)
+        z = None if sigmoid else torch.empty(groups, dtype=torch.float32, device=device)
+        counts = torch.empty(groups + (E,), dtype=torch.int64, device=device)
+        kept = torch.empty(n * (E + 1), dtype=torch.float32, device=device)          # slope [n, E], then inv_rows [n]
+        sets = _router_sets(logits, masks, experts)
+        with ops._on(device):
+            workspace = _router_workspace(sets, S, B, E, per_image, device)
+            rc = lib.dm_balance_loss(sets, S, B, E, top_k, dtype, sigmoid, per_image,
+                                     None if given_counts is None else given_counts.data_ptr(), balance.data_ptr(),
+                                     None if z is None else z.data_ptr(), counts.data_ptr(), kept.data_ptr(),
+                                     kept.data_ptr() + 4 * n * E, workspace.data_ptr(), workspace.numel(),
+                                     _status_word(device).data_ptr(), torch.cuda.current_stream(device).cuda_stream)
+        _lib.check(rc, "dm_balance_loss")
+        ctx.call = (dtype, sigmoid, per_image, [m is not None for m in masks])
+        ctx.save_for_backward(kept, *logits, *[m for m in masks if m is not None])
+        ctx.mark_non_differentiable(counts)
+        ctx.set_materialize_grads(False)
+        return balance, z, counts
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_balance, grad_z, _):
+        dtype, sigmoid, per_image, masked = ctx.call
+        kept, *rest = ctx.saved_tensors
+        S = len(masked)
+        logits, rest = rest[:S], iter(rest[S:])
+        if grad_balance is None and grad_z is None:
+            return (None,) * (5 + S)
+        device, B, E = kept.device, int(logits[0].shape[0]), int(logits[0].shape[2])
+        n = S * B if per_image else S
+        grads = [torch.empty(x.shape, dtype=x.dtype, device=device) for x in logits]
+        gb, gz = (None if g is None else g.contiguous() for g in (grad_balance, grad_z))
+        sets = _router_sets(logits, [next(rest) if m else None for m in masked], [None] * S, grads)
+        with ops._on(device):
+            rc = lib.dm_balance_backward(sets, S, B, E, dtype, sigmoid, per_image, kept.data_ptr(), kept.data_ptr() + 4 * n * E,
+                                         None if gb is None else gb.data_ptr(), None if gz is None else gz.data_ptr(),
+                                         torch.cuda.current_stream(device).cuda_stream)
+        _lib.check(rc, "dm_balance_backward")
+        return (None,) * 5 + tuple(g if need else None for g, need in zip(grads, ctx.needs_input_grad[5:]))
+
+
+def balance_losses(router_logits, top_k: int, mask=None, experts=None, counts: Optional[torch.Tensor] = None,
+                   scores: str = "softmax", per_image: bool = False) -> BalanceLosses:
+    """Balance loss, router z-loss and per-expert counts of the expert routers of a step's decoder layers, all in one call:
+    `router_logits` is the [B, Q, E] logits of every layer (a list of tensors that share B, E, type -- float32, bfloat16 or
+    float16 -- and device; a single tensor is a list of one).  For each set, or with `per_image` for each image of a set:
+
+        balance = E sum_e c_e / (sum c) P_e    c_e: how often expert e is among a row's `top_k` largest logits (the lowest
+                                               index first among equals; an expert at -inf is never chosen), P_e: the mean
+                                               of the row's score p_e -- softmax, or sigmoid over the sum of the row's sigmoids
+        z       = mean of logsumexp(row)^2     (softmax scores; None with sigmoid)
+        counts  = c, int64
+
+    `mask` [B, Q] bool (one for all sets, or a list): rows that are False count for nothing; neither does a row whose logits
+    are all -inf.  `experts` [B, Q, top_k] int64 (a list, like the logits): the experts the model's own router has chosen, -1
+    for one that was dropped; an index outside [-1, E) is reported by `check_cls_status()` and counts as -1.  `counts`
+    [S, E] (or [S, B, E]): the counts the shares c_e / sum c are taken from, instead of the call's own -- under data
+    parallelism those of all ranks (`expert_counts`, then `dist.all_reduce_expert_counts`).  Differentiable in the logits
+    through P and z (the counts are constants); rounded once to the logits' type."""
+    if scores not in ("softmax", "sigmoid"):
+        raise ValueError("scores must be 'softmax' or 'sigmoid'")
+    router_logits = [router_logits] if isinstance(router_logits, torch.Tensor) else list(router_logits)
+    checked = _checked_routers(router_logits, top_k, mask, experts)
+    if counts is not None:
+        first = checked[0][0]
+        want = _groups(len(router_logits), int(first.shape[0]), per_image) + (int(first.shape[2]),)
+        if counts.dtype != torch.int64 or counts.device != first.device:
+            raise TypeError("counts must be an int64 tensor on the device of the router logits")
+        if tuple(counts.shape) != want:
+            raise ValueError(f"counts must be {want}, got {tuple(counts.shape)}")
+        counts = counts.contiguous()
+    return BalanceLosses(*_BalanceLosses.apply(checked, top_k, counts, int(scores == "sigmoid"), int(per_image), *router_logits))
+
+
+@torch.no_grad()
+def expert_counts(router_logits, top_k: int, mask=None, per_image: bool = False) -> torch.Tensor:
+    """The counts of `balance_losses` alone, int64 [S, E] (or [S, B, E]): one pass that takes no exponentials."""
+    logits, masks, experts = _checked_routers(router_logits, top_k, mask, None)
+    first = logits[0]
+    device, S, B, E = first.device, len(logits), int(first.shape[0]), int(first.shape[2])
+    counts = torch.empty(_groups(S, B, per_image) + (E,), dtype=torch.int64, device=device)
+    sets = _router_sets(logits, masks, experts)
+    with ops._on(device):
+        workspace = _router_workspace(sets, S, B, E, int(per_image), device)
+        rc = lib.dm_expert_counts(sets, S, B, E, top_k, _lib.DTYPE_CODES[first.dtype], int(per_image), counts.data_ptr(),
+                                  workspace.data_ptr(), workspace.numel(), _status_word(device).data_ptr(),
+                                  torch.cuda.current_stream(device).cuda_stream)
+    _lib.check(rc, "dm_expert_counts")
+    return counts
+
+
+def balance_loss_total(router_logits, top_k: int, balance_weight: float = 0.01, z_weight: float = 0.0, mask=None, experts=None,
+                       counts: Optional[torch.Tensor] = None, scores: str = "softmax", per_image: bool = False,
+                       reduction: str = "mean") -> torch.Tensor:
+    """`balance_weight * balance + z_weight * z` of `balance_losses` over the sets as one scalar: their mean
+    (reduction='mean') or their sum; with `per_image` over the mean of each set's images."""
+    if reduction not in ("mean", "sum"):
+        raise ValueError("reduction must be 'mean' or 'sum'")
+    if z_weight and scores != "softmax":
+        raise ValueError("the router z-loss goes with softmax scores")
+    out = balance_losses(router_logits, top_k, mask, experts, counts, scores, per_image)
+    share = 1.0 / out.balance.shape[0] if reduction == "mean" else 1.0
+    if per_image:
+        share /= max(int(out.balance.shape[1]), 1)
+    total = out.balance.sum() * (share * balance_weight)
+    return total + out.z.sum() * (share * z_weight) if z_weight else total
 
 
 def set_losses(matcher, outputs_list, targets, n_cls: int, cls_loss: str = "focal", focal_alpha: float = 0.25,

@@ -332,6 +332,62 @@ int dm_cross_entropy_f32(const float *logits, const int64_t *target_cls, const f
                          int32_t *status, void *stream);
 
 /*
+ * ---- Balance loss of expert routers, and per-expert counts -----------------------------------------
+ * For models whose decoder layers have expert blocks: from the router's logits x [B][Q][E] of every layer (a "set"; no
+ * counterpart in the reference), with one group per set, or one per image of a set (per_image):
+ *   a row counts when its mask byte is not 0 and not all of its logits are -infinity; n = rows of the group that count
+ *   chosen   the top_k largest logits of the row, the lowest index first among equals, never one that is -infinity or
+ *            NaN; or, with `experts`, the indices given there (-1: none; an index outside [-1, E) raises
+ *            DM_ST_LABEL_RANGE and counts as -1)
+ *   c_e      how often expert e was chosen in the group; f_e = E c_e / sum c (0 when nothing was chosen)
+ *   p        DM_SCORES_SOFTMAX: softmax(x); DM_SCORES_SIGMOID: sigmoid(x) / sum sigmoid(x); P_e = the mean of p_e
+ *   balance  sum_e f_e P_e (1 when all is even; differentiated through P only)
+ *   z        the mean of logsumexp(x)^2 (softmax only)
+ * The sets of a call share B, E, top_k, dtype; their Q may differ.
+ *   sets[s].logits        device dtype[B][Q][E], rows dense inside an image
+ *   sets[s].mask          device uint8[B][Q], or NULL: every row counts
+ *   sets[s].experts       device int64[B][Q][top_k], or NULL for all sets
+ *   sets[s].grad          device dtype[B][Q][E], contiguous (dm_balance_backward)
+ *   sets[s].image_stride  elements from one image's logits to the next, 0 when contiguous
+ * Groups are numbered set * (per_image ? B : 1) + image.
+ *   given_counts          device int64[groups][E] or NULL: the counts the shares f are taken from, instead of the call's
+ *                         own (data parallelism: the counts of all ranks)
+ *   balance, z            device float[groups] (z may be NULL with DM_SCORES_SIGMOID)
+ *   counts                device int64[groups][E], the call's own counts
+ *   slope, inv_rows       device float[groups][E], float[groups]: f - 1 and 1 / n, what dm_balance_backward needs
+ *   workspace             device memory, 16-byte aligned, dm_balance_workspace bytes, overwritten
+ * grad = grad_balance / n * p_e (f_e - sum_j f_j p_j) [* (1 - sigmoid(x_e))] + grad_z / n * 2 logsumexp(x) p_e;
+ * grad_balance, grad_z: device float[groups], either may be NULL (no gradient from that side).
+ * Sums of a fixed order: bitwise reproducible.  1 <= E <= 1024, 1 <= top_k <= E (with experts: top_k >= 1), Q of a set and
+ * the total number of groups < 2^31 (DM_E_UNSUPPORTED beyond).  dm_balance_workspace returns a negative code for
+ * arguments that the calls refuse.
+ */
+#define DM_F32 0
+#define DM_BF16 1
+#define DM_F16 2
+#define DM_SCORES_SOFTMAX 0
+#define DM_SCORES_SIGMOID 1
+typedef struct {
+    const void *logits;
+    const uint8_t *mask;
+    const int64_t *experts;
+    void *grad;
+    int64_t image_stride;
+    int32_t Q;
+    int32_t reserved;
+} DmRouterSet;
+int64_t dm_balance_workspace(const DmRouterSet *sets, int S, int B, int E, int per_image);
+int dm_balance_loss(const DmRouterSet *sets, int S, int B, int E, int top_k, int dtype, int scores, int per_image,
+                    const int64_t *given_counts, float *balance, float *z, int64_t *counts, float *slope,
+                    float *inv_rows, void *workspace, int64_t workspace_bytes, int32_t *status, void *stream);
+int dm_balance_backward(const DmRouterSet *sets, int S, int B, int E, int dtype, int scores, int per_image,
+                        const float *slope, const float *inv_rows, const float *grad_balance, const float *grad_z,
+                        void *stream);
+/* The counts alone: one pass that takes no exponentials. */
+int dm_expert_counts(const DmRouterSet *sets, int S, int B, int E, int top_k, int dtype, int per_image, int64_t *counts,
+                     void *workspace, int64_t workspace_bytes, int32_t *status, void *stream);
+
+/*
  * ---- Co-DETR auxiliary assigners ---------------------------------------------------------------
  * Replace ATSS.forward and FasterRCNN.forward of
  * /root/reference/models/co_detr/auxiliary_head.py:22-60 and 69-96 for all output sets of a step
