@@ -14,8 +14,10 @@ ROOT = os.path.dirname(os.path.abspath(__file__))
 PKG = os.path.join(ROOT, "detr_amd")
 CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "libdetr_match.so")
-SOURCES = ["cost_kernel.hip", "lap_kernel.hip", "pack_kernel.hip", "consumer_kernels.hip", "cls_loss_kernels.hip", "routing_kernels.hip", "aux_kernels.hip", "abi.hip"]
-HEADERS = [os.path.join(CSRC, "dm_common.h"), os.path.join(CSRC, "lanes.h"), os.path.join(CSRC, "cost_math.h"), os.path.join(ROOT, "include", "detr_match.h")]
+SOURCES = ["cost_kernel.hip", "lap_kernel.hip", "pack_kernel.hip", "consumer_kernels.hip", "cls_loss_kernels.hip",
+           "saved_logits_kernels.hip", "routing_kernels.hip", "aux_kernels.hip", "abi.hip"]
+HEADERS = [os.path.join(CSRC, h) for h in ("dm_common.h", "lanes.h", "cls_common.h", "cost_math.h")] + \
+          [os.path.join(ROOT, "include", "detr_match.h")]
 # -ffp-contract=off: every fp32 operation of the cost is rounded separately, as in the
 # reference's elementwise torch ops (hipcc would otherwise fuse a*b+c into an fma).
 # -packed-fp32-ops: no v_pk_*_f32, which -O3 makes of ordinary float code by itself; some of their forms have given wrong

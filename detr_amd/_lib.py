@@ -56,6 +56,7 @@ EXPORTS = ["dm_pack_targets", "dm_abi_version", "dm_strerror", "dm_last_hip_erro
            "dm_debug_set_knob",
            "dm_pair_loss_f32", "dm_pair_loss_backward_f32", "dm_pair_list_loss_f32", "dm_pair_list_backward_f32", "dm_target_classes_i64",
            "dm_focal_loss_f32", "dm_cross_entropy_f32",
+           "dm_focal_loss_saved", "dm_focal_loss_from_saved", "dm_cross_entropy_saved", "dm_cross_entropy_from_saved",
            "dm_balance_workspace", "dm_balance_loss", "dm_balance_backward", "dm_expert_counts",
            "dm_atss_f32", "dm_frcnn_f32", "dm_frcnn_dense_i64"]
 
@@ -114,7 +115,15 @@ def _load():
                                       ctypes.c_int64, i32, vp, vp, vp, vp, vp]
     lib.dm_cross_entropy_f32.restype = ctypes.c_int
     lib.dm_cross_entropy_f32.argtypes = [vp, vp, vp, ctypes.c_int64, i32, ctypes.c_int64, vp, vp, vp, vp, vp]
-    i64 = ctypes.c_int64
+    i64, f32 = ctypes.c_int64, ctypes.c_float
+    lib.dm_focal_loss_saved.restype = ctypes.c_int
+    lib.dm_focal_loss_saved.argtypes = [vp, i32, vp, i64, i32, f32, f32, f32, i64, i32, vp, vp, vp, vp, vp, vp]
+    lib.dm_focal_loss_from_saved.restype = ctypes.c_int
+    lib.dm_focal_loss_from_saved.argtypes = [vp, vp, i32, vp, i64, i32, f32, f32, f32, i64, i32, vp, vp, vp]
+    lib.dm_cross_entropy_saved.restype = ctypes.c_int
+    lib.dm_cross_entropy_saved.argtypes = [vp, i32, vp, vp, i64, i32, i64, vp, vp, vp, vp, vp, vp]
+    lib.dm_cross_entropy_from_saved.restype = ctypes.c_int
+    lib.dm_cross_entropy_from_saved.argtypes = [vp, vp, i32, vp, vp, i64, i32, i64, vp, vp, vp, vp]
     lib.dm_balance_workspace.restype = i64
     lib.dm_balance_workspace.argtypes = [setp, i32, i32, i32, i32]
     lib.dm_balance_loss.restype = ctypes.c_int

@@ -67,16 +67,18 @@ def aux_head_like(other):
     return other
 
 
-def fuse_cls_criterion(own, seen_devices=None) -> bool:
+def fuse_cls_criterion(own, seen_devices=None, saved_bits: int = 32) -> bool:
     """Put the one-pass kernels of :mod:`detr_amd.losses` in front of `own.forward` when `own` is one of the reference's
     classification criteria -- ``FocalLoss(alpha, gamma, n_cls)`` (/root/reference/models/detr/loss.py:198-213) or
     ``CrossEntropy(weight)`` around an ``nn.CrossEntropyLoss`` (:185-195) -- told by their class name and the attributes
     they keep.  The module object, its buffers and its ``state_dict`` stay as they are: the replacement is an instance
     attribute ``forward`` (removed by `unfuse_cls_criterion`), which reads the parameters from `own` at every call and
     hands anything the kernels do not take (CPU or non-float32 tensors, a [B, Q, C] / [B, C, Q] layout that cannot be told
-    because Q == C) to the module's own forward.  Returns whether `own` was recognised."""
+    because Q == C) to the module's own forward.  `saved_bits` as in `losses.focal_loss`.  Returns whether `own` was
+    recognised."""
     from . import losses
 
+    losses._check_saved_bits(saved_bits)
     if "forward" in own.__dict__:
         return True
     name = type(own).__name__
@@ -84,11 +86,11 @@ def fuse_cls_criterion(own, seen_devices=None) -> bool:
     if name == "FocalLoss" and all(hasattr(own, a) for a in ("alpha", "gamma", "n_cls")):
         def forward(inputs, targets, num_boxes):
             x = losses._class_last(inputs, targets, own.n_cls, None)
-            if x is None or x.shape[-1] != own.n_cls or not losses._takes(x, targets):
+            if x is None or x.shape[-1] != own.n_cls or not losses._takes(x, targets, saved_bits):
                 return own_forward(inputs, targets, num_boxes)
             if seen_devices is not None:
                 seen_devices.add(x.device)
-            return losses.focal_loss(x, targets, num_boxes, own.alpha, own.gamma)
+            return losses.focal_loss(x, targets, num_boxes, own.alpha, own.gamma, saved_bits=saved_bits)
     elif name == "CrossEntropy" and isinstance(getattr(own, "criterion", None), torch.nn.CrossEntropyLoss) \
             and own.criterion.reduction == "mean" and own.criterion.label_smoothing == 0.0:
         def forward(inputs, targets, num_boxes=None):
@@ -96,11 +98,11 @@ def fuse_cls_criterion(own, seen_devices=None) -> bool:
             w = inner.weight
             C = w.shape[0] if w is not None else None
             x = losses._class_last(inputs, targets, C, None) if C is not None else None
-            if x is None or not losses._takes(x, targets) or w.device != x.device or w.dtype != torch.float32:
+            if x is None or not losses._takes(x, targets, saved_bits) or w.device != x.device or w.dtype != torch.float32:
                 return own_forward(inputs, targets, num_boxes)
             if seen_devices is not None:
                 seen_devices.add(x.device)
-            return losses.cross_entropy(x, targets, w, inner.ignore_index)
+            return losses.cross_entropy(x, targets, w, inner.ignore_index, saved_bits)
     else:
         return False
     own.forward = forward          # (an instance attribute in front of the class's method)
@@ -169,7 +171,7 @@ def flat_of_foreign_indices(matcher: HungarianMatcher, outputs, targets, indices
 
 
 def attach(criterion: torch.nn.Module, keys: Sequence[str] = MATCHED_KEYS, aux_heads: bool = True,
-           device_indices: bool = False, fused_consumers: bool = False) -> HungarianMatcher:
+           device_indices: bool = False, fused_consumers: bool = False, saved_bits: int = 32) -> HungarianMatcher:
     """Make `criterion` (an instance of one of the reference's Criterion classes, or anything that keeps its
     matcher in ``.matcher`` and is called as ``criterion(outputs, targets)``) use the gfx950 matcher, all sets
     of a step matched in one call.  `aux_heads`: also swap the ATSS / Faster-RCNN assigners a Co-DETR criterion keeps
@@ -199,10 +201,13 @@ def attach(criterion: torch.nn.Module, keys: Sequence[str] = MATCHED_KEYS, aux_h
     reference's ``one_hot`` / ``cross_entropy`` would refuse is raised as RuntimeError when the criterion returns.
     A Co-DETR criterion's ``calc_cls_loss_with_ignore`` (/root/reference/models/co_detr/loss.py:143-167) computes its
     loss with the same kernel on the dense map with the ignored rows marked, in place of the boolean-mask gather (a
-    host synchronisation), the one-hot tensor and the elementwise chain.
+    host synchronisation), the one-hot tensor and the elementwise chain.  `saved_bits` (with `fused_consumers`): what those
+    classification losses keep of every logit for the backward pass, as in `losses.focal_loss`.
     The wrappers are instance attributes holding local functions:
     `detach` the criterion before pickling the object itself (its ``state_dict`` is not affected).  Returns the
     matcher.  Calling it twice on one criterion is harmless."""
+    if saved_bits not in (32, 8) or (saved_bits == 8 and not fused_consumers):
+        raise ValueError("saved_bits must be 32, or 8 with fused_consumers")
     matcher = matcher_like(criterion.matcher)
     criterion.matcher = matcher
     heads = getattr(criterion, "aux_heads", None)
@@ -214,7 +219,7 @@ def attach(criterion: torch.nn.Module, keys: Sequence[str] = MATCHED_KEYS, aux_h
     device_indices = device_indices or fused_consumers
     cls_devices = set()
     if fused_consumers and isinstance(getattr(criterion, "cls_criterion", None), torch.nn.Module):
-        fuse_cls_criterion(criterion.cls_criterion, cls_devices)
+        fuse_cls_criterion(criterion.cls_criterion, cls_devices, saved_bits)
     if fused_consumers and callable(getattr(criterion, "calc_box_loss", None)):
         from . import losses
 
@@ -280,7 +285,7 @@ def attach(criterion: torch.nn.Module, keys: Sequence[str] = MATCHED_KEYS, aux_h
             n_cls = criterion.n_cls
             device = logits.device
             if logits.dim() != 3 or logits.shape[-1] != n_cls \
-                    or not losses._takes(logits, torch.empty(0, dtype=torch.int64, device=device)):
+                    or not losses._takes(logits, torch.empty(0, dtype=torch.int64, device=device), saved_bits):
                 return own_with_ignore(outputs, targets, pos_indices, neg_indices)
             n_pos = sum(int(src.shape[0]) for src, _ in pos_indices)
             target_cls = torch.full(logits.shape[:2], -1, dtype=torch.int64, device=device)
@@ -307,7 +312,7 @@ def attach(criterion: torch.nn.Module, keys: Sequence[str] = MATCHED_KEYS, aux_h
                     neg_b, neg_q = neg_b.to(device), neg_q.to(device)
                 target_cls[neg_b, neg_q] = n_cls
             cls_devices.add(device)
-            return losses.focal_loss(logits, target_cls, max(n_pos, 1), 0.25, 2.0, ignore_index=-1)
+            return losses.focal_loss(logits, target_cls, max(n_pos, 1), 0.25, 2.0, ignore_index=-1, saved_bits=saved_bits)
 
         criterion.calc_cls_loss_with_ignore = calc_cls_loss_with_ignore
 

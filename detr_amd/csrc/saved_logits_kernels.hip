@@ -1,0 +1,619 @@
+// The classification losses with 8 bits per logit kept for the backward pass, for gfx950 (MI355X): the forward pass reads
+// the logits once, sums the loss and leaves one byte per logit; the backward pass computes the gradient from the bytes.
+// Against keeping the float32 gradient (cls_loss_kernels.hip) the state between the two is a quarter, and a step moves
+// 4 + 1 and 1 + 4 bytes per float32 logit instead of 4 + 4 and 4 + 4.
+//
+// The code.  A block of logits shares a step 2^e, the finest from 2^-16 up to a coarsest one for which the whole numbers
+// rint(x 2^-e) of the block span at most 255; a logit's byte is how many steps it lies below the block's largest, 255 at
+// most.  With a power of two every operation of this is exact in float32 -- the byte does not depend on the arithmetic it
+// was found with -- and the logit is off by at most half a step.
+//   focal           blocks of 128 consecutive logits of the flat array, clamped to +-20 first: sigmoid(-20) = 2e-9 is below
+//                   the rounding of a float32 gradient of order one, and one masked logit does not take the block's
+//                   resolution away.  The span is 40 at most, so 2^-2 always suffices and no byte is cut off at 255.
+//                   A head per block, 32 bits: largest whole number << 8 | e.
+//   cross entropy   a block is a row: the softmax does not change when a row's largest logit is taken off, so e is all that
+//                   is kept beside the bytes.  2^-3 at most: logits further below the largest than 31.9 are cut off there,
+//                   at a probability of e^-31.9 = 1e-14.  (Logits beyond +-2^20 count as +-2^20.)
+// e = -128 marks a block with a NaN (cross entropy: a row whose softmax is NaN); its gradient is NaN.
+//
+// The gradient is that of the loss at the decoded logits; the loss itself is of the logits as they came.
+#include <algorithm>
+
+#include "cls_common.h"
+#include "lanes.h"
+
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr int FINEST = -16, FOCAL_COARSEST = -2, CE_COARSEST = -3, NOT_A_NUMBER = -128;
+constexpr float FOCAL_CLAMP = 20.0f, CE_CLAMP = 1048576.0f;
+
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((unsigned)(127 + e) << 23); }
+
+// The exponent of the step of a block whose logits lie in [low, high].  With high - low in [2^E, 2^(E+1)) the span at
+// 2^(E-9) is above 510 and at 2^(E-6) below 130: two trials after the first candidate E - 8.
+__device__ __forceinline__ int step_exponent(float high, float low, int coarsest)
+{
+    int e = (int)((__float_as_uint(high - low) >> 23) & 255u) - 127 - 8;
+    e = min(max(e, FINEST), coarsest);
+#pragma unroll
+    for (int trial = 0; trial < 2; ++trial) {
+        const float inverse = power_of_two(-e);
+        const bool wide = __builtin_rintf(high * inverse) - __builtin_rintf(low * inverse) > 255.0f;
+        e += wide && e < coarsest ? 1 : 0;
+    }
+    return e;
+}
+
+// softplus(z) and sigmoid(z)^gamma with z = -x for the positive logit and z = x for the others (the loss of a logit is
+// alpha_t times their product), and the derivative of that product.  e = exp(-|z|) serves all: sigmoid(z) = 1 / (1 + e) or
+// e / (1 + e), softplus(z) = max(z, 0) + log1p(e), sigmoid(z)^gamma = exp(-gamma softplus(-z)).
+struct FocalParts {
+    float softplus, power, sigmoid, rest;      // rest = 1 - sigmoid
+};
+template <bool GAMMA2>
+__device__ __forceinline__ FocalParts focal_parts(float z, float gamma)
+{
+    FocalParts f;
+    const float e = __builtin_amdgcn_exp2f(-__builtin_fabsf(z) * LOG2E);
+    const float one_e = 1.0f + e, r = __builtin_amdgcn_rcpf(one_e), er = e * r;
+    const bool up = z >= 0.0f;
+    f.sigmoid = up ? r : er;
+    f.rest = up ? er : r;
+    // log1p(e) = log(1 + e) + what the rounding of 1 + e dropped, over 1 + e
+    const float l1p = __builtin_amdgcn_logf(one_e) * LN2 + (e - (one_e - 1.0f)) * r;
+    f.softplus = __builtin_fmaxf(z, 0.0f) + l1p;
+    // (NaN: fminf passes it over, e carries it)
+    if (GAMMA2) f.power = f.sigmoid * f.sigmoid;
+    else f.power = __builtin_amdgcn_exp2f(-gamma * LOG2E * __builtin_fminf(__builtin_fmaxf(-z, 0.0f) + l1p, 1e30f));      // (0 x infinity)
+    return f;
+}
+
+__device__ __forceinline__ float flip(float x, bool positive)
+{
+    return __uint_as_float(__float_as_uint(x) ^ (positive ? 0x80000000u : 0u));
+}
+__device__ __forceinline__ float focal_alpha(const FocalParams &fp, bool positive)
+{
+    return fp.alpha >= 0.0f ? (positive ? fp.alpha : 1.0f - fp.alpha) : 1.0f;
+}
+
+// Rows and columns of a thread's quads of four consecutive logits, `stride` quads apart, walked by additions.
+struct Walk {
+    unsigned row, col, step_row, step_col, C;
+    __device__ __forceinline__ Walk(unsigned quad, unsigned stride, unsigned C_) : C(C_)
+    {
+        step_row = (stride << 2) / C;
+        step_col = (stride << 2) - step_row * C;
+        row = (quad << 2) / C;
+        col = (quad << 2) - row * C;
+    }
+    __device__ __forceinline__ void next()
+    {
+        col += step_col;
+        const bool over = col >= C;
+        col = over ? col - C : col;
+        row += step_row + (over ? 1u : 0u);
+    }
+};
+
+// The class codes of a quad's logits: with two or more classes four consecutive logits lie in at most two rows (the flat
+// array's quads start at multiples of four, so that also holds for two classes); with one, each is a row.
+template <bool ONE_CLASS>
+struct QuadRows {
+    int code[ONE_CLASS ? 4 : 2];
+    unsigned col, C;
+    __device__ __forceinline__ QuadRows(const int64_t *cls, unsigned row, unsigned col_, unsigned C_, unsigned rows,
+                                        const FocalParams &fp) : col(col_), C(C_)
+    {
+#pragma unroll
+        for (unsigned k = 0; k < (ONE_CLASS ? 4u : 2u); ++k) code[k] = row_code(cls[min(row + k, rows - 1)], C, fp);
+    }
+    // class code of logit k's row, and whether k is the row's positive logit
+    __device__ __forceinline__ int row_class(unsigned k, bool *positive) const
+    {
+        const bool wrapped = !ONE_CLASS && col + k >= C;
+        const int c = ONE_CLASS ? code[k] : (wrapped ? code[1] : code[0]);
+        const unsigned column = ONE_CLASS ? 0u : (wrapped ? col + k - C : col + k);
+        *positive = c == (int)column;
+        return c;
+    }
+};
+
+constexpr unsigned BLOCK_QUADS = 32;      // 128 logits: 32 lanes with four each
+
+// Loss, bytes and heads.  codes NULL: the loss alone.
+template <typename T, bool GAMMA2, bool ONE_CLASS>
+__global__ __launch_bounds__(CLS_THREADS) void focal_saved_kernel(const T *__restrict__ x, const int64_t *__restrict__ cls,
+                                                                  const unsigned n, const unsigned C, const unsigned rows,
+                                                                  const FocalParams fp, unsigned *__restrict__ codes,
+                                                                  int32_t *__restrict__ heads, double *__restrict__ partials,
+                                                                  int32_t *__restrict__ status)
+{
+    __shared__ double lds[CLS_THREADS / 64];
+    const unsigned quads = (n + 127) / 128 * BLOCK_QUADS;             // whole blocks
+    const unsigned stride = gridDim.x * CLS_THREADS;
+    unsigned i = blockIdx.x * CLS_THREADS + threadIdx.x;
+    Walk at(i, stride, C);
+    float acc = 0.0f;
+    bool bad = false;
+    // (the 32 lanes of a block run the same trips: the stride is a multiple of 32)
+    for (; i < quads; i += stride) {
+        const unsigned first = i << 2;
+        float v[4];
+        dm::load_quad(x, first, n, 0.0f, v);
+        const QuadRows<ONE_CLASS> q(cls, ONE_CLASS ? first : at.row, at.col, C, rows, fp);
+        float high = -__builtin_huge_valf(), low = __builtin_huge_valf(), c[4];
+#pragma unroll
+        for (unsigned k = 0; k < 4; ++k) {
+            bool positive;
+            const int row_class = q.row_class(k, &positive);
+            const bool inside = first + k < n;
+            const FocalParts f = focal_parts<GAMMA2>(flip(v[k], positive), fp.gamma);
+            acc += inside && row_class >= 0 ? focal_alpha(fp, positive) * (f.softplus * f.power) : 0.0f;
+            bad |= inside && row_class == ROW_BAD;
+            c[k] = fminf(fmaxf(v[k], -FOCAL_CLAMP), FOCAL_CLAMP);
+            low = inside ? fminf(low, c[k]) : low;
+            high = inside ? fmaxf(high, v[k] != v[k] ? __builtin_huge_valf() : c[k]) : high;      // (infinity: a NaN)
+        }
+        if (codes) {
+            high = dm::over_group<32>(high, dm::Max());
+            low = dm::over_group<32>(low, dm::Min());
+            const bool nan = high > FOCAL_CLAMP;
+            const int e = step_exponent(nan ? low : high, low, FOCAL_COARSEST);
+            const float inverse = power_of_two(-e);
+            const float top = __builtin_rintf(high * inverse);
+            unsigned packed = 0;
+#pragma unroll
+            for (unsigned k = 0; k < 4; ++k) {
+                const float code = fminf(top - __builtin_rintf(c[k] * inverse), 255.0f);
+                packed |= ((unsigned)(int)fmaxf(code, 0.0f) & 255u) << (8 * k);
+            }
+            codes[i] = packed;
+            if ((threadIdx.x & 31) == 0) heads[i / BLOCK_QUADS] = nan ? (NOT_A_NUMBER & 255) : (int)top * 256 | (e & 255);
+        }
+        if (!ONE_CLASS) at.next();
+    }
+    if (bad) dm::raise_status(status, DM_ST_LABEL_RANGE);
+    const double total = block_sum((double)acc, lds);
+    if (threadIdx.x == 0) partials[blockIdx.x] = total;
+}
+
+template <typename T, bool GAMMA2, bool ONE_CLASS>
+__global__ __launch_bounds__(CLS_THREADS) void focal_from_saved_kernel(const unsigned *__restrict__ codes,
+                                                                       const int32_t *__restrict__ heads,
+                                                                       const int64_t *__restrict__ cls, const unsigned n,
+                                                                       const unsigned C, const unsigned rows, const FocalParams fp,
+                                                                       const float *__restrict__ grad_loss, T *__restrict__ grad)
+{
+    const unsigned quads = (n + 3) / 4;
+    const unsigned stride = gridDim.x * CLS_THREADS;
+    unsigned i = blockIdx.x * CLS_THREADS + threadIdx.x;
+    Walk at(i, stride, C);
+    const float scale = fp.scale * grad_loss[0];
+    for (; i < quads; i += stride) {
+        const unsigned first = i << 2;
+        const unsigned packed = codes[i];
+        const int head = heads[i / BLOCK_QUADS];
+        const QuadRows<ONE_CLASS> q(cls, ONE_CLASS ? first : at.row, at.col, C, rows, fp);
+        const int e = (int)(int8_t)(head & 255);
+        const float step = e == NOT_A_NUMBER ? __builtin_nanf("") : power_of_two(e);
+        const float top = (float)(head >> 8);
+        float g[4];
+#pragma unroll
+        for (unsigned k = 0; k < 4; ++k) {
+            bool positive;
+            const int row_class = q.row_class(k, &positive);
+            const float x = (top - (float)((packed >> (8 * k)) & 255u)) * step;
+            const FocalParts f = focal_parts<GAMMA2>(flip(x, positive), fp.gamma);
+            const float gamma = GAMMA2 ? 2.0f : fp.gamma;
+            const float slope = f.power * (f.sigmoid + gamma * (f.softplus * f.rest));
+            g[k] = row_class >= 0 ? flip(focal_alpha(fp, positive) * scale * slope, positive) : 0.0f;
+        }
+        dm::store_quad(grad, first, n, g);
+        if (!ONE_CLASS) at.next();
+    }
+}
+
+// What a row of the class map weighs in the cross entropy: 0 when it is ignored or its class is none of the row's.
+__device__ __forceinline__ float row_weight(int64_t y, unsigned C, int64_t ignore_index, const float *weight, bool *bad)
+{
+    if (y == ignore_index) return 0.0f;
+    if (y < 0 || y >= (int64_t)C) {
+        *bad = true;
+        return 0.0f;
+    }
+    return weight ? weight[y] : 1.0f;
+}
+
+// L lanes share a row and keep it in registers, NQ quads of four logits each.
+template <typename T, int NQ, int L>
+__global__ __launch_bounds__(CLS_THREADS) void ce_saved_kernel(const T *__restrict__ x, const int64_t *__restrict__ cls,
+                                                               const float *__restrict__ weight, const unsigned rows,
+                                                               const unsigned C, const int64_t ignore_index,
+                                                               uint8_t *__restrict__ codes, int8_t *__restrict__ steps,
+                                                               double *__restrict__ partials, int32_t *__restrict__ status)
+{
+    __shared__ double lds[CLS_THREADS / 64];
+    const unsigned sub = threadIdx.x & (L - 1);
+    constexpr unsigned ROWS = CLS_THREADS / L;
+    const float inf = __builtin_huge_valf();
+    float num = 0.0f, den = 0.0f;
+    bool bad = false;
+    // (every lane makes the same trips: the reductions need all lanes of a row)
+    for (unsigned r0 = blockIdx.x * ROWS; r0 < rows; r0 += gridDim.x * ROWS) {
+        const unsigned row = r0 + threadIdx.x / L;
+        const bool live = row < rows;
+        const T *lg = x + (size_t)(live ? row : 0) * C;
+        float v[4 * NQ];
+        float mx = -inf, mn = inf;
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) {
+            const unsigned c = 4 * (q * L + sub);
+            float t[4];
+            dm::load_quad(lg, c, C, -inf, t);
+#pragma unroll
+            for (unsigned k = 0; k < 4; ++k) {
+                v[4 * q + k] = t[k];
+                mx = fmaxf(mx, t[k]);
+                mn = c + k < C ? fminf(mn, t[k]) : mn;
+            }
+        }
+        mx = dm::over_group<L>(mx, dm::Max());
+        mn = dm::over_group<L>(mn, dm::Min());
+        float sum = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 4 * NQ; ++k) sum += __builtin_amdgcn_exp2f((v[k] - mx) * LOG2E);      // (past the row: exp2(-inf) = 0)
+        sum = dm::over_group<L>(sum, dm::Add());
+        if (!live) continue;
+        const int64_t y = cls[row];
+        const float w = row_weight(y, C, ignore_index, weight, &bad);
+        if (sub == 0 && w != 0.0f) {
+            num += w * ((mx + __builtin_amdgcn_logf(sum) * LN2) - (float)lg[y]);
+            den += w;
+        }
+        if (!codes) continue;
+        const float high = fminf(fmaxf(mx, -CE_CLAMP), CE_CLAMP), low = fminf(fmaxf(mn, -CE_CLAMP), CE_CLAMP);
+        const int e = step_exponent(high, low, CE_COARSEST);
+        const float inverse = power_of_two(-e), top = __builtin_rintf(high * inverse);
+        uint8_t *out = codes + (size_t)row * C;
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) {
+            const unsigned c = 4 * (q * L + sub);
+            unsigned code[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float z = fminf(fmaxf(v[4 * q + k], -CE_CLAMP), CE_CLAMP);
+                code[k] = (unsigned)fminf(top - __builtin_rintf(z * inverse), 255.0f);
+            }
+            if (c + 4 <= C) {
+                dm::Quad<uint8_t>::type t;
+                t.x = (uint8_t)code[0]; t.y = (uint8_t)code[1]; t.z = (uint8_t)code[2]; t.w = (uint8_t)code[3];
+                *reinterpret_cast<dm::Quad<uint8_t>::type *>(out + c) = t;
+            } else {
+#pragma unroll
+                for (unsigned k = 0; k < 4; ++k)
+                    if (c + k < C) out[c + k] = (uint8_t)code[k];
+            }
+        }
+        if (sub == 0) steps[row] = (int8_t)(sum == sum ? e : NOT_A_NUMBER);
+    }
+    if (bad) dm::raise_status(status, DM_ST_LABEL_RANGE);
+    const double a = block_sum((double)num, lds);
+    const double b = block_sum((double)den, lds);
+    if (threadIdx.x == 0) {
+        partials[2 * blockIdx.x] = a;
+        partials[2 * blockIdx.x + 1] = b;
+    }
+}
+
+template <typename T, int NQ, int L>
+__global__ __launch_bounds__(CLS_THREADS) void ce_from_saved_kernel(const uint8_t *__restrict__ codes, const int8_t *__restrict__ steps,
+                                                                    const int64_t *__restrict__ cls, const float *__restrict__ weight,
+                                                                    const unsigned rows, const unsigned C,
+                                                                    const int64_t ignore_index, const float *__restrict__ inv_weight,
+                                                                    const float *__restrict__ grad_loss, T *__restrict__ grad)
+{
+    const unsigned sub = threadIdx.x & (L - 1);
+    constexpr unsigned ROWS = CLS_THREADS / L;
+    const float scale = inv_weight[0] * grad_loss[0];
+    for (unsigned r0 = blockIdx.x * ROWS; r0 < rows; r0 += gridDim.x * ROWS) {
+        const unsigned row = r0 + threadIdx.x / L;
+        const bool live = row < rows;
+        const size_t base = (size_t)(live ? row : 0) * C;
+        const int e = steps[live ? row : 0];
+        const float step = e == NOT_A_NUMBER ? __builtin_nanf("") : -power_of_two(e) * LOG2E;
+        float p[4 * NQ];
+        float sum = 0.0f;
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) {
+            float t[4];
+            dm::load_quad(codes + base, 4 * (q * L + sub), C, __builtin_huge_valf(), t);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                p[4 * q + k] = __builtin_amdgcn_exp2f(t[k] * step);
+                sum += p[4 * q + k];
+            }
+        }
+        sum = dm::over_group<L>(sum, dm::Add());
+        if (!live) continue;
+        bool bad = false;
+        const int64_t y = cls[row];
+        const float w = row_weight(y, C, ignore_index, weight, &bad);
+        const float inv = __builtin_amdgcn_rcpf(sum), ws = w * scale;
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) {
+            const unsigned c = 4 * (q * L + sub);
+            float g[4];
+#pragma unroll
+            for (unsigned k = 0; k < 4; ++k)
+                g[k] = w == 0.0f ? 0.0f : (p[4 * q + k] * inv - ((int64_t)(c + k) == y ? 1.0f : 0.0f)) * ws;
+            dm::store_quad(grad + base, c, C, g);
+        }
+    }
+}
+
+// Rows too long for a wavefront's registers: a workgroup per row, which it walks twice (forward: largest, smallest and sum
+// of exponentials in one pass, the bytes in the second, out of the cache; backward: the sum, then the gradient).
+constexpr int WIDE_WAVES = CLS_THREADS / 64;
+
+struct RowStats {
+    float mx, mn, sum;      // sum of exp(x - mx)
+};
+__device__ __forceinline__ RowStats join(const RowStats &a, const RowStats &b)
+{
+    RowStats r;
+    r.mx = fmaxf(a.mx, b.mx);
+    r.mn = fminf(a.mn, b.mn);
+    // (two parts at -infinity have equal maxima: no difference is taken of them, a sum of zero stays zero)
+    const float fa = a.mx == r.mx ? 1.0f : __builtin_amdgcn_exp2f((a.mx - r.mx) * LOG2E);
+    const float fb = b.mx == r.mx ? 1.0f : __builtin_amdgcn_exp2f((b.mx - r.mx) * LOG2E);
+    r.sum = a.sum * fa + b.sum * fb;
+    return r;
+}
+
+template <typename T>
+__global__ __launch_bounds__(CLS_THREADS) void ce_saved_wide_kernel(const T *__restrict__ x, const int64_t *__restrict__ cls,
+                                                                    const float *__restrict__ weight, const unsigned rows,
+                                                                    const unsigned C, const int64_t ignore_index,
+                                                                    uint8_t *__restrict__ codes, int8_t *__restrict__ steps,
+                                                                    double *__restrict__ partials, int32_t *__restrict__ status)
+{
+    __shared__ RowStats lds[WIDE_WAVES];
+    const float inf = __builtin_huge_valf();
+    double num = 0.0, den = 0.0;
+    bool bad = false;
+    for (unsigned row = blockIdx.x; row < rows; row += gridDim.x) {
+        const T *lg = x + (size_t)row * C;
+        RowStats s{-inf, inf, 0.0f};
+        for (unsigned c = 4 * threadIdx.x; c < C; c += 4 * CLS_THREADS) {
+            float t[4];
+            dm::load_quad(lg, c, C, -inf, t);
+            const float m4 = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+            const float m = fmaxf(s.mx, m4);
+            const float keep = s.mx == m ? 1.0f : __builtin_amdgcn_exp2f((s.mx - m) * LOG2E);
+            float add = 0.0f;
+#pragma unroll
+            for (unsigned k = 0; k < 4; ++k) {
+                // (-infinity adds nothing, also while nothing larger has been met; a NaN, or an infinity over itself, is NaN)
+                if (c + k < C) {
+                    add += t[k] == -inf ? 0.0f : __builtin_amdgcn_exp2f((t[k] - m) * LOG2E);
+                    s.mn = fminf(s.mn, t[k]);
+                }
+            }
+            s.sum = s.sum * keep + add;
+            s.mx = m;
+        }
+#pragma unroll
+        for (int off = 32; off >= 1; off >>= 1)
+            s = join(s, RowStats{__shfl_xor(s.mx, off), __shfl_xor(s.mn, off), __shfl_xor(s.sum, off)});
+        __syncthreads();                 // (the previous row's use of lds is over)
+        if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = s;
+        __syncthreads();
+        s = lds[0];
+        for (int w = 1; w < WIDE_WAVES; ++w) s = join(s, lds[w]);
+        const float sum = s.mx == -inf ? __builtin_nanf("") : s.sum;       // (nothing but -infinity: NaN, as in a softmax)
+        if (threadIdx.x == 0) {
+            const int64_t y = cls[row];
+            const float w = row_weight(y, C, ignore_index, weight, &bad);
+            if (w != 0.0f) {
+                num += (double)(w * ((s.mx + __builtin_amdgcn_logf(sum) * LN2) - (float)lg[y]));
+                den += (double)w;
+            }
+        }
+        if (!codes) continue;
+        const float high = fminf(fmaxf(s.mx, -CE_CLAMP), CE_CLAMP), low = fminf(fmaxf(s.mn, -CE_CLAMP), CE_CLAMP);
+        const int e = step_exponent(high, low, CE_COARSEST);
+        const float inverse = power_of_two(-e), top = __builtin_rintf(high * inverse);
+        uint8_t *out = codes + (size_t)row * C;
+        for (unsigned c = 4 * threadIdx.x; c < C; c += 4 * CLS_THREADS) {
+            float t[4];
+            dm::load_quad(lg, c, C, -inf, t);
+            for (unsigned k = 0; k < 4; ++k) {
+                const float z = fminf(fmaxf(t[k], -CE_CLAMP), CE_CLAMP);
+                if (c + k < C) out[c + k] = (uint8_t)(unsigned)fminf(top - __builtin_rintf(z * inverse), 255.0f);
+            }
+        }
+        if (threadIdx.x == 0) steps[row] = (int8_t)(sum == sum ? e : NOT_A_NUMBER);
+    }
+    if (bad) dm::raise_status(status, DM_ST_LABEL_RANGE);
+    if (threadIdx.x == 0) {
+        partials[2 * blockIdx.x] = num;
+        partials[2 * blockIdx.x + 1] = den;
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(CLS_THREADS) void ce_from_saved_wide_kernel(const uint8_t *__restrict__ codes,
+                                                                         const int8_t *__restrict__ steps,
+                                                                         const int64_t *__restrict__ cls,
+                                                                         const float *__restrict__ weight, const unsigned rows,
+                                                                         const unsigned C, const int64_t ignore_index,
+                                                                         const float *__restrict__ inv_weight,
+                                                                         const float *__restrict__ grad_loss, T *__restrict__ grad)
+{
+    __shared__ float lds[WIDE_WAVES];
+    const float scale = inv_weight[0] * grad_loss[0];
+    for (unsigned row = blockIdx.x; row < rows; row += gridDim.x) {
+        const size_t base = (size_t)row * C;
+        const int e = steps[row];
+        const float step = e == NOT_A_NUMBER ? __builtin_nanf("") : -power_of_two(e) * LOG2E;
+        float sum = 0.0f;
+        for (unsigned c = 4 * threadIdx.x; c < C; c += 4 * CLS_THREADS) {
+            float t[4];
+            dm::load_quad(codes + base, c, C, __builtin_huge_valf(), t);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) sum += __builtin_amdgcn_exp2f(t[k] * step);
+        }
+        sum = dm::over_group<64>(sum, dm::Add());
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = sum;
+        __syncthreads();
+        sum = lds[0];
+        for (int w = 1; w < WIDE_WAVES; ++w) sum += lds[w];
+        bool bad = false;
+        const int64_t y = cls[row];
+        const float w = row_weight(y, C, ignore_index, weight, &bad);
+        const float inv = __builtin_amdgcn_rcpf(sum), ws = w * scale;
+        for (unsigned c = 4 * threadIdx.x; c < C; c += 4 * CLS_THREADS) {
+            float t[4], g[4];
+            dm::load_quad(codes + base, c, C, __builtin_huge_valf(), t);
+#pragma unroll
+            for (unsigned k = 0; k < 4; ++k)
+                g[k] = w == 0.0f ? 0.0f : (__builtin_amdgcn_exp2f(t[k] * step) * inv - ((int64_t)(c + k) == y ? 1.0f : 0.0f)) * ws;
+            dm::store_quad(grad + base, c, C, g);
+        }
+    }
+}
+
+// ---- host side ----
+
+template <typename T>
+void launch_focal_saved(const void *logits, const int64_t *cls, unsigned n, unsigned C, unsigned rows, const FocalParams &fp,
+                        uint8_t *codes, int32_t *heads, double *partials, int32_t *status, int blocks, hipStream_t st)
+{
+    auto kernel = fp.gamma == 2.0f ? (C == 1 ? focal_saved_kernel<T, true, true> : focal_saved_kernel<T, true, false>)
+                                   : (C == 1 ? focal_saved_kernel<T, false, true> : focal_saved_kernel<T, false, false>);
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(CLS_THREADS), 0, st, static_cast<const T *>(logits), cls, n, C, rows, fp,
+                       reinterpret_cast<unsigned *>(codes), heads, partials, status);
+}
+template <typename T>
+void launch_focal_from_saved(const uint8_t *codes, const int32_t *heads, const int64_t *cls, unsigned n, unsigned C, unsigned rows,
+                             const FocalParams &fp, const float *grad_loss, void *grad, int blocks, hipStream_t st)
+{
+    auto kernel = fp.gamma == 2.0f ? (C == 1 ? focal_from_saved_kernel<T, true, true> : focal_from_saved_kernel<T, true, false>)
+                                   : (C == 1 ? focal_from_saved_kernel<T, false, true> : focal_from_saved_kernel<T, false, false>);
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(CLS_THREADS), 0, st, reinterpret_cast<const unsigned *>(codes), heads, cls, n, C,
+                       rows, fp, grad_loss, static_cast<T *>(grad));
+}
+
+constexpr unsigned WIDEST = 2048;      // logits of a row that a wavefront keeps in registers
+
+unsigned ce_blocks(unsigned rows, unsigned C)
+{
+    const unsigned rows_per_block = C <= WIDEST ? CLS_THREADS / 64 : 1;
+    return std::max(1u, std::min((unsigned)CLS_MAX_BLOCKS, (rows + rows_per_block - 1) / rows_per_block));
+}
+template <typename T>
+void launch_ce_saved(const void *logits, const int64_t *cls, const float *weight, unsigned rows, unsigned C, int64_t ignore_index,
+                     uint8_t *codes, int8_t *steps, double *partials, int32_t *status, unsigned blocks, hipStream_t st)
+{
+    auto kernel = C <= 256 ? ce_saved_kernel<T, 1, 64> : C <= 512 ? ce_saved_kernel<T, 2, 64> : C <= 1024 ? ce_saved_kernel<T, 4, 64>
+                  : C <= WIDEST ? ce_saved_kernel<T, 8, 64> : ce_saved_wide_kernel<T>;
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(CLS_THREADS), 0, st, static_cast<const T *>(logits), cls, weight, rows, C,
+                       ignore_index, codes, steps, partials, status);
+}
+template <typename T>
+void launch_ce_from_saved(const uint8_t *codes, const int8_t *steps, const int64_t *cls, const float *weight, unsigned rows, unsigned C,
+                          int64_t ignore_index, const float *inv_weight, const float *grad_loss, void *grad, unsigned blocks,
+                          hipStream_t st)
+{
+    auto kernel = C <= 256 ? ce_from_saved_kernel<T, 1, 64> : C <= 512 ? ce_from_saved_kernel<T, 2, 64>
+                  : C <= 1024 ? ce_from_saved_kernel<T, 4, 64> : C <= WIDEST ? ce_from_saved_kernel<T, 8, 64> : ce_from_saved_wide_kernel<T>;
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(CLS_THREADS), 0, st, codes, steps, cls, weight, rows, C, ignore_index, inv_weight,
+                       grad_loss, static_cast<T *>(grad));
+}
+
+bool known(int dtype) { return dtype == DM_F32 || dtype == DM_BF16 || dtype == DM_F16; }
+
+int check_from_saved(const uint8_t *codes, const void *marks, int dtype, const int64_t *target_cls, int64_t rows, int C,
+                     const float *grad_loss, const void *grad_out)
+{
+    if (rows < 0 || C < 1 || !known(dtype)) return DM_E_INVALID_ARG;
+    if (rows > 0 && (!codes || !marks || !target_cls || !grad_loss || !grad_out)) return DM_E_INVALID_ARG;
+    if ((unsigned long long)rows * (unsigned long long)C >= (1ull << 31)) return DM_E_UNSUPPORTED;
+    return DM_OK;
+}
+
+}  // namespace
+
+extern "C" int dm_focal_loss_saved(const void *logits, int dtype, const int64_t *target_cls, int64_t rows, int C, float alpha,
+                                   float gamma, float scale, int64_t ignore_index, int use_ignore, float *loss_out,
+                                   uint8_t *codes, int32_t *heads, double *partials, int32_t *status, void *stream)
+{
+    int rc = check_common(logits, target_cls, rows, C, loss_out, partials, status);
+    if (rc != DM_OK) return rc;
+    if (!known(dtype) || (codes != nullptr) != (heads != nullptr)) return DM_E_INVALID_ARG;
+    if (((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(heads)) & 3) != 0) return DM_E_INVALID_ARG;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    const unsigned n = (unsigned)(rows * C);
+    const unsigned quads = (n + 127) / 128 * BLOCK_QUADS;
+    const int blocks = (int)std::max(1u, std::min((unsigned)CLS_MAX_BLOCKS, (quads + CLS_THREADS - 1) / CLS_THREADS));
+    const FocalParams fp{alpha, gamma, scale, ignore_index, use_ignore};
+    auto launch = dtype == DM_F32 ? launch_focal_saved<float> : dtype == DM_BF16 ? launch_focal_saved<dm::bf16_t> : launch_focal_saved<dm::half_t>;
+    launch(logits, target_cls, n, (unsigned)C, (unsigned)rows, fp, codes, heads, partials, status, blocks, st);
+    rc = dm::check_hip(hipGetLastError(), "focal_saved_kernel launch");
+    if (rc != DM_OK) return rc;
+    hipLaunchKernelGGL(cls_loss_finish_kernel<true>, dim3(1), dim3(CLS_THREADS), 0, st, partials, blocks, scale, loss_out);
+    return dm::check_hip(hipGetLastError(), "cls_loss_finish_kernel launch");
+}
+
+extern "C" int dm_focal_loss_from_saved(const uint8_t *codes, const int32_t *heads, int dtype, const int64_t *target_cls,
+                                        int64_t rows, int C, float alpha, float gamma, float scale, int64_t ignore_index,
+                                        int use_ignore, const float *grad_loss, void *grad_out, void *stream)
+{
+    const int rc = check_from_saved(codes, heads, dtype, target_cls, rows, C, grad_loss, grad_out);
+    if (rc != DM_OK) return rc;
+    if (((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(heads)) & 3) != 0) return DM_E_INVALID_ARG;
+    if (rows == 0) return DM_OK;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    const unsigned n = (unsigned)(rows * C), quads = (n + 3) / 4;
+    const int blocks = (int)std::min((unsigned)CLS_MAX_BLOCKS, (quads + CLS_THREADS - 1) / CLS_THREADS);
+    const FocalParams fp{alpha, gamma, scale, ignore_index, use_ignore};
+    auto launch = dtype == DM_F32 ? launch_focal_from_saved<float>
+                  : dtype == DM_BF16 ? launch_focal_from_saved<dm::bf16_t> : launch_focal_from_saved<dm::half_t>;
+    launch(codes, heads, target_cls, n, (unsigned)C, (unsigned)rows, fp, grad_loss, grad_out, blocks, st);
+    return dm::check_hip(hipGetLastError(), "focal_from_saved_kernel launch");
+}
+
+extern "C" int dm_cross_entropy_saved(const void *logits, int dtype, const int64_t *target_cls, const float *weight, int64_t rows,
+                                      int C, int64_t ignore_index, float *loss_out, uint8_t *codes, int8_t *steps,
+                                      double *partials, int32_t *status, void *stream)
+{
+    int rc = check_common(logits, target_cls, rows, C, loss_out, partials, status);
+    if (rc != DM_OK) return rc;
+    if (!known(dtype) || (codes != nullptr) != (steps != nullptr)) return DM_E_INVALID_ARG;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    const unsigned blocks = ce_blocks((unsigned)rows, (unsigned)C);
+    auto launch = dtype == DM_F32 ? launch_ce_saved<float> : dtype == DM_BF16 ? launch_ce_saved<dm::bf16_t> : launch_ce_saved<dm::half_t>;
+    launch(logits, target_cls, weight, (unsigned)rows, (unsigned)C, ignore_index, codes, steps, partials, status, blocks, st);
+    rc = dm::check_hip(hipGetLastError(), "ce_saved_kernel launch");
+    if (rc != DM_OK) return rc;
+    hipLaunchKernelGGL(cls_loss_finish_kernel<false>, dim3(1), dim3(CLS_THREADS), 0, st, partials, (int)blocks, 1.0f, loss_out);
+    return dm::check_hip(hipGetLastError(), "cls_loss_finish_kernel launch");
+}
+
+extern "C" int dm_cross_entropy_from_saved(const uint8_t *codes, const int8_t *steps, int dtype, const int64_t *target_cls,
+                                           const float *weight, int64_t rows, int C, int64_t ignore_index, const float *inv_weight,
+                                           const float *grad_loss, void *grad_out, void *stream)
+{
+    const int rc = check_from_saved(codes, steps, dtype, target_cls, rows, C, grad_loss, grad_out);
+    if (rc != DM_OK) return rc;
+    if (rows == 0) return DM_OK;
+    if (!inv_weight) return DM_E_INVALID_ARG;
+    auto launch = dtype == DM_F32 ? launch_ce_from_saved<float>
+                  : dtype == DM_BF16 ? launch_ce_from_saved<dm::bf16_t> : launch_ce_from_saved<dm::half_t>;
+    launch(codes, steps, target_cls, weight, (unsigned)rows, (unsigned)C, ignore_index, inv_weight, grad_loss, grad_out,
+           ce_blocks((unsigned)rows, (unsigned)C), static_cast<hipStream_t>(stream));
+    return dm::check_hip(hipGetLastError(), "ce_from_saved_kernel launch");
+}

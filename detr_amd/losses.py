@@ -16,7 +16,14 @@ The classification loss on the dense class map (the criterion's `cls_criterion`,
     check_cls_status()                                        raises for class values the reference refuses
 
 one pass over the logits per call (loss and gradient together) instead of a dozen elementwise torch kernels
-forward and as many backward.
+forward and as many backward.  With `saved_bits=8` they keep a byte per logit for the backward pass instead of a float32
+gradient.
+
+For models whose decoder layers have expert blocks:
+
+    balance_losses(router_logits, top_k)                      balance loss, router z-loss and per-expert counts, differentiable
+    balance_loss_total(router_logits, top_k, ...)             their weighted mean over the layers, one scalar
+    expert_counts(router_logits, top_k)                       the counts alone
 
     set_losses(matcher, outputs_list, targets, n_cls, ...)    -> [(l1_loss, giou_loss, cls_loss)] per output set
 
@@ -330,26 +337,144 @@ class _CrossEntropy(torch.autograd.Function):
         return (grad * (grad_out * out[1])).view(ctx.shape), None, None, None
 
 
+def _checked_for_8_bits(logits, target_cls):
+    if not logits.is_cuda:
+        raise RuntimeError("detr_amd.losses: the classification loss runs on the GPU (there is no CPU path)")
+    if logits.dtype not in _lib.DTYPE_CODES:
+        raise TypeError(f"logits must be float32, bfloat16 or float16, got {logits.dtype}")
+    if target_cls.dtype != torch.int64 or target_cls.device != logits.device:
+        raise TypeError("target_cls must be an int64 tensor on the device of the logits")
+    if logits.dim() < 1 or tuple(logits.shape[:-1]) != tuple(target_cls.shape):
+        raise ValueError(f"logits {tuple(logits.shape)} must be target_cls {tuple(target_cls.shape)} + [C]")
+    if logits.shape[-1] < 1:
+        raise ValueError("logits of no class")
+    return logits.detach().contiguous(), target_cls.contiguous()
+
+
+class _FocalLoss8(torch.autograd.Function):
+    """`_FocalLoss` that keeps a byte per logit (and a word per 128 of them) instead of the gradient."""
+
+    @staticmethod
+    def forward(ctx, logits, target_cls, alpha, gamma, scale, ignore_index):
+        x, cls = _checked_for_8_bits(logits, target_cls)
+        device, n, C = x.device, x.numel(), int(x.shape[-1])
+        blocks = (n + 127) // 128
+        keep = ctx.needs_input_grad[0]
+        codes = torch.empty(132 * blocks, dtype=torch.uint8, device=device) if keep else None      # the bytes, then the heads
+        codes_ptr, heads_ptr = (codes.data_ptr(), codes.data_ptr() + 128 * blocks) if keep and n else (None, None)
+        partials = torch.empty(_lib.CLS_LOSS_PARTIALS, dtype=torch.float64, device=device)
+        out = torch.empty((), dtype=torch.float32, device=device)
+        call = (_lib.DTYPE_CODES[x.dtype], cls.numel(), C, alpha, gamma, scale, 0 if ignore_index is None else int(ignore_index),
+                0 if ignore_index is None else 1)
+        with ops._on(device):
+            rc = lib.dm_focal_loss_saved(x.data_ptr(), call[0], cls.data_ptr(), *call[1:], out.data_ptr(), codes_ptr, heads_ptr,
+                                         partials.data_ptr(), _status_word(device).data_ptr(),
+                                         torch.cuda.current_stream(device).cuda_stream)
+        _lib.check(rc, "dm_focal_loss_saved")
+        if keep:
+            ctx.call, ctx.shape, ctx.dtype, ctx.blocks = call, logits.shape, x.dtype, blocks
+            ctx.save_for_backward(codes, cls)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_out):
+        codes, cls = ctx.saved_tensors
+        device = codes.device
+        grad = torch.empty(ctx.shape, dtype=ctx.dtype, device=device)
+        if grad.numel():
+            with ops._on(device):
+                rc = lib.dm_focal_loss_from_saved(codes.data_ptr(), codes.data_ptr() + 128 * ctx.blocks, ctx.call[0], cls.data_ptr(),
+                                                  *ctx.call[1:], grad_out.data_ptr(), grad.data_ptr(),
+                                                  torch.cuda.current_stream(device).cuda_stream)
+            _lib.check(rc, "dm_focal_loss_from_saved")
+        return grad, None, None, None, None, None
+
+
+class _CrossEntropy8(torch.autograd.Function):
+    """`_CrossEntropy` that keeps a byte per logit (and one per row) instead of the gradient."""
+
+    @staticmethod
+    def forward(ctx, logits, target_cls, weight, ignore_index):
+        x, cls = _checked_for_8_bits(logits, target_cls)
+        device, n, C, rows = x.device, x.numel(), int(x.shape[-1]), cls.numel()
+        if weight is not None:
+            if weight.dtype != torch.float32 or weight.device != device or tuple(weight.shape) != (C,):
+                raise ValueError("weight must be a float32 [C] tensor on the device of the logits")
+            weight = weight.detach().contiguous()
+        keep = ctx.needs_input_grad[0]
+        codes = torch.empty(n + rows, dtype=torch.uint8, device=device) if keep else None          # the bytes, then the steps
+        codes_ptr, steps_ptr = (codes.data_ptr(), codes.data_ptr() + n) if keep and n else (None, None)
+        partials = torch.empty(_lib.CLS_LOSS_PARTIALS, dtype=torch.float64, device=device)
+        out = torch.empty(2, dtype=torch.float32, device=device)
+        dtype = _lib.DTYPE_CODES[x.dtype]
+        with ops._on(device):
+            rc = lib.dm_cross_entropy_saved(x.data_ptr(), dtype, cls.data_ptr(), None if weight is None else weight.data_ptr(), rows, C,
+                                            ignore_index, out.data_ptr(), codes_ptr, steps_ptr, partials.data_ptr(),
+                                            _status_word(device).data_ptr(), torch.cuda.current_stream(device).cuda_stream)
+        _lib.check(rc, "dm_cross_entropy_saved")
+        if keep:
+            ctx.call, ctx.shape, ctx.dtype, ctx.n = (dtype, rows, C, ignore_index), logits.shape, x.dtype, n
+            ctx.save_for_backward(codes, cls, out.detach(), *([] if weight is None else [weight]))
+        return out[0]
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_out):
+        codes, cls, out, *weight = ctx.saved_tensors
+        device = codes.device
+        dtype, rows, C, ignore_index = ctx.call
+        grad = torch.empty(ctx.shape, dtype=ctx.dtype, device=device)
+        if grad.numel():
+            with ops._on(device):
+                rc = lib.dm_cross_entropy_from_saved(codes.data_ptr(), codes.data_ptr() + ctx.n, dtype, cls.data_ptr(),
+                                                     weight[0].data_ptr() if weight else None, rows, C, ignore_index,
+                                                     out.data_ptr() + 4, grad_out.data_ptr(), grad.data_ptr(),
+                                                     torch.cuda.current_stream(device).cuda_stream)
+            _lib.check(rc, "dm_cross_entropy_from_saved")
+        return grad, None, None, None
+
+
+def _check_saved_bits(saved_bits):
+    if saved_bits not in (32, 8):
+        raise ValueError(f"saved_bits must be 32 or 8, got {saved_bits}")
+    return saved_bits == 8
+
+
 def focal_loss(logits: torch.Tensor, target_cls: torch.Tensor, num_boxes, alpha: float = 0.25, gamma: float = 2.0,
-               ignore_index: Optional[int] = None) -> torch.Tensor:
+               ignore_index: Optional[int] = None, saved_bits: int = 32) -> torch.Tensor:
     """`FocalLoss.forward` (/root/reference/models/detr/loss.py:198-213 with `sigmoid_focal_loss` :217-242) on
     class-last `logits [..., C]` and the class map `target_cls [...]` (C = no object): the sum of the focal terms of all
     logits divided by `num_boxes` -- the reference's `loss.mean(1).sum() / num_boxes * Q`.  `alpha < 0`: no alpha
     weighting.  `ignore_index`: rows of that class contribute nothing (with -1, the foreground selection of
-    /root/reference/models/co_detr/loss.py:153-166).  A 0-dim tensor; differentiable in `logits`."""
+    /root/reference/models/co_detr/loss.py:153-166).  A 0-dim tensor; differentiable in `logits`.
+
+    `saved_bits`: what is kept of every logit for the backward pass.  32: its float32 gradient, computed with the loss.  8: a
+    byte that stands for the logit itself -- 128 consecutive logits share a power-of-two step, 2^-16 to 2^-2 as their range
+    asks, 1/16 for a range of 8 to 15.9; logits beyond +-20 count as +-20 -- from which the backward pass computes the
+    gradient: a quarter of the memory between the passes, the same loss, and the gradient at logits that are off by at most
+    half a step.  With 8 bits the logits may also be bfloat16 or float16; their gradient is of their type."""
+    if _check_saved_bits(saved_bits):
+        return _FocalLoss8.apply(logits, target_cls, float(alpha), float(gamma), 1.0 / float(num_boxes), ignore_index)
     return _FocalLoss.apply(logits, target_cls, float(alpha), float(gamma), 1.0 / float(num_boxes), ignore_index)
 
 
 def cross_entropy(logits: torch.Tensor, target_cls: torch.Tensor, weight: Optional[torch.Tensor] = None,
-                  ignore_index: int = -100) -> torch.Tensor:
+                  ignore_index: int = -100, saved_bits: int = 32) -> torch.Tensor:
     """`CrossEntropy.forward` (/root/reference/models/detr/loss.py:185-195): `nn.CrossEntropyLoss(weight)` with the
-    default 'mean' reduction, on class-last `logits [..., C]`.  A 0-dim tensor; differentiable in `logits`."""
+    default 'mean' reduction, on class-last `logits [..., C]`.  A 0-dim tensor; differentiable in `logits`.
+
+    `saved_bits` as in `focal_loss`: with 8, a byte per logit, the logits of a row sharing a power-of-two step from 2^-16 to
+    2^-3 (1/16 for a range of 8 to 15.9; what lies further than 31.9 below the row's largest counts as 31.9 below)."""
+    if _check_saved_bits(saved_bits):
+        return _CrossEntropy8.apply(logits, target_cls, weight, int(ignore_index))
     return _CrossEntropy.apply(logits, target_cls, weight, ignore_index)
 
 
-def _takes(x, targets) -> bool:
+def _takes(x, targets, saved_bits: int = 32) -> bool:
     """Whether the kernels take these tensors as they are (anything else goes to the caller's own implementation)."""
-    return x.is_cuda and x.dtype == torch.float32 and targets.dtype == torch.int64 and targets.device == x.device
+    return x.is_cuda and (x.dtype == torch.float32 or (saved_bits == 8 and x.dtype in _lib.DTYPE_CODES)) \
+        and targets.dtype == torch.int64 and targets.device == x.device
 
 
 def _class_last(inputs, targets, C, channels_first):
@@ -374,41 +499,45 @@ class FocalLoss(torch.nn.Module):
     `forward(inputs, targets, num_boxes)` with `inputs` [B, n_cls, Q] (/root/reference/models/detr/loss.py:208-213) or
     [B, Q, n_cls] (/root/reference/models/co_detr/loss.py:272-276) -- `channels_first` says which, None tells them
     apart by their shape -- and `targets` the [B, Q] class map.  Inputs the kernel does not take (not float32, not on
-    a GPU, a layout that cannot be told) go to `fallback` when one is given."""
+    a GPU, a layout that cannot be told) go to `fallback` when one is given.  `saved_bits` as in `focal_loss`."""
 
-    def __init__(self, alpha: float, gamma: float, n_cls: int, channels_first: Optional[bool] = None, fallback=None):
+    def __init__(self, alpha: float, gamma: float, n_cls: int, channels_first: Optional[bool] = None, fallback=None,
+                 saved_bits: int = 32):
         super().__init__()
+        _check_saved_bits(saved_bits)
         self.alpha, self.gamma, self.n_cls, self.channels_first = alpha, gamma, n_cls, channels_first
-        self.fallback = fallback
+        self.fallback, self.saved_bits = fallback, saved_bits
 
     def forward(self, inputs, targets, num_boxes):
         x = _class_last(inputs, targets, self.n_cls, self.channels_first)
-        if x is None or x.shape[-1] != self.n_cls or not _takes(x, targets):
+        if x is None or x.shape[-1] != self.n_cls or not _takes(x, targets, self.saved_bits):
             if self.fallback is None:
                 raise RuntimeError("detr_amd.losses.FocalLoss: float32 GPU logits of [B, Q, n_cls] or [B, n_cls, Q] expected")
             return self.fallback(inputs, targets, num_boxes)
-        return focal_loss(x, targets, num_boxes, self.alpha, self.gamma)
+        return focal_loss(x, targets, num_boxes, self.alpha, self.gamma, saved_bits=self.saved_bits)
 
 
 class CrossEntropy(torch.nn.Module):
     """Takes the place of the reference's `CrossEntropy(weight)` (/root/reference/models/detr/loss.py:185-195, input
-    [B, C, Q]; /root/reference/models/co_detr/loss.py:249-259, input [B, Q, C])."""
+    [B, C, Q]; /root/reference/models/co_detr/loss.py:249-259, input [B, Q, C]).  `saved_bits` as in `cross_entropy`."""
 
     def __init__(self, weight: Optional[torch.Tensor] = None, channels_first: Optional[bool] = None,
-                 ignore_index: int = -100, fallback=None):
+                 ignore_index: int = -100, fallback=None, saved_bits: int = 32):
         super().__init__()
+        _check_saved_bits(saved_bits)
         self.register_buffer("weight", None if weight is None else weight.detach().clone().float())
         self.channels_first, self.ignore_index, self.fallback = channels_first, ignore_index, fallback
+        self.saved_bits = saved_bits
 
     def forward(self, inputs, targets, num_boxes=None):
         C = self.weight.shape[0] if self.weight is not None else \
             (inputs.shape[1] if self.channels_first else inputs.shape[-1] if self.channels_first is False else None)
         x = _class_last(inputs, targets, C, self.channels_first) if C is not None else None
-        if x is None or not _takes(x, targets) or (self.weight is not None and self.weight.device != x.device):
+        if x is None or not _takes(x, targets, self.saved_bits) or (self.weight is not None and self.weight.device != x.device):
             if self.fallback is None:
                 raise RuntimeError("detr_amd.losses.CrossEntropy: float32 GPU logits of [B, Q, C] or [B, C, Q] expected")
             return self.fallback(inputs, targets, num_boxes)
-        return cross_entropy(x, targets, self.weight, self.ignore_index)
+        return cross_entropy(x, targets, self.weight, self.ignore_index, self.saved_bits)
 
 
 # ---- the balance loss of expert routers ------------------------------------------------------------------------
@@ -616,7 +745,7 @@ def balance_loss_total(router_logits, top_k: int, balance_weight: float = 0.01, 
 
 
 def set_losses(matcher, outputs_list, targets, n_cls: int, cls_loss: str = "focal", focal_alpha: float = 0.25,
-               focal_gamma: float = 2.0, class_weight: Optional[torch.Tensor] = None
+               focal_gamma: float = 2.0, class_weight: Optional[torch.Tensor] = None, saved_bits: int = 32
                ) -> List[Tuple[torch.Tensor, torch.Tensor, torch.Tensor]]:
     """What the loop of the reference's `Criterion.forward` computes for its Hungarian-matched output sets
     (/root/reference/models/detr/loss.py:164-176: matcher, `calc_box_loss`, `calc_cls_loss`), for all of
@@ -625,7 +754,7 @@ def set_losses(matcher, outputs_list, targets, n_cls: int, cls_loss: str = "foca
     the pair losses of all sets, one for their class maps, one pass over each set's logits; no host synchronisation
     (`matcher.check_status()` and `check_cls_status()` raise what the reference would have raised for bad inputs).
     `cls_loss` 'ce': weighted cross entropy over n_cls + 1 classes with `class_weight` (the reference's ones with
-    `noobj_weight` last, :59-62); anything else: the focal loss over n_cls logits."""
+    `noobj_weight` last, :59-62); anything else: the focal loss over n_cls logits.  `saved_bits`: as in `focal_loss`."""
     outputs_list = list(outputs_list)
     flats = matcher.match_flat(outputs_list, targets)
     if not flats:
@@ -636,9 +765,9 @@ def set_losses(matcher, outputs_list, targets, n_cls: int, cls_loss: str = "foca
     for o, f, (l1, giou), cls_map in zip(outputs_list, flats, box, maps):
         logits = o["pred_logits"]
         if cls_loss == "ce":
-            c = cross_entropy(logits, cls_map, class_weight)
+            c = cross_entropy(logits, cls_map, class_weight, saved_bits=saved_bits)
         else:
-            c = focal_loss(logits, cls_map, max(f.num_matched, 1), focal_alpha, focal_gamma)
+            c = focal_loss(logits, cls_map, max(f.num_matched, 1), focal_alpha, focal_gamma, saved_bits=saved_bits)
         result.append((l1, giou, c))
     return result
 
@@ -681,16 +810,90 @@ class _ClsLossOfSets(torch.autograd.Function):
         return (None,) * 6 + tuple(next(scaled) if present else None for present in ctx.present)
 
 
+class _ClsLossOfSets8(torch.autograd.Function):
+    """`_ClsLossOfSets` that keeps a byte per logit instead of the gradients."""
+
+    @staticmethod
+    def forward(ctx, kind, maps, scales, alpha, gamma, weight, *logits):
+        S = len(logits)
+        checked = [_checked_for_8_bits(x, m) for x, m in zip(logits, maps)]
+        device = checked[0][0].device
+        out = torch.empty(S, 2, dtype=torch.float32, device=device)
+        if weight is not None:
+            weight = weight.detach().contiguous()
+        kept = []
+        with ops._on(device):
+            partials = torch.empty(_lib.CLS_LOSS_PARTIALS, dtype=torch.float64, device=device)
+            status, stream = _status_word(device).data_ptr(), torch.cuda.current_stream(device).cuda_stream
+            for i, (x, cls) in enumerate(checked):
+                n, C, rows, dtype = x.numel(), int(x.shape[-1]), cls.numel(), _lib.DTYPE_CODES[x.dtype]
+                data = 128 * ((n + 127) // 128) if kind == "focal" else n
+                marks = 4 * ((n + 127) // 128) if kind == "focal" else rows
+                codes, codes_ptr, marks_ptr = None, None, None
+                if ctx.needs_input_grad[6 + i] and n:
+                    codes = torch.empty(data + marks, dtype=torch.uint8, device=device)
+                    codes_ptr, marks_ptr = codes.data_ptr(), codes.data_ptr() + data
+                kept.append(codes)
+                if kind == "ce":
+                    rc = lib.dm_cross_entropy_saved(x.data_ptr(), dtype, cls.data_ptr(), None if weight is None else weight.data_ptr(),
+                                                    rows, C, -100, out.data_ptr() + 8 * i, codes_ptr, marks_ptr,
+                                                    partials.data_ptr(), status, stream)
+                else:
+                    rc = lib.dm_focal_loss_saved(x.data_ptr(), dtype, cls.data_ptr(), rows, C, alpha, gamma, scales[i], 0, 0,
+                                                 out.data_ptr() + 8 * i, codes_ptr, marks_ptr, partials.data_ptr(), status, stream)
+                _lib.check(rc, "dm_cross_entropy_saved" if kind == "ce" else "dm_focal_loss_saved")
+        ctx.call = (kind, scales, alpha, gamma, [k is not None for k in kept], [(x.shape, x.dtype) for x in logits])
+        ctx.save_for_backward(out.detach(), *[c for _, c in checked], *[k for k in kept if k is not None],
+                              *([] if weight is None else [weight]))
+        return out[:, 0]
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_losses):
+        kind, scales, alpha, gamma, present, like = ctx.call
+        out, *saved = ctx.saved_tensors
+        S = len(like)
+        maps, kept = saved[:S], iter(saved[S:S + sum(present)])
+        weight = saved[S + sum(present)].data_ptr() if len(saved) > S + sum(present) else None
+        device = out.device
+        grad_losses = grad_losses.contiguous()
+        grads = []
+        with ops._on(device):
+            stream = torch.cuda.current_stream(device).cuda_stream
+            for i, ((shape, dtype), cls) in enumerate(zip(like, maps)):
+                grad = torch.empty(shape, dtype=dtype, device=device) if ctx.needs_input_grad[6 + i] else None
+                grads.append(grad)
+                if not present[i]:
+                    continue
+                codes, n, C, code = next(kept), grad.numel(), int(shape[-1]), _lib.DTYPE_CODES[dtype]
+                upstream = grad_losses.data_ptr() + 4 * i
+                if kind == "ce":
+                    rc = lib.dm_cross_entropy_from_saved(codes.data_ptr(), codes.data_ptr() + n, code, cls.data_ptr(), weight, cls.numel(), C,
+                                                         -100, out.data_ptr() + 8 * i + 4, upstream, grad.data_ptr(), stream)
+                else:
+                    rc = lib.dm_focal_loss_from_saved(codes.data_ptr(), codes.data_ptr() + 128 * ((n + 127) // 128), code, cls.data_ptr(),
+                                                      cls.numel(), C, alpha, gamma, scales[i], 0, 0, upstream, grad.data_ptr(), stream)
+                _lib.check(rc, "dm_cross_entropy_from_saved" if kind == "ce" else "dm_focal_loss_from_saved")
+        return (None,) * 6 + tuple(grads)
+
+
 def set_loss_total(matcher, outputs_list, targets, n_cls: int, cls_loss: str = "focal", l1_weight: float = 1.0,
                    giou_weight: float = 1.0, cls_weight: float = 1.0, focal_alpha: float = 0.25, focal_gamma: float = 2.0,
-                   class_weight: Optional[torch.Tensor] = None, reduction: str = "mean") -> torch.Tensor:
+                   class_weight: Optional[torch.Tensor] = None, reduction: str = "mean", saved_bits: int = 32,
+                   router_logits: Optional[Sequence[torch.Tensor]] = None, router_top_k: int = 1, router_mask=None,
+                   balance_weight: float = 0.01, router_z_weight: float = 0.0) -> torch.Tensor:
     """`l1_weight * l1 + giou_weight * giou + cls_weight * cls` over the Hungarian-matched output sets of ONE output group
     as one scalar -- with reduction='mean' what the reference's `calc_total_loss` makes of the group's per-layer losses
     (/root/reference/models/detr/loss.py:135-158: the mean of each kind over the layers, weighted and summed) -- with
     three autograd nodes for the whole group instead of some twenty per set: the values of `set_losses`, and a step that
-    is no longer bound by the host's walk through tiny tensor operations."""
+    is no longer bound by the host's walk through tiny tensor operations.  `saved_bits`: as in `focal_loss`.
+
+    `router_logits`: for a model whose decoder layers have expert blocks, the [B, Q, E] logits of their routers; the
+    `balance_loss_total` of them (`router_top_k`, `router_mask`, `balance_weight`, `router_z_weight`, the group's
+    `reduction` over the layers) is added."""
     if reduction not in ("mean", "sum"):
         raise ValueError("reduction must be 'mean' or 'sum'")
+    eight = _check_saved_bits(saved_bits)
     outputs_list = list(outputs_list)
     flats = matcher.match_flat(outputs_list, targets)
     if not flats:
@@ -700,6 +903,10 @@ def set_loss_total(matcher, outputs_list, targets, n_cls: int, cls_loss: str = "
     box = matched_box_loss_total(outputs_list, flats, l1_weight, giou_weight, reduction=reduction)
     maps = target_class_maps(flats, n_cls)
     scales = [1.0 / float(max(f.num_matched, 1)) for f in flats]
-    cls = _ClsLossOfSets.apply("ce" if cls_loss == "ce" else "focal", maps, scales, float(focal_alpha), float(focal_gamma),
+    cls = (_ClsLossOfSets8 if eight else _ClsLossOfSets).apply("ce" if cls_loss == "ce" else "focal", maps, scales, float(focal_alpha), float(focal_gamma),
                                class_weight, *[o["pred_logits"] for o in outputs_list])
-    return box + cls.sum() * (share * cls_weight)
+    total = box + cls.sum() * (share * cls_weight)
+    if router_logits is not None:
+        total = total + balance_loss_total(router_logits, router_top_k, balance_weight, router_z_weight, mask=router_mask,
+                                           reduction=reduction)
+    return total

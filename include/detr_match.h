@@ -45,6 +45,11 @@ extern "C" {
 #define DM_ABI_VERSION 2
 #define DM_MAX_SETS_PER_LAUNCH 16
 
+/* element types of the calls that take more than one */
+#define DM_F32 0
+#define DM_BF16 1
+#define DM_F16 2
+
 /* return codes */
 #define DM_OK 0
 #define DM_E_INVALID_ARG (-1)
@@ -332,6 +337,37 @@ int dm_cross_entropy_f32(const float *logits, const int64_t *target_cls, const f
                          int32_t *status, void *stream);
 
 /*
+ * ---- The classification loss with 8 bits per logit kept for the backward pass -----------------------
+ * dm_focal_loss_f32 and dm_cross_entropy_f32 in two halves, for logits of DM_F32, DM_BF16 or DM_F16 at any alignment: the
+ * forward call writes the loss of the logits as they come and one byte per logit, the backward call the gradient (of the
+ * logits' type, rounded once) at the logits that the bytes stand for.  Blocks of logits share a step 2^e, the finest with
+ * e >= -16 for which the whole numbers q(x) = rint(x 2^-e) of the block span at most 255; a byte is
+ * min(max q - q(x), 255).  All of it is exact in float32: the bytes follow from this definition alone.
+ *   focal          blocks of 128 consecutive logits of the flat array (the last one may be shorter), clamped to +-20 first;
+ *                  e <= -2; heads[block] = max q << 8 | (e & 255); the logit is (max q - byte) 2^e
+ *   cross entropy  a block is a row, clamped to +-2^20 first; e <= -3; steps[row] = e; the logit is -byte 2^e, but for a
+ *                  constant of the row (the byte 255 stands for anything further below the largest than 31.9)
+ * e = -128: the block holds a NaN (cross entropy: the row's softmax is NaN); its gradient is NaN.
+ *   codes          device, 4-byte aligned for the focal loss: rows * C bytes rounded up to 128 there, rows * C for the
+ *                  cross entropy; NULL with heads / steps NULL: the loss alone
+ *   grad_loss      device float: the gradient of the loss
+ *   inv_weight     device float: loss_out[1] of the forward call
+ * The other arguments, the limits and the status bits are those of the calls above.
+ */
+int dm_focal_loss_saved(const void *logits, int dtype, const int64_t *target_cls, int64_t rows, int C, float alpha,
+                        float gamma, float scale, int64_t ignore_index, int use_ignore, float *loss_out,
+                        uint8_t *codes, int32_t *heads, double *partials, int32_t *status, void *stream);
+int dm_focal_loss_from_saved(const uint8_t *codes, const int32_t *heads, int dtype, const int64_t *target_cls,
+                             int64_t rows, int C, float alpha, float gamma, float scale, int64_t ignore_index,
+                             int use_ignore, const float *grad_loss, void *grad_out, void *stream);
+int dm_cross_entropy_saved(const void *logits, int dtype, const int64_t *target_cls, const float *weight,
+                           int64_t rows, int C, int64_t ignore_index, float *loss_out, uint8_t *codes,
+                           int8_t *steps, double *partials, int32_t *status, void *stream);
+int dm_cross_entropy_from_saved(const uint8_t *codes, const int8_t *steps, int dtype, const int64_t *target_cls,
+                                const float *weight, int64_t rows, int C, int64_t ignore_index,
+                                const float *inv_weight, const float *grad_loss, void *grad_out, void *stream);
+
+/*
  * ---- Balance loss of expert routers, and per-expert counts -----------------------------------------
  * For models whose decoder layers have expert blocks: from the router's logits x [B][Q][E] of every layer (a "set"; no
  * counterpart in the reference), with one group per set, or one per image of a set (per_image):
@@ -362,9 +398,6 @@ int dm_cross_entropy_f32(const float *logits, const int64_t *target_cls, const f
  * the total number of groups < 2^31 (DM_E_UNSUPPORTED beyond).  dm_balance_workspace returns a negative code for
  * arguments that the calls refuse.
  */
-#define DM_F32 0
-#define DM_BF16 1
-#define DM_F16 2
 #define DM_SCORES_SOFTMAX 0
 #define DM_SCORES_SIGMOID 1
 typedef struct {
