@@ -36,35 +36,46 @@ def _stale():
 
 HELPER_SRC = os.path.join(CSRC, "index_views.cpp")
 HELPER = os.path.join(PKG, "_index_views.so")
+NODES_SRC = os.path.join(CSRC, "loss_nodes.cpp")
+NODES = os.path.join(PKG, "_loss_nodes.so")
 
 
-def build_helper(force=False, verbose=False):
-    """The host-side helper module detr_amd._index_views (bulk creation of the per-image index views;
-    plain C++ against the torch headers, no GPU code)."""
+def build_helper(force=False, verbose=False, src=HELPER_SRC, out=HELPER, what="index_views", flags=()):
+    """A host-side module of plain C++ against the torch headers (no GPU code): detr_amd._index_views (bulk creation of the
+    per-image index views) or, through `build_nodes`, detr_amd._loss_nodes."""
     import sysconfig
 
     import torch
     from torch.utils import cpp_extension
 
     # the helper reaches into tensor internals: it is built for exactly one torch version and says which
-    stamp = ("detr_amd_index_views built for torch %s;" % torch.__version__).encode()
-    if not force and os.path.exists(HELPER) and os.path.getmtime(HELPER) >= os.path.getmtime(HELPER_SRC):
-        with open(HELPER, "rb") as f:
+    stamp = ("detr_amd_%s built for torch %s;" % (what, torch.__version__)).encode()
+    newest = max(os.path.getmtime(p) for p in (src, HEADERS[-1]))
+    if not force and os.path.exists(out) and os.path.getmtime(out) >= newest:
+        with open(out, "rb") as f:
             if stamp in f.read():
-                return HELPER
+                return out
 
     libdir = cpp_extension.library_paths()[0]
     cmd = ["g++", "-O2", "-shared", "-fPIC", "-std=c++17",
            "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI),
-           '-DDM_BUILT_FOR_TORCH="%s"' % torch.__version__]
+           '-DDM_BUILT_FOR_TORCH="%s"' % torch.__version__, *flags]
     for inc in cpp_extension.include_paths() + [sysconfig.get_paths()["include"]]:
         cmd += ["-I", inc]
-    cmd += [HELPER_SRC, "-o", HELPER, "-L", libdir, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10",
+    cmd += [src, "-o", out, "-L", libdir, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip",
             "-Wl,-rpath," + libdir]
     if verbose:
         print(" ".join(cmd))
     subprocess.check_call(cmd)
-    return HELPER
+    return out
+
+
+def build_nodes(force=False, verbose=False):
+    """detr_amd._loss_nodes: the autograd nodes of the losses (C++, so that no backward pass waits for the interpreter)."""
+    rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
+    return build_helper(force, verbose, NODES_SRC, NODES, "loss_nodes",
+                        ["-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_EXTENSION_NAME=_loss_nodes", "-I",
+                         os.path.join(ROOT, "include"), "-I", os.path.join(rocm, "include")])
 
 
 DEMO_SRC = os.path.join(ROOT, "tests", "c_abi", "abi_demo.c")
@@ -89,6 +100,7 @@ def build_demo(force=False, verbose=False):
 
 def build_library(force=False, verbose=False):
     build_helper(force=force, verbose=verbose)
+    build_nodes(force=force, verbose=verbose)
     _build_kernels(force=force, verbose=verbose)
     build_demo(force=force, verbose=verbose)
     return LIB

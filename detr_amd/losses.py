@@ -30,7 +30,7 @@ For models whose decoder layers have expert blocks:
 is the body of a criterion's loop over its Hungarian-matched output sets (loss.py:164-176) on top of all of the above:
 one matching launch for the step, nothing synchronises.
 """
-import struct
+import ctypes
 from typing import List, NamedTuple, Optional, Sequence, Tuple
 
 import torch
@@ -38,6 +38,20 @@ import torch
 from . import _lib, ops
 from ._lib import DmIndexSet, lib
 from .matcher import FlatMatches
+
+try:        # the autograd nodes written in C++ (csrc/loss_nodes.cpp, built by build_ext.py)
+    from . import _loss_nodes as _nodes
+except ImportError:
+    _nodes = None
+if _nodes is not None and _nodes.built_for_torch == torch.__version__:
+    _nodes.bind({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in _lib.EXPORTS})
+
+
+def _loss_nodes():
+    """The C++ nodes.  There is no other implementation behind the losses that use them."""
+    if _nodes is None or _nodes.built_for_torch != torch.__version__:
+        raise RuntimeError("detr_amd._loss_nodes is not built for torch %s: run `python build_ext.py`" % torch.__version__)
+    return _nodes
 
 
 def _same_launch(flats: Sequence[FlatMatches]):
@@ -235,6 +249,8 @@ _cls_status = {}         # device index -> int32 word the kernels OR their findi
 
 
 def _status_word(device):
+    if device.type != "cuda":
+        raise RuntimeError("detr_amd.losses: the losses run on the GPU (there is no CPU path)")
     index = device.index if device.index is not None else torch.cuda.current_device()
     status = _cls_status.get(index)
     if status is None:
@@ -337,104 +353,6 @@ class _CrossEntropy(torch.autograd.Function):
         return (grad * (grad_out * out[1])).view(ctx.shape), None, None, None
 
 
-def _checked_for_8_bits(logits, target_cls):
-    if not logits.is_cuda:
-        raise RuntimeError("detr_amd.losses: the classification loss runs on the GPU (there is no CPU path)")
-    if logits.dtype not in _lib.DTYPE_CODES:
-        raise TypeError(f"logits must be float32, bfloat16 or float16, got {logits.dtype}")
-    if target_cls.dtype != torch.int64 or target_cls.device != logits.device:
-        raise TypeError("target_cls must be an int64 tensor on the device of the logits")
-    if logits.dim() < 1 or tuple(logits.shape[:-1]) != tuple(target_cls.shape):
-        raise ValueError(f"logits {tuple(logits.shape)} must be target_cls {tuple(target_cls.shape)} + [C]")
-    if logits.shape[-1] < 1:
-        raise ValueError("logits of no class")
-    return logits.detach().contiguous(), target_cls.contiguous()
-
-
-class _FocalLoss8(torch.autograd.Function):
-    """`_FocalLoss` that keeps a byte per logit (and a word per 128 of them) instead of the gradient."""
-
-    @staticmethod
-    def forward(ctx, logits, target_cls, alpha, gamma, scale, ignore_index):
-        x, cls = _checked_for_8_bits(logits, target_cls)
-        device, n, C = x.device, x.numel(), int(x.shape[-1])
-        blocks = (n + 127) // 128
-        keep = ctx.needs_input_grad[0]
-        codes = torch.empty(132 * blocks, dtype=torch.uint8, device=device) if keep else None      # the bytes, then the heads
-        codes_ptr, heads_ptr = (codes.data_ptr(), codes.data_ptr() + 128 * blocks) if keep and n else (None, None)
-        partials = torch.empty(_lib.CLS_LOSS_PARTIALS, dtype=torch.float64, device=device)
-        out = torch.empty((), dtype=torch.float32, device=device)
-        call = (_lib.DTYPE_CODES[x.dtype], cls.numel(), C, alpha, gamma, scale, 0 if ignore_index is None else int(ignore_index),
-                0 if ignore_index is None else 1)
-        with ops._on(device):
-            rc = lib.dm_focal_loss_saved(x.data_ptr(), call[0], cls.data_ptr(), *call[1:], out.data_ptr(), codes_ptr, heads_ptr,
-                                         partials.data_ptr(), _status_word(device).data_ptr(),
-                                         torch.cuda.current_stream(device).cuda_stream)
-        _lib.check(rc, "dm_focal_loss_saved")
-        if keep:
-            ctx.call, ctx.shape, ctx.dtype, ctx.blocks = call, logits.shape, x.dtype, blocks
-            ctx.save_for_backward(codes, cls)
-        return out
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad_out):
-        codes, cls = ctx.saved_tensors
-        device = codes.device
-        grad = torch.empty(ctx.shape, dtype=ctx.dtype, device=device)
-        if grad.numel():
-            with ops._on(device):
-                rc = lib.dm_focal_loss_from_saved(codes.data_ptr(), codes.data_ptr() + 128 * ctx.blocks, ctx.call[0], cls.data_ptr(),
-                                                  *ctx.call[1:], grad_out.data_ptr(), grad.data_ptr(),
-                                                  torch.cuda.current_stream(device).cuda_stream)
-            _lib.check(rc, "dm_focal_loss_from_saved")
-        return grad, None, None, None, None, None
-
-
-class _CrossEntropy8(torch.autograd.Function):
-    """`_CrossEntropy` that keeps a byte per logit (and one per row) instead of the gradient."""
-
-    @staticmethod
-    def forward(ctx, logits, target_cls, weight, ignore_index):
-        x, cls = _checked_for_8_bits(logits, target_cls)
-        device, n, C, rows = x.device, x.numel(), int(x.shape[-1]), cls.numel()
-        if weight is not None:
-            if weight.dtype != torch.float32 or weight.device != device or tuple(weight.shape) != (C,):
-                raise ValueError("weight must be a float32 [C] tensor on the device of the logits")
-            weight = weight.detach().contiguous()
-        keep = ctx.needs_input_grad[0]
-        codes = torch.empty(n + rows, dtype=torch.uint8, device=device) if keep else None          # the bytes, then the steps
-        codes_ptr, steps_ptr = (codes.data_ptr(), codes.data_ptr() + n) if keep and n else (None, None)
-        partials = torch.empty(_lib.CLS_LOSS_PARTIALS, dtype=torch.float64, device=device)
-        out = torch.empty(2, dtype=torch.float32, device=device)
-        dtype = _lib.DTYPE_CODES[x.dtype]
-        with ops._on(device):
-            rc = lib.dm_cross_entropy_saved(x.data_ptr(), dtype, cls.data_ptr(), None if weight is None else weight.data_ptr(), rows, C,
-                                            ignore_index, out.data_ptr(), codes_ptr, steps_ptr, partials.data_ptr(),
-                                            _status_word(device).data_ptr(), torch.cuda.current_stream(device).cuda_stream)
-        _lib.check(rc, "dm_cross_entropy_saved")
-        if keep:
-            ctx.call, ctx.shape, ctx.dtype, ctx.n = (dtype, rows, C, ignore_index), logits.shape, x.dtype, n
-            ctx.save_for_backward(codes, cls, out.detach(), *([] if weight is None else [weight]))
-        return out[0]
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad_out):
-        codes, cls, out, *weight = ctx.saved_tensors
-        device = codes.device
-        dtype, rows, C, ignore_index = ctx.call
-        grad = torch.empty(ctx.shape, dtype=ctx.dtype, device=device)
-        if grad.numel():
-            with ops._on(device):
-                rc = lib.dm_cross_entropy_from_saved(codes.data_ptr(), codes.data_ptr() + ctx.n, dtype, cls.data_ptr(),
-                                                     weight[0].data_ptr() if weight else None, rows, C, ignore_index,
-                                                     out.data_ptr() + 4, grad_out.data_ptr(), grad.data_ptr(),
-                                                     torch.cuda.current_stream(device).cuda_stream)
-            _lib.check(rc, "dm_cross_entropy_from_saved")
-        return grad, None, None, None
-
-
 def _check_saved_bits(saved_bits):
     if saved_bits not in (32, 8):
         raise ValueError(f"saved_bits must be 32 or 8, got {saved_bits}")
@@ -455,7 +373,8 @@ def focal_loss(logits: torch.Tensor, target_cls: torch.Tensor, num_boxes, alpha:
     gradient: a quarter of the memory between the passes, the same loss, and the gradient at logits that are off by at most
     half a step.  With 8 bits the logits may also be bfloat16 or float16; their gradient is of their type."""
     if _check_saved_bits(saved_bits):
-        return _FocalLoss8.apply(logits, target_cls, float(alpha), float(gamma), 1.0 / float(num_boxes), ignore_index)
+        return _loss_nodes().focal_losses([logits], [target_cls], float(alpha), float(gamma), [1.0 / float(num_boxes)], ignore_index,
+                                          True, _status_word(logits.device))
     return _FocalLoss.apply(logits, target_cls, float(alpha), float(gamma), 1.0 / float(num_boxes), ignore_index)
 
 
@@ -467,7 +386,7 @@ def cross_entropy(logits: torch.Tensor, target_cls: torch.Tensor, weight: Option
     `saved_bits` as in `focal_loss`: with 8, a byte per logit, the logits of a row sharing a power-of-two step from 2^-16 to
     2^-3 (1/16 for a range of 8 to 15.9; what lies further than 31.9 below the row's largest counts as 31.9 below)."""
     if _check_saved_bits(saved_bits):
-        return _CrossEntropy8.apply(logits, target_cls, weight, int(ignore_index))
+        return _loss_nodes().cross_entropies([logits], [target_cls], weight, int(ignore_index), True, _status_word(logits.device))
     return _CrossEntropy.apply(logits, target_cls, weight, ignore_index)
 
 
@@ -550,17 +469,6 @@ class BalanceLosses(NamedTuple):
     counts: torch.Tensor
 
 
-_ROUTER_SET = struct.Struct("=4Qq2i")          # DmRouterSet
-
-
-def _router_sets(tensors, masks, experts, grads=None) -> bytes:
-    """The DmRouterSet records of a call."""
-    return b"".join(
-        _ROUTER_SET.pack(x.data_ptr(), 0 if m is None else m.data_ptr(), 0 if e is None else e.data_ptr(),
-                         0 if g is None else g.data_ptr(), ops.image_stride(x), x.shape[1], 0)
-        for x, m, e, g in zip(tensors, masks, experts, grads or [None] * len(tensors)))
-
-
 def _per_set(value, n, what):
     """`value` for each of n sets: None, one tensor for all of them, or a list of n."""
     if value is None or isinstance(value, torch.Tensor):
@@ -571,110 +479,13 @@ def _per_set(value, n, what):
     return value
 
 
-def _checked_routers(router_logits, top_k, mask, experts):
-    """(logits, masks, experts) per set, as the kernels read them."""
+def _router_arguments(router_logits, top_k):
     logits = [router_logits] if isinstance(router_logits, torch.Tensor) else list(router_logits)
     if not logits:
         raise ValueError("no router logits")
-    first = logits[0]
-    if not first.is_cuda:
-        raise RuntimeError("detr_amd.losses: the balance loss runs on the GPU (there is no CPU path)")
-    if first.dtype not in _lib.DTYPE_CODES:
-        raise TypeError(f"router logits must be float32, bfloat16 or float16, got {first.dtype}")
-    if first.dim() != 3:
-        raise ValueError(f"router logits must be [B, Q, E], got {tuple(first.shape)}")
-    B, E = int(first.shape[0]), int(first.shape[2])
-    if E < 1:
-        raise ValueError("router logits for no expert")
-    if not isinstance(top_k, int) or top_k < 1 or (experts is None and top_k > E):
-        raise ValueError(f"top_k must be a whole number from 1 to the number of experts ({E}), got {top_k}")
-    masks, experts = _per_set(mask, len(logits), "mask"), _per_set(experts, len(logits), "experts")
-    for i, x in enumerate(logits):
-        if x.dtype != first.dtype or x.device != first.device:
-            raise TypeError("the router logits of a call must share their type and device")
-        if x.dim() != 3 or x.shape[0] != B or x.shape[2] != E:
-            raise ValueError("the router logits of a call must be [B, Q, E] with the same B and E")
-        x = x.detach()
-        logits[i] = x if ops.image_stride(x) is not None else x.contiguous()
-        m, e = masks[i], experts[i]
-        if m is not None:
-            if m.dtype != torch.bool or m.device != x.device:
-                raise TypeError("mask must be a bool tensor on the device of the router logits")
-            if tuple(m.shape) != (B, x.shape[1]):
-                raise ValueError(f"mask must be [B, Q] = {(B, int(x.shape[1]))}, got {tuple(m.shape)}")
-            masks[i] = m.contiguous()
-        if e is not None:
-            if e.dtype != torch.int64 or e.device != x.device:
-                raise TypeError("experts must be an int64 tensor on the device of the router logits")
-            if tuple(e.shape) != (B, x.shape[1], top_k):
-                raise ValueError(f"experts must be [B, Q, top_k] = {(B, int(x.shape[1]), top_k)}, got {tuple(e.shape)}")
-            experts[i] = e.contiguous()
-        elif i and experts[0] is not None:
-            raise ValueError("experts for all sets of the call or for none")
-    if experts[0] is None and any(e is not None for e in experts):
-        raise ValueError("experts for all sets of the call or for none")
-    return logits, masks, experts
-
-
-def _router_workspace(sets, S, B, E, per_image, device):
-    need = lib.dm_balance_workspace(sets, S, B, E, per_image)
-    if need < 0:
-        _lib.check(need, "dm_balance_workspace")
-    return torch.empty(need, dtype=torch.uint8, device=device)
-
-
-def _groups(S, B, per_image):
-    return (S, B) if per_image else (S,)
-
-
-class _BalanceLosses(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, checked, top_k, given_counts, sigmoid, per_image, *router_logits):
-        logits, masks, experts = checked
-        first = logits[0]
-        device, S, B, E = first.device, len(logits), int(first.shape[0]), int(first.shape[2])
-        groups = _groups(S, B, per_image)
-        n = S * B if per_image else S
-        dtype = _lib.DTYPE_CODES[first.dtype]
-        balance = torch.empty(groups, dtype=torch.float32, device=device)
-        z = None if sigmoid else torch.empty(groups, dtype=torch.float32, device=device)
-        counts = torch.empty(groups + (E,), dtype=torch.int64, device=device)
-        kept = torch.empty(n * (E + 1), dtype=torch.float32, device=device)          # slope [n, E], then inv_rows [n]
-        sets = _router_sets(logits, masks, experts)
-        with ops._on(device):
-            workspace = _router_workspace(sets, S, B, E, per_image, device)
-            rc = lib.dm_balance_loss(sets, S, B, E, top_k, dtype, sigmoid, per_image,
-                                     None if given_counts is None else given_counts.data_ptr(), balance.data_ptr(),
-                                     None if z is None else z.data_ptr(), counts.data_ptr(), kept.data_ptr(),
-                                     kept.data_ptr() + 4 * n * E, workspace.data_ptr(), workspace.numel(),
-                                     _status_word(device).data_ptr(), torch.cuda.current_stream(device).cuda_stream)
-        _lib.check(rc, "dm_balance_loss")
-        ctx.call = (dtype, sigmoid, per_image, [m is not None for m in masks])
-        ctx.save_for_backward(kept, *logits, *[m for m in masks if m is not None])
-        ctx.mark_non_differentiable(counts)
-        ctx.set_materialize_grads(False)
-        return balance, z, counts
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad_balance, grad_z, _):
-        dtype, sigmoid, per_image, masked = ctx.call
-        kept, *rest = ctx.saved_tensors
-        S = len(masked)
-        logits, rest = rest[:S], iter(rest[S:])
-        if grad_balance is None and grad_z is None:
-            return (None,) * (5 + S)
-        device, B, E = kept.device, int(logits[0].shape[0]), int(logits[0].shape[2])
-        n = S * B if per_image else S
-        grads = [torch.empty(x.shape, dtype=x.dtype, device=device) for x in logits]
-        gb, gz = (None if g is None else g.contiguous() for g in (grad_balance, grad_z))
-        sets = _router_sets(logits, [next(rest) if m else None for m in masked], [None] * S, grads)
-        with ops._on(device):
-            rc = lib.dm_balance_backward(sets, S, B, E, dtype, sigmoid, per_image, kept.data_ptr(), kept.data_ptr() + 4 * n * E,
-                                         None if gb is None else gb.data_ptr(), None if gz is None else gz.data_ptr(),
-                                         torch.cuda.current_stream(device).cuda_stream)
-        _lib.check(rc, "dm_balance_backward")
-        return (None,) * 5 + tuple(g if need else None for g, need in zip(grads, ctx.needs_input_grad[5:]))
+    if not isinstance(top_k, int):
+        raise ValueError(f"top_k must be a whole number, got {top_k}")
+    return logits
 
 
 def balance_losses(router_logits, top_k: int, mask=None, experts=None, counts: Optional[torch.Tensor] = None,
@@ -697,34 +508,17 @@ def balance_losses(router_logits, top_k: int, mask=None, experts=None, counts: O
     through P and z (the counts are constants); rounded once to the logits' type."""
     if scores not in ("softmax", "sigmoid"):
         raise ValueError("scores must be 'softmax' or 'sigmoid'")
-    router_logits = [router_logits] if isinstance(router_logits, torch.Tensor) else list(router_logits)
-    checked = _checked_routers(router_logits, top_k, mask, experts)
-    if counts is not None:
-        first = checked[0][0]
-        want = _groups(len(router_logits), int(first.shape[0]), per_image) + (int(first.shape[2]),)
-        if counts.dtype != torch.int64 or counts.device != first.device:
-            raise TypeError("counts must be an int64 tensor on the device of the router logits")
-        if tuple(counts.shape) != want:
-            raise ValueError(f"counts must be {want}, got {tuple(counts.shape)}")
-        counts = counts.contiguous()
-    return BalanceLosses(*_BalanceLosses.apply(checked, top_k, counts, int(scores == "sigmoid"), int(per_image), *router_logits))
+    logits = _router_arguments(router_logits, top_k)
+    n = len(logits)
+    return BalanceLosses(*_loss_nodes().balance_losses(logits, top_k, _per_set(mask, n, "mask"), _per_set(experts, n, "experts"), counts,
+                                                       scores == "sigmoid", bool(per_image), _status_word(logits[0].device)))
 
 
-@torch.no_grad()
 def expert_counts(router_logits, top_k: int, mask=None, per_image: bool = False) -> torch.Tensor:
     """The counts of `balance_losses` alone, int64 [S, E] (or [S, B, E]): one pass that takes no exponentials."""
-    logits, masks, experts = _checked_routers(router_logits, top_k, mask, None)
-    first = logits[0]
-    device, S, B, E = first.device, len(logits), int(first.shape[0]), int(first.shape[2])
-    counts = torch.empty(_groups(S, B, per_image) + (E,), dtype=torch.int64, device=device)
-    sets = _router_sets(logits, masks, experts)
-    with ops._on(device):
-        workspace = _router_workspace(sets, S, B, E, int(per_image), device)
-        rc = lib.dm_expert_counts(sets, S, B, E, top_k, _lib.DTYPE_CODES[first.dtype], int(per_image), counts.data_ptr(),
-                                  workspace.data_ptr(), workspace.numel(), _status_word(device).data_ptr(),
-                                  torch.cuda.current_stream(device).cuda_stream)
-    _lib.check(rc, "dm_expert_counts")
-    return counts
+    logits = _router_arguments(router_logits, top_k)
+    return _loss_nodes().expert_counts(logits, top_k, _per_set(mask, len(logits), "mask"), bool(per_image),
+                                       _status_word(logits[0].device))
 
 
 def balance_loss_total(router_logits, top_k: int, balance_weight: float = 0.01, z_weight: float = 0.0, mask=None, experts=None,
@@ -810,73 +604,6 @@ class _ClsLossOfSets(torch.autograd.Function):
         return (None,) * 6 + tuple(next(scaled) if present else None for present in ctx.present)
 
 
-class _ClsLossOfSets8(torch.autograd.Function):
-    """`_ClsLossOfSets` that keeps a byte per logit instead of the gradients."""
-
-    @staticmethod
-    def forward(ctx, kind, maps, scales, alpha, gamma, weight, *logits):
-        S = len(logits)
-        checked = [_checked_for_8_bits(x, m) for x, m in zip(logits, maps)]
-        device = checked[0][0].device
-        out = torch.empty(S, 2, dtype=torch.float32, device=device)
-        if weight is not None:
-            weight = weight.detach().contiguous()
-        kept = []
-        with ops._on(device):
-            partials = torch.empty(_lib.CLS_LOSS_PARTIALS, dtype=torch.float64, device=device)
-            status, stream = _status_word(device).data_ptr(), torch.cuda.current_stream(device).cuda_stream
-            for i, (x, cls) in enumerate(checked):
-                n, C, rows, dtype = x.numel(), int(x.shape[-1]), cls.numel(), _lib.DTYPE_CODES[x.dtype]
-                data = 128 * ((n + 127) // 128) if kind == "focal" else n
-                marks = 4 * ((n + 127) // 128) if kind == "focal" else rows
-                codes, codes_ptr, marks_ptr = None, None, None
-                if ctx.needs_input_grad[6 + i] and n:
-                    codes = torch.empty(data + marks, dtype=torch.uint8, device=device)
-                    codes_ptr, marks_ptr = codes.data_ptr(), codes.data_ptr() + data
-                kept.append(codes)
-                if kind == "ce":
-                    rc = lib.dm_cross_entropy_saved(x.data_ptr(), dtype, cls.data_ptr(), None if weight is None else weight.data_ptr(),
-                                                    rows, C, -100, out.data_ptr() + 8 * i, codes_ptr, marks_ptr,
-                                                    partials.data_ptr(), status, stream)
-                else:
-                    rc = lib.dm_focal_loss_saved(x.data_ptr(), dtype, cls.data_ptr(), rows, C, alpha, gamma, scales[i], 0, 0,
-                                                 out.data_ptr() + 8 * i, codes_ptr, marks_ptr, partials.data_ptr(), status, stream)
-                _lib.check(rc, "dm_cross_entropy_saved" if kind == "ce" else "dm_focal_loss_saved")
-        ctx.call = (kind, scales, alpha, gamma, [k is not None for k in kept], [(x.shape, x.dtype) for x in logits])
-        ctx.save_for_backward(out.detach(), *[c for _, c in checked], *[k for k in kept if k is not None],
-                              *([] if weight is None else [weight]))
-        return out[:, 0]
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad_losses):
-        kind, scales, alpha, gamma, present, like = ctx.call
-        out, *saved = ctx.saved_tensors
-        S = len(like)
-        maps, kept = saved[:S], iter(saved[S:S + sum(present)])
-        weight = saved[S + sum(present)].data_ptr() if len(saved) > S + sum(present) else None
-        device = out.device
-        grad_losses = grad_losses.contiguous()
-        grads = []
-        with ops._on(device):
-            stream = torch.cuda.current_stream(device).cuda_stream
-            for i, ((shape, dtype), cls) in enumerate(zip(like, maps)):
-                grad = torch.empty(shape, dtype=dtype, device=device) if ctx.needs_input_grad[6 + i] else None
-                grads.append(grad)
-                if not present[i]:
-                    continue
-                codes, n, C, code = next(kept), grad.numel(), int(shape[-1]), _lib.DTYPE_CODES[dtype]
-                upstream = grad_losses.data_ptr() + 4 * i
-                if kind == "ce":
-                    rc = lib.dm_cross_entropy_from_saved(codes.data_ptr(), codes.data_ptr() + n, code, cls.data_ptr(), weight, cls.numel(), C,
-                                                         -100, out.data_ptr() + 8 * i + 4, upstream, grad.data_ptr(), stream)
-                else:
-                    rc = lib.dm_focal_loss_from_saved(codes.data_ptr(), codes.data_ptr() + 128 * ((n + 127) // 128), code, cls.data_ptr(),
-                                                      cls.numel(), C, alpha, gamma, scales[i], 0, 0, upstream, grad.data_ptr(), stream)
-                _lib.check(rc, "dm_cross_entropy_from_saved" if kind == "ce" else "dm_focal_loss_from_saved")
-        return (None,) * 6 + tuple(grads)
-
-
 def set_loss_total(matcher, outputs_list, targets, n_cls: int, cls_loss: str = "focal", l1_weight: float = 1.0,
                    giou_weight: float = 1.0, cls_weight: float = 1.0, focal_alpha: float = 0.25, focal_gamma: float = 2.0,
                    class_weight: Optional[torch.Tensor] = None, reduction: str = "mean", saved_bits: int = 32,
@@ -903,8 +630,15 @@ def set_loss_total(matcher, outputs_list, targets, n_cls: int, cls_loss: str = "
     box = matched_box_loss_total(outputs_list, flats, l1_weight, giou_weight, reduction=reduction)
     maps = target_class_maps(flats, n_cls)
     scales = [1.0 / float(max(f.num_matched, 1)) for f in flats]
-    cls = (_ClsLossOfSets8 if eight else _ClsLossOfSets).apply("ce" if cls_loss == "ce" else "focal", maps, scales, float(focal_alpha), float(focal_gamma),
-                               class_weight, *[o["pred_logits"] for o in outputs_list])
+    logits = [o["pred_logits"] for o in outputs_list]
+    if not eight:
+        cls = _ClsLossOfSets.apply("ce" if cls_loss == "ce" else "focal", maps, scales, float(focal_alpha), float(focal_gamma),
+                                   class_weight, *logits)
+    elif cls_loss == "ce":
+        cls = _loss_nodes().cross_entropies(logits, maps, class_weight, -100, False, _status_word(logits[0].device))
+    else:
+        cls = _loss_nodes().focal_losses(logits, maps, float(focal_alpha), float(focal_gamma), scales, None, False,
+                                         _status_word(logits[0].device))
     total = box + cls.sum() * (share * cls_weight)
     if router_logits is not None:
         total = total + balance_loss_total(router_logits, router_top_k, balance_weight, router_z_weight, mask=router_mask,

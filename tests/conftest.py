@@ -13,7 +13,8 @@ def pytest_configure(config):
     # a fresh checkout has no built library yet (it is git-ignored): build it once, where hipcc exists
     lib = os.path.join(ROOT, "detr_amd", "libdetr_match.so")
     helper = os.path.join(ROOT, "detr_amd", "_index_views.so")
-    if (not os.path.exists(lib) or not os.path.exists(helper)) and not os.environ.get("DETR_AMD_LIB"):
+    nodes = os.path.join(ROOT, "detr_amd", "_loss_nodes.so")
+    if not all(os.path.exists(f) for f in (lib, helper, nodes)) and not os.environ.get("DETR_AMD_LIB"):
         import shutil
 
         if shutil.which("hipcc") or os.path.exists("/opt/rocm/bin/hipcc"):
