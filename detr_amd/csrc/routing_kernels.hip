@@ -19,7 +19,6 @@ namespace {
 constexpr int RT_THREADS = 256;
 constexpr int RT_WAVES = RT_THREADS / 64;
 constexpr int RT_MAX_EXPERTS = 1024;
-constexpr int FINISH_THREADS = 1024;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 // One set as the kernels see it: `images` images of Q rows (a contiguous set asked for as one group is one image of B * Q
@@ -58,18 +57,6 @@ __device__ __forceinline__ Place place_of(const RouterSets &a, unsigned block)
     return Place{set, image, row0, row0 < s.Q ? min(s.chunk_rows, s.Q - row0) : 0u};
 }
 
-// Order of the logits as an unsigned key; 0 for those that are never chosen (-infinity, NaN).  -0 counts as +0.
-__device__ __forceinline__ unsigned order_key(float x)
-{
-    const unsigned u = __float_as_uint(x + 0.0f);
-    const unsigned key = u ^ ((unsigned)((int)u >> 31) | 0x80000000u);
-    return x > -__builtin_huge_valf() ? key : 0u;
-}
-__device__ __forceinline__ float value_of_key(unsigned key)
-{
-    return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
-}
-
 // The scores of a row before they are divided by their sum, and what turns them into p: w_e / sum w.
 // Sigmoid: sigmoid(x) times a constant of the row that keeps the largest from underflowing: with c = min(max x, 0),
 // t = exp(-|x| - c), sigmoid(x) exp(-c) = (x >= 0 ? 1 : t) / (1 + t exp(c)).  `rest` = 1 - sigmoid(x).
@@ -82,23 +69,52 @@ __device__ __forceinline__ float sigmoid_weight(float x, float c, float exp_c, f
     return (x >= 0.0f ? 1.0f : t) * r;
 }
 
-template <typename T, int NQ, int L, bool COUNT_ONLY>
-__global__ __launch_bounds__(RT_THREADS) void router_forward_kernel(const RouterSets a, const int sigmoid, unsigned *__restrict__ slots,
-                                                                    int32_t *__restrict__ status)
+// What the choice compares.  float32: the logits, with what is never chosen at -infinity.  16-bit logits are equal to one
+// another often, and equal ones are to go to the lowest index: as float32 their low 13 or 16 bits are zero, so the expert's
+// number goes into the low ten (1023 - e for positive logits, e for negative ones, where a longer mantissa means smaller).  No
+// two are equal then, and the order is that of (logit, lowest index).  +infinity becomes a number that is larger than any.
+constexpr unsigned ABOVE_ALL = 0x7F7F8000u;
+__device__ __forceinline__ float order_f32(float x) { return x > -__builtin_huge_valf() ? x : -__builtin_huge_valf(); }
+__device__ __forceinline__ float order_16(float x, unsigned e)
+{
+    const float finite = __builtin_amdgcn_fmed3f(x + 0.0f, -__builtin_huge_valf(), __uint_as_float(ABOVE_ALL));      // (-0 is +0)
+    const unsigned u = __float_as_uint(finite);
+    const unsigned low = (1023u - e) ^ ((unsigned)((int)u >> 31) & 1023u);
+    return x > -__builtin_huge_valf() ? __uint_as_float(u | low) : -__builtin_huge_valf();
+}
+__device__ __forceinline__ float logit_of_order_16(float y)
+{
+    const float x = __uint_as_float(__float_as_uint(y) & ~1023u);
+    return x == __uint_as_float(ABOVE_ALL) ? __builtin_huge_valf() : (y == -__builtin_huge_valf() ? y : x);
+}
+
+// K: the longest list of largest logits that a lane keeps (k <= K), or 0: k of any size, in rounds over all logits.
+//
+// The choice.  A lane inserts its logits into a sorted list of its K largest, one instruction per place (the new place i is
+// the median of the old i - 1, the old i and the logit); then k times the largest head of the row's lanes is taken off its
+// list, and the last one taken, T, is the row's k-th largest: the experts with a logit of at least T are the chosen ones.
+// Where equal logits lie across the border, or T came out too low because equal heads went together, more than k are: those
+// rows are chosen again, one by one (float32 only, 16-bit logits are made unequal).  k rounds over all logits, each a
+// comparison, a selection and a maximum, take 2.5 k instructions per logit instead of k.
+template <int NQ, int L, int K, bool WIDE, bool COUNT_ONLY>
+__global__ __launch_bounds__(RT_THREADS) void router_forward_kernel(const RouterSets a, const int dtype, const int sigmoid,
+                                                                    unsigned *__restrict__ slots, int32_t *__restrict__ status)
 {
     constexpr int N = 4 * NQ;                                  // logits of a row per lane
-    __shared__ unsigned hist[RT_MAX_EXPERTS];
-    __shared__ float psum_lds[COUNT_ONLY ? 1 : RT_WAVES][COUNT_ONLY ? 1 : RT_MAX_EXPERTS];
+    constexpr int PARTS = L <= 16 ? 4 : 64 / L;                // partial sums of p that a wave leaves
+    constexpr unsigned WIDTH = N * L;                          // E, rounded up to what the lanes hold
+    __shared__ unsigned hist[WIDTH];
+    __shared__ float psum_lds[COUNT_ONLY ? 1 : RT_WAVES * PARTS][COUNT_ONLY ? 1 : WIDTH];
     __shared__ double z_lds[RT_WAVES];
     __shared__ unsigned n_lds[RT_WAVES];
     const unsigned E = a.E, k = a.k;
     const float ninf = -__builtin_huge_valf();
-    for (unsigned e = threadIdx.x; e < E; e += RT_THREADS) hist[e] = 0;
+    for (unsigned e = threadIdx.x; e < WIDTH; e += RT_THREADS) hist[e] = 0;
     __syncthreads();
 
     const Place at = place_of(a, blockIdx.x);
     const RouterSetK &set = a.s[at.set];
-    const T *base = static_cast<const T *>(set.logits) + (size_t)at.image * (size_t)set.image_stride;
+    const size_t image_at = (size_t)at.image * (size_t)set.image_stride;
     const size_t image_row = (size_t)at.image * set.Q;
     const unsigned lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const unsigned sub = lane & (L - 1);
@@ -110,116 +126,182 @@ __global__ __launch_bounds__(RT_THREADS) void router_forward_kernel(const Router
     bool bad = false;
 
     // (every lane makes the same trips: the reductions need all lanes of a row's group)
+    const unsigned local = threadIdx.x / L;
+    dm::RawRow<NQ, WIDE> next;
+    uint8_t next_counts = 1;
+    auto fetch = [&](unsigned r) {
+        const size_t row = (size_t)at.row0 + (r < at.rows ? r : 0);
+        next = dm::fetch_row<NQ, L, WIDE>(set.logits, image_at + row * E, sub, E);
+        if (set.mask) next_counts = set.mask[image_row + row];
+    };
+    if (at.rows) fetch(local);
     for (unsigned r0 = 0; r0 < at.rows; r0 += ROWS) {
-        const unsigned r = r0 + threadIdx.x / L;
+        const unsigned r = r0 + local;
         const bool there = r < at.rows;
         const size_t row = (size_t)at.row0 + (there ? r : 0);
-        const bool wanted = there && (!set.mask || set.mask[image_row + row] != 0);
+        const dm::RawRow<NQ, WIDE> raw = next;
+        const bool counts = there && next_counts != 0;
+        if (r0 + ROWS < at.rows) fetch(r + ROWS);
         float x[N];
-        unsigned key[N];
-        unsigned top = 0;
-        bool any_nan = false;
+        dm::row_values<NQ, L, WIDE>(raw, dtype, sub, E, ninf, x);
+        if (!counts) {
 #pragma unroll
-        for (int q = 0; q < NQ; ++q) {
-            float v[4] = {ninf, ninf, ninf, ninf};
-            if (wanted) dm::load_quad(base + row * E, 4 * (q * L + sub), E, ninf, v);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                x[4 * q + j] = v[j];
-                key[4 * q + j] = order_key(v[j]);
-                top = max(top, key[4 * q + j]);
-                any_nan |= v[j] != v[j];
-            }
+            for (int j = 0; j < N; ++j) x[j] = ninf;
         }
-        top = dm::over_group<L>(top, dm::Max());
+        // the order, its largest, and whether the row counts
+        float y[N];
+        if (WIDE) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) y[j] = order_f32(x[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; ++j) y[j] = order_16(x[j], 4 * ((j >> 2) * L + sub) + (j & 3));
+        }
+        float list[K ? K : 1];
+#pragma unroll
+        for (int i = 0; i < (K ? K : 1); ++i) list[i] = ninf;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+#pragma unroll
+            for (int i = (K ? K : 1) - 1; i >= 1; --i) list[i] = __builtin_amdgcn_fmed3f(list[i - 1], list[i], y[j]);
+            list[0] = __builtin_amdgcn_fmed3f(list[0], y[j], __builtin_huge_valf());
+        }
+        const float top = dm::largest<L>(list[0]);
         bool live;
         if (!COUNT_ONLY) {
-            const float mx = top ? value_of_key(top) : 0.0f;
-            const float c = fminf(mx, 0.0f), exp_c = __builtin_amdgcn_exp2f(c * LOG2E);
-            float sum = 0.0f, rest;
+            float mx = WIDE ? top : logit_of_order_16(top);
+            mx = top == ninf ? 0.0f : mx;
+            float sum = 0.0f;
+            if (sigmoid) {
+                const float c = fminf(mx, 0.0f), exp_c = __builtin_amdgcn_exp2f(c * LOG2E);
 #pragma unroll
-            for (int j = 0; j < N; ++j) {
-                x[j] = sigmoid ? (x[j] == ninf ? 0.0f : sigmoid_weight(x[j], c, exp_c, &rest)) : softmax_weight(x[j], mx);
-                sum += x[j];
+                for (int j = 0; j < N; ++j) {
+                    float rest;
+                    x[j] = x[j] == ninf ? 0.0f : sigmoid_weight(x[j], c, exp_c, &rest);
+                    sum += x[j];
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < N; ++j) {
+                    x[j] = softmax_weight(x[j], mx);
+                    sum += x[j];
+                }
             }
             sum = dm::over_group<L>(sum, dm::Add());
             live = sum != 0.0f;                                // (a NaN makes it NaN)
             const float inv = live ? __builtin_amdgcn_rcpf(sum) : 0.0f;
 #pragma unroll
-            for (int j = 0; j < N; ++j) psum[j] += x[j] * inv;
+            for (int j = 0; j < N; ++j) psum[j] = __builtin_fmaf(x[j], inv, psum[j]);
             if (live && sub == 0) {
                 const float lse = mx + __builtin_amdgcn_logf(sum) * LN2;
                 z += lse * lse;
                 ++n;
             }
         } else {
-            live = dm::over_group<L>((unsigned)(top != 0 || any_nan), dm::Max()) != 0;
+            live = true;                                       // (a row with nothing but -infinity and NaN chooses nothing)
         }
-        if (set.experts) {
+        if (!COUNT_ONLY && set.experts) {
             if (live)
                 for (unsigned j = sub; j < k; j += L) {
                     const int64_t e = set.experts[(image_row + row) * k + j];
                     if (e >= 0 && e < (int64_t)E) atomicAdd(&hist[(unsigned)e], 1u);
                     else bad |= e != -1;
                 }
-        } else {
-            // k times the largest key that is left, of the lowest expert that has it
-            for (unsigned i = 0; i < k; ++i) {
-                unsigned best = 0;
+            continue;
+        }
+        bool again = K == 0;
+        if (K) {
+            float last = ninf;
+            if (L == 1) {
 #pragma unroll
-                for (int j = 0; j < N; ++j) best = max(best, key[j]);
-                best = dm::over_group<L>(best, dm::Max());
+                for (int i = 0; i < K; ++i) last = i + 1 == (int)k ? list[i] : last;
+            } else {
+                last = top;
+#pragma unroll
+                for (int i = 1; i < K; ++i) {
+                    if (i < (int)k) {
+                        // (the median of a place, the next and -infinity is the next, of +infinity the place itself)
+                        const float gone = list[0] == last ? ninf : __builtin_huge_valf();
+#pragma unroll
+                        for (int j = 0; j + 1 < K; ++j) list[j] = __builtin_amdgcn_fmed3f(list[j], list[j + 1], gone);
+                        list[K - 1] = __builtin_amdgcn_fmed3f(list[K - 1], ninf, gone);
+                        last = dm::largest<L>(list[0]);
+                    }
+                }
+            }
+            last = __builtin_amdgcn_fmed3f(last, -__FLT_MAX__, __builtin_huge_valf());       // (fewer than k: all that can be)
+            if (WIDE) {
+                unsigned chosen = 0;
+#pragma unroll
+                for (int j = 0; j < N; ++j) chosen += y[j] >= last ? 1u : 0u;
+                chosen = dm::over_group<L>(chosen, dm::Add());
+                again = __any(chosen > k);
+            }
+            if (!again) {
+#pragma unroll
+                for (int j = 0; j < N; ++j) cnt[j] += y[j] >= last ? 1u : 0u;
+            }
+        }
+        if (again) {
+            // k times the largest that is left, of the lowest expert that has it
+            for (unsigned i = 0; i < k; ++i) {
+                float best = y[0];
+#pragma unroll
+                for (int j = 1; j < N; ++j) best = __builtin_amdgcn_fmed3f(best, y[j], __builtin_huge_valf());
+                best = dm::largest<L>(best);
                 unsigned first = 0xFFFFFFFFu;
 #pragma unroll
                 for (int j = N - 1; j >= 0; --j)
-                    if (key[j] == best) first = (unsigned)(4 * ((j >> 2) * L + sub) + (j & 3));
+                    if (y[j] == best) first = (unsigned)(4 * ((j >> 2) * L + sub) + (j & 3));
                 first = dm::over_group<L>(first, dm::Min());
 #pragma unroll
                 for (int j = 0; j < N; ++j) {
-                    const bool hit = best != 0 && first == (unsigned)(4 * ((j >> 2) * L + sub) + (j & 3));
+                    const bool hit = best != ninf && first == (unsigned)(4 * ((j >> 2) * L + sub) + (j & 3));
                     cnt[j] += hit ? 1u : 0u;
-                    key[j] = hit ? 0u : key[j];
+                    y[j] = hit ? ninf : y[j];
                 }
             }
         }
     }
     if (bad) dm::raise_status(status, DM_ST_LABEL_RANGE);
 
-    // the wave's rows, then the waves in index order
+    // the rows of a wave whose lanes are 16 apart or more leave a part each; the parts are added in order
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-#pragma unroll
-        for (int off = L; off < 64; off <<= 1) {
-            if (!COUNT_ONLY) psum[j] += __shfl_xor(psum[j], off);
-            cnt[j] += __shfl_xor(cnt[j], off);
-        }
         const unsigned e = 4 * ((j >> 2) * L + sub) + (j & 3);
-        if (lane < L && e < E) {
-            if (!COUNT_ONLY) psum_lds[wave][e] = psum[j];
+        if (L <= 16) {
+            cnt[j] = dm::over_row16<L>(cnt[j]);
+            if (!COUNT_ONLY) psum[j] = dm::over_row16<L>(psum[j]);
+        }
+        if ((lane & 15) < L || L > 16) {
+            if (!COUNT_ONLY) psum_lds[wave * PARTS + lane / (L <= 16 ? 16 : L)][e] = psum[j];
             if (cnt[j]) atomicAdd(&hist[e], cnt[j]);
         }
     }
     double zd = z;
+    if (!COUNT_ONLY) {
 #pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) {
-        zd += __shfl_xor(zd, off);
-        n += __shfl_xor(n, off);
-    }
-    if (lane == 0) {
-        z_lds[wave] = zd;
-        n_lds[wave] = n;
+        for (int off = 32; off >= 1; off >>= 1) {
+            zd += __shfl_xor(zd, off);
+            n += __shfl_xor(n, off);
+        }
+        if (lane == 0) {
+            z_lds[wave] = zd;
+            n_lds[wave] = n;
+        }
     }
     __syncthreads();
     unsigned *slot = slots + (size_t)blockIdx.x * slot_words(E);
     for (unsigned e = threadIdx.x; e < E; e += RT_THREADS) {
         if (!COUNT_ONLY) {
             float s = psum_lds[0][e];
-            for (int w = 1; w < RT_WAVES; ++w) s += psum_lds[w][e];
+#pragma unroll
+            for (int w = 1; w < RT_WAVES * PARTS; ++w) s += psum_lds[w][e];
             slot[e] = __float_as_uint(s);
         }
         slot[E + e] = hist[e];
     }
-    if (threadIdx.x == 0) {
+    if (!COUNT_ONLY && threadIdx.x == 0) {
         double s = z_lds[0];
         unsigned rows = n_lds[0];
         for (int w = 1; w < RT_WAVES; ++w) {
@@ -231,104 +313,125 @@ __global__ __launch_bounds__(RT_THREADS) void router_forward_kernel(const Router
     }
 }
 
-// One workgroup per group: the slots of its workgroups added in index order, columns of COLS experts at a time, a thread
-// per expert and every FINISH_THREADS / COLS-th slot.
-__global__ __launch_bounds__(FINISH_THREADS) void router_finish_kernel(const RouterSets a, const unsigned *__restrict__ slots,
-                                                                       const unsigned cols, const int64_t *__restrict__ given_counts,
-                                                                       float *__restrict__ balance, float *__restrict__ z,
-                                                                       int64_t *__restrict__ counts, float *__restrict__ slope,
-                                                                       float *__restrict__ inv_rows)
+// The slots of a group's workgroups added in index order: `cols` experts at a time (a power of two, 64 at most), a thread per
+// expert and every FINISH_THREADS / cols-th slot, their sums joined in order.  Then the loss of the sums.
+//   SUMS and LOSS   a workgroup per group does both
+//   SUMS alone      gridDim.y workgroups per group, each its share of the experts; the sums go to counts and means
+//   LOSS alone      a workgroup per group, from counts and means
+// Two launches are taken for few groups of many experts, where one workgroup would read a megabyte of slots by itself.  (One
+// launch in which the last of a group's workgroups makes the loss is slower: the fences it needs write the caches back.)
+constexpr int FINISH_THREADS = 1024, FINISH_WAVES = FINISH_THREADS / 64;
+static_assert(RT_MAX_EXPERTS <= FINISH_THREADS, "a thread per expert");
+
+// Sum over the workgroup, in every thread.
+template <typename V>
+__device__ __forceinline__ V finish_sum(V v, V *lds)
 {
-    __shared__ double p_lds[FINISH_THREADS];
-    __shared__ unsigned long long c_lds[FINISH_THREADS];
-    __shared__ double P[RT_MAX_EXPERTS];
-    __shared__ long long C[RT_MAX_EXPERTS];
-    const unsigned E = a.E, words = slot_words(E), tid = threadIdx.x;
-    int set = 0;
-    while (set + 1 < a.S && blockIdx.x >= a.first_group[set + 1]) ++set;
-    const RouterSetK &s = a.s[set];
-    const unsigned image = blockIdx.x - a.first_group[set];              // (0 unless per_image)
-    const unsigned slots_of_group = a.per_image ? s.chunks : s.images * s.chunks;
-    const unsigned *first = slots + (size_t)(s.first_block + image * s.chunks) * words;
-    const unsigned slices = FINISH_THREADS / cols, col = tid & (cols - 1), slice = tid / cols;
-    for (unsigned e0 = 0; e0 < E; e0 += cols) {
-        double p = 0.0;
-        unsigned long long c = 0;
-        if (e0 + col < E)
-            for (unsigned i = slice; i < slots_of_group; i += slices) {
-                const unsigned *slot = first + (size_t)i * words;
-                if (balance) p += (double)__uint_as_float(slot[e0 + col]);
-                c += slot[E + e0 + col];
-            }
-        __syncthreads();
-        p_lds[tid] = p;
-        c_lds[tid] = c;
-        __syncthreads();
-        if (tid < cols && e0 + tid < E) {
-            for (unsigned i = 1; i < slices; ++i) {
-                p += p_lds[i * cols + tid];
-                c += c_lds[i * cols + tid];
-            }
-            P[e0 + tid] = p;
-            C[e0 + tid] = (long long)c;
-            counts[(size_t)blockIdx.x * E + e0 + tid] = (int64_t)c;
-        }
-    }
-    if (!balance) return;
-    // the rows that count and the sum of lse^2
-    double zs = 0.0;
-    unsigned long long rows = 0;
-    for (unsigned i = tid; i < slots_of_group; i += FINISH_THREADS) {
-        const unsigned *slot = first + (size_t)i * words;
-        zs += *reinterpret_cast<const double *>(slot + 2 * E);
-        rows += slot[2 * E + 2];
-    }
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off);
     __syncthreads();
-    p_lds[tid] = zs;
-    c_lds[tid] = rows;
-    if (given_counts)
-        for (unsigned e = tid; e < E; e += FINISH_THREADS) C[e] = given_counts[(size_t)blockIdx.x * E + e];
-    for (unsigned half = FINISH_THREADS / 2; half >= 1; half >>= 1) {
-        __syncthreads();
-        if (tid < half) {
-            p_lds[tid] += p_lds[tid + half];
-            c_lds[tid] += c_lds[tid + half];
-        }
-    }
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
     __syncthreads();
-    const double inv_n = c_lds[0] ? 1.0 / (double)c_lds[0] : 0.0;
-    const double z_mean = p_lds[0] * inv_n;
-    // sum of the counts, then sum_e c_e P_e
-    __syncthreads();
-    long long total = 0;
-    double dot = 0.0;
-    for (unsigned e = tid; e < E; e += FINISH_THREADS) {
-        total += C[e];
-        dot += (double)C[e] * P[e];
-    }
-    p_lds[tid] = dot;
-    c_lds[tid] = (unsigned long long)total;
-    for (unsigned half = FINISH_THREADS / 2; half >= 1; half >>= 1) {
-        __syncthreads();
-        if (tid < half) {
-            p_lds[tid] += p_lds[tid + half];
-            c_lds[tid] += c_lds[tid + half];
-        }
-    }
-    __syncthreads();
-    const long long all = (long long)c_lds[0];
-    const double per_count = all > 0 ? (double)E / (double)all : 0.0;
-    if (tid == 0) {
-        balance[blockIdx.x] = (float)(p_lds[0] * per_count * inv_n);
-        if (z) z[blockIdx.x] = (float)z_mean;
-        inv_rows[blockIdx.x] = (float)inv_n;
-    }
-    for (unsigned e = tid; e < E; e += FINISH_THREADS)
-        slope[(size_t)blockIdx.x * E + e] = all > 0 ? (float)((double)C[e] * per_count - 1.0) : 0.0f;
+    v = lds[0];
+#pragma unroll
+    for (int w = 1; w < FINISH_WAVES; ++w) v += lds[w];
+    return v;
 }
 
-template <typename T, int NQ, int L>
-__global__ __launch_bounds__(RT_THREADS) void router_backward_kernel(const RouterSets a, const int sigmoid,
+template <bool SUMS, bool LOSS>
+__global__ __launch_bounds__(FINISH_THREADS) void router_finish_kernel(const RouterSets a, const unsigned *__restrict__ slots,
+                                                                       const unsigned cols, const int64_t *__restrict__ given_counts,
+                                                                       double *__restrict__ means, float *__restrict__ balance,
+                                                                       float *__restrict__ z, int64_t *__restrict__ counts,
+                                                                       float *__restrict__ slope, float *__restrict__ inv_rows)
+{
+    __shared__ double p_lds[FINISH_WAVES][64];
+    __shared__ unsigned long long c_lds[FINISH_WAVES][64];
+    __shared__ double P[RT_MAX_EXPERTS];
+    __shared__ long long C[RT_MAX_EXPERTS];
+    const unsigned E = a.E, words = slot_words(E), tid = threadIdx.x, group = blockIdx.x;
+    int set = 0;
+    while (set + 1 < a.S && group >= a.first_group[set + 1]) ++set;
+    const RouterSetK &s = a.s[set];
+    const unsigned image = group - a.first_group[set];                   // (0 unless per_image)
+    const unsigned slots_of_group = a.per_image ? s.chunks : s.images * s.chunks;
+    const unsigned *first = slots + (size_t)(s.first_block + image * s.chunks) * words;
+    // the rows that count and the sum of lse^2 are asked for first
+    double zs = 0.0;
+    unsigned long long rows = 0;
+    if (LOSS)
+        for (unsigned i = tid; i < slots_of_group; i += FINISH_THREADS) {
+            const unsigned *slot = first + (size_t)i * words;
+            zs += *reinterpret_cast<const double *>(slot + 2 * E);
+            rows += slot[2 * E + 2];
+        }
+    if (SUMS) {
+        const unsigned col = tid & (cols - 1), slice = tid / cols, slices = FINISH_THREADS / cols;
+        const bool with_p = means != nullptr || LOSS;
+        for (unsigned e0 = blockIdx.y * cols; e0 < E; e0 += gridDim.y * cols) {
+            const unsigned e = e0 + col;
+            double p = 0.0;
+            unsigned long long c = 0;
+            if (e < E) {
+#pragma unroll 8
+                for (unsigned i = slice; i < slots_of_group; i += slices) {
+                    const unsigned *slot = first + (size_t)i * words;
+                    if (with_p) p += (double)__uint_as_float(slot[e]);
+                    c += slot[E + e];
+                }
+            }
+            for (unsigned off = cols; off < 64; off <<= 1) {
+                p += __shfl_xor(p, off);
+                c += __shfl_xor(c, off);
+            }
+            if ((tid & 63) < cols) {
+                p_lds[tid >> 6][col] = p;
+                c_lds[tid >> 6][col] = c;
+            }
+            __syncthreads();
+            if (tid < cols && e < E) {
+#pragma unroll
+                for (int i = 1; i < FINISH_WAVES; ++i) {
+                    p += p_lds[i][col];
+                    c += c_lds[i][col];
+                }
+                counts[(size_t)group * E + e] = (int64_t)c;
+                if (LOSS) {
+                    P[e] = p;
+                    C[e] = (long long)c;
+                } else if (means) {
+                    means[(size_t)group * E + e] = p;
+                }
+            }
+            __syncthreads();
+        }
+    }
+    if (!LOSS) return;
+    double *sums = &p_lds[0][0];
+    unsigned long long *whole = &c_lds[0][0];
+    long long mine = 0;
+    double mean = 0.0;
+    if (tid < E) {
+        const int64_t *shares = given_counts ? given_counts : SUMS ? nullptr : counts;
+        mine = shares ? shares[(size_t)group * E + tid] : C[tid];
+        mean = SUMS ? P[tid] : means[(size_t)group * E + tid];
+    }
+    rows = finish_sum(rows, whole);
+    const long long all = (long long)finish_sum((unsigned long long)mine, whole);
+    zs = finish_sum(zs, sums);
+    const double dot = finish_sum((double)mine * mean, sums);
+    const double inv_n = rows ? 1.0 / (double)rows : 0.0;
+    const double per_count = all > 0 ? (double)E / (double)all : 0.0;
+    if (tid == 0) {
+        balance[group] = (float)(dot * per_count * inv_n);
+        if (z) z[group] = (float)(zs * inv_n);
+        inv_rows[group] = (float)inv_n;
+    }
+    if (tid < E) slope[(size_t)group * E + tid] = all > 0 ? (float)((double)mine * per_count - 1.0) : 0.0f;
+}
+
+template <int NQ, int L, bool WIDE>
+__global__ __launch_bounds__(RT_THREADS) void router_backward_kernel(const RouterSets a, const int dtype, const int sigmoid,
                                                                      const float *__restrict__ slope,
                                                                      const float *__restrict__ inv_rows,
                                                                      const float *__restrict__ grad_balance,
@@ -339,9 +442,8 @@ __global__ __launch_bounds__(RT_THREADS) void router_backward_kernel(const Route
     const float ninf = -__builtin_huge_valf();
     const Place at = place_of(a, blockIdx.x);
     const RouterSetK &set = a.s[at.set];
-    const T *base = static_cast<const T *>(set.logits) + (size_t)at.image * (size_t)set.image_stride;
+    const size_t image_at = (size_t)at.image * (size_t)set.image_stride;
     const size_t image_row = (size_t)at.image * set.Q;
-    T *out = static_cast<T *>(set.grad) + image_row * E;
     const unsigned group = a.first_group[at.set] + (a.per_image ? at.image : 0);
     const float inv_n = inv_rows[group];
     const float gb = grad_balance ? grad_balance[group] * inv_n : 0.0f;
@@ -349,61 +451,69 @@ __global__ __launch_bounds__(RT_THREADS) void router_backward_kernel(const Route
     const unsigned sub = threadIdx.x & (L - 1);
     constexpr unsigned ROWS = RT_THREADS / L;
     float f[N];
-#pragma unroll
-    for (int q = 0; q < NQ; ++q) {
-        float v[4];
-        dm::load_quad(slope + (size_t)group * E, 4 * (q * L + sub), E, 0.0f, v);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) f[4 * q + j] = v[j];
-    }
+    dm::row_values<NQ, L, true>(dm::fetch_row<NQ, L, true>(slope, (size_t)group * E, sub, E), DM_F32, sub, E, 0.0f, f);
+    const unsigned local = threadIdx.x / L;
+    dm::RawRow<NQ, WIDE> next;
+    uint8_t next_counts = 1;
+    auto fetch = [&](unsigned r) {
+        const size_t row = (size_t)at.row0 + (r < at.rows ? r : 0);
+        next = dm::fetch_row<NQ, L, WIDE>(set.logits, image_at + row * E, sub, E);
+        if (set.mask) next_counts = set.mask[image_row + row];
+    };
+    if (at.rows) fetch(local);
     for (unsigned r0 = 0; r0 < at.rows; r0 += ROWS) {
-        const unsigned r = r0 + threadIdx.x / L;
+        const unsigned r = r0 + local;
         const bool there = r < at.rows;
         const size_t row = (size_t)at.row0 + (there ? r : 0);
-        const bool wanted = there && (!set.mask || set.mask[image_row + row] != 0);
+        const dm::RawRow<NQ, WIDE> raw = next;
+        const bool counts = next_counts != 0;
+        if (r0 + ROWS < at.rows) fetch(r + ROWS);
         float x[N];
-        float mx = ninf;
+        dm::row_values<NQ, L, WIDE>(raw, dtype, sub, E, ninf, x);
+        if (!counts) {
 #pragma unroll
-        for (int q = 0; q < NQ; ++q) {
-            float v[4] = {ninf, ninf, ninf, ninf};
-            if (wanted) dm::load_quad(base + row * E, 4 * (q * L + sub), E, ninf, v);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                x[4 * q + j] = v[j];
-                mx = fmaxf(mx, v[j]);                          // (NaN is passed over)
-            }
+            for (int j = 0; j < N; ++j) x[j] = ninf;
         }
-        mx = dm::over_group<L>(mx, dm::Max());
+        float mx = ninf;                                       // (a NaN makes the whole row NaN, whatever is found here)
+#pragma unroll
+        for (int j = 0; j < N; j += 2) mx = dm::max3(mx, x[j], x[j + 1]);
+        mx = dm::largest<L>(mx);
         mx = mx == ninf ? 0.0f : mx;
-        const float c = fminf(mx, 0.0f), exp_c = __builtin_amdgcn_exp2f(c * LOG2E);
         float sum = 0.0f, dot = 0.0f;
         float rest[N];
+        if (sigmoid) {
+            const float c = fminf(mx, 0.0f), exp_c = __builtin_amdgcn_exp2f(c * LOG2E);
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                rest[j] = 1.0f;
+                x[j] = x[j] == ninf ? 0.0f : sigmoid_weight(x[j], c, exp_c, &rest[j]);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                rest[j] = 1.0f;
+                x[j] = softmax_weight(x[j], mx);
+            }
+        }
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            rest[j] = 1.0f;
-            x[j] = sigmoid ? (x[j] == ninf ? 0.0f : sigmoid_weight(x[j], c, exp_c, &rest[j])) : softmax_weight(x[j], mx);
             sum += x[j];
-            dot += x[j] * f[j];
+            dot = __builtin_fmaf(x[j], f[j], dot);
         }
         sum = dm::over_group<L>(sum, dm::Add());
         dot = dm::over_group<L>(dot, dm::Add());
         const bool live = sum != 0.0f;
         const float inv = live ? __builtin_amdgcn_rcpf(sum) : 0.0f;
         dot *= inv;
+        // p (gb (f - dot) + gz lse)
         const float lse = live ? mx + __builtin_amdgcn_logf(sum) * LN2 : 0.0f;
         const float zpart = gz * lse;
-        if (there) {
 #pragma unroll
-            for (int q = 0; q < NQ; ++q) {
-                float v[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int i = 4 * q + j;
-                    v[j] = live ? x[i] * inv * (gb * (f[i] - dot) + zpart) * rest[i] : 0.0f;
-                }
-                dm::store_quad(out + row * E, 4 * (q * L + sub), E, v);
-            }
+        for (int j = 0; j < N; ++j) {
+            const float g = (x[j] * inv) * __builtin_fmaf(gb, f[j] - dot, zpart);
+            x[j] = live ? g * rest[j] : 0.0f;
         }
+        if (there) dm::store_row<NQ, L, WIDE>(set.grad, dtype, (image_row + row) * E, sub, E, x);
     }
 }
 
@@ -431,15 +541,44 @@ int check_shape(const DmRouterSet *sets, int S, int B, int E, int per_image, Sha
     return DM_OK;
 }
 
-constexpr unsigned ROWS_AT_A_TIME = RT_THREADS / 64;
+// Lanes per row and logits per lane.  Forward: ... 
+struct Form {
+    int NQ, L;
+};
+Form forward_form(unsigned E)
+{
+    if (E <= 4) return {1, 1};
+    if (E <= 8) return {2, 1};
+    if (E <= 16) return {2, 2};
+    if (E <= 32) return {2, 4};
+    if (E <= 64) return {4, 4};
+    if (E <= 96) return {3, 8};
+    if (E <= 128) return {4, 8};
+    if (E <= 192) return {3, 16};
+    if (E <= 256) return {4, 16};
+    return {4, E <= 512 ? 32 : 64};
+}
+Form backward_form(unsigned E)
+{
+    if (E <= 4) return {1, 1};
+    if (E <= 8) return {1, 2};
+    if (E <= 16) return {1, 4};
+    if (E <= 32) return {1, 8};
+    if (E <= 64) return {1, 16};
+    if (E <= 128) return {2, 16};
+    if (E <= 192) return {3, 16};
+    if (E <= 256) return {4, 16};
+    return {4, E <= 512 ? 32 : 64};
+}
 
 // Chunks per image of a set: enough workgroups to fill the chip over all sets of the call, none with less than one trip.
 unsigned chunks_of(const Shape &sh, int Q)
 {
     const long long images = sh.merged ? 1 : sh.B;
     const long long rows = sh.merged ? (long long)sh.B * Q : Q;
+    const long long trip = RT_THREADS / forward_form((unsigned)sh.E).L;
     const long long want = std::max(1ll, 1024 / std::max(1ll, (long long)sh.S * images));
-    return (unsigned)std::max(1ll, std::min(want, (rows + ROWS_AT_A_TIME - 1) / ROWS_AT_A_TIME));
+    return (unsigned)std::max(1ll, std::min(want, (rows + trip - 1) / trip));
 }
 
 // The kernel arguments of sets first .. first + n - 1; returns the launch's workgroups.
@@ -482,27 +621,61 @@ unsigned long long most_blocks(const DmRouterSet *sets, const Shape &sh)
     return most;
 }
 
-typedef void (*ForwardKernel)(RouterSets, int, unsigned *, int32_t *);
-typedef void (*BackwardKernel)(RouterSets, int, const float *, const float *, const float *, const float *);
+typedef void (*ForwardKernel)(RouterSets, int, int, unsigned *, int32_t *);
+typedef void (*BackwardKernel)(RouterSets, int, int, const float *, const float *, const float *, const float *);
 
-template <typename T, int NQ>
-ForwardKernel forward_of(bool count_only)
+template <int NQ, int L, int K>
+ForwardKernel forward_of(bool wide, bool count_only)
 {
-    return count_only ? router_forward_kernel<T, NQ, 64, true> : router_forward_kernel<T, NQ, 64, false>;
+    return wide ? (count_only ? router_forward_kernel<NQ, L, K, true, true> : router_forward_kernel<NQ, L, K, true, false>)
+                : (count_only ? router_forward_kernel<NQ, L, K, false, true> : router_forward_kernel<NQ, L, K, false, false>);
 }
-template <typename T>
-ForwardKernel forward_for(unsigned E, bool count_only)
+template <int NQ, int L>
+ForwardKernel forward_with(unsigned k, bool wide, bool count_only)
 {
-    if (E <= 256) return forward_of<T, 1>(count_only);
-    if (E <= 512) return forward_of<T, 2>(count_only);
-    return forward_of<T, 4>(count_only);
+    if (k <= 2) return forward_of<NQ, L, 2>(wide, count_only);
+    if (k <= 4) return forward_of<NQ, L, 4>(wide, count_only);
+    if (k <= 8) return forward_of<NQ, L, 8>(wide, count_only);
+    return forward_of<NQ, L, 0>(wide, count_only);
 }
-template <typename T>
+ForwardKernel forward_for(unsigned E, unsigned k, bool wide, bool count_only)
+{
+    const Form f = forward_form(E);
+    switch (f.L) {
+    case 1: return f.NQ == 1 ? forward_with<1, 1>(k, wide, count_only) : forward_with<2, 1>(k, wide, count_only);
+    case 2: return forward_with<2, 2>(k, wide, count_only);
+    case 4: return f.NQ == 2 ? forward_with<2, 4>(k, wide, count_only) : forward_with<4, 4>(k, wide, count_only);
+    case 8: return f.NQ == 3 ? forward_with<3, 8>(k, wide, count_only) : forward_with<4, 8>(k, wide, count_only);
+    case 16: return f.NQ == 3 ? forward_with<3, 16>(k, wide, count_only) : forward_with<4, 16>(k, wide, count_only);
+    case 32: return forward_with<4, 32>(k, wide, count_only);
+    default: return forward_with<4, 64>(k, wide, count_only);
+    }
+}
+template <bool WIDE>
 BackwardKernel backward_for(unsigned E)
 {
-    if (E <= 256) return router_backward_kernel<T, 1, 64>;
-    if (E <= 512) return router_backward_kernel<T, 2, 64>;
-    return router_backward_kernel<T, 4, 64>;
+    const Form f = backward_form(E);
+    switch (f.L) {
+    case 1: return router_backward_kernel<1, 1, WIDE>;
+    case 2: return router_backward_kernel<1, 2, WIDE>;
+    case 4: return router_backward_kernel<1, 4, WIDE>;
+    case 8: return router_backward_kernel<1, 8, WIDE>;
+    case 16:
+        return f.NQ == 1 ? router_backward_kernel<1, 16, WIDE> : f.NQ == 2 ? router_backward_kernel<2, 16, WIDE>
+               : f.NQ == 3 ? router_backward_kernel<3, 16, WIDE> : router_backward_kernel<4, 16, WIDE>;
+    case 32: return router_backward_kernel<4, 32, WIDE>;
+    default: return router_backward_kernel<4, 64, WIDE>;
+    }
+}
+
+// Workspace: the slots of a launch's workgroups, then the sums of p of its groups.
+struct Workspace {
+    unsigned long long blocks, groups;
+    int64_t bytes(int E) const { return (int64_t)(std::max(1ull, blocks) * slot_words((unsigned)E) * 4 + groups * (unsigned long long)E * 8); }
+};
+Workspace workspace_of(const DmRouterSet *sets, const Shape &sh)
+{
+    return Workspace{most_blocks(sets, sh), (unsigned long long)std::min(sh.S, DM_MAX_SETS_PER_LAUNCH) * (sh.per_image ? (unsigned long long)sh.B : 1ull)};
 }
 
 int forward(const DmRouterSet *sets, int S, int B, int E, int top_k, int dtype, int scores, int per_image,
@@ -525,32 +698,44 @@ int forward(const DmRouterSet *sets, int S, int B, int E, int top_k, int dtype, 
         if (!sets[s].logits || (given >= 0 && has != given) || (!has && top_k > E)) return DM_E_INVALID_ARG;
         given = has;
     }
-    const unsigned long long blocks_needed = most_blocks(sets, sh);
-    if (blocks_needed >= (1ull << 31)) return DM_E_UNSUPPORTED;
-    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0 ||
-        workspace_bytes < (int64_t)(blocks_needed * slot_words((unsigned)E) * 4)) return DM_E_INVALID_ARG;
+    if (given == 1 && !balance) return DM_E_INVALID_ARG;       // (the counts of given indices need no logits)
+    const Workspace need = workspace_of(sets, sh);
+    if (need.blocks >= (1ull << 31)) return DM_E_UNSUPPORTED;
+    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0 || workspace_bytes < need.bytes(E)) return DM_E_INVALID_ARG;
     unsigned *slots = static_cast<unsigned *>(workspace);
-    unsigned cols = 1;
-    while (cols < 64 && cols < (unsigned)E) cols <<= 1;
+    double *means = reinterpret_cast<double *>(slots + (size_t)std::max(1ull, need.blocks) * slot_words((unsigned)E));
     for (int first = 0; first < S; first += DM_MAX_SETS_PER_LAUNCH) {
         RouterSets a;
         const int n = std::min(S - first, DM_MAX_SETS_PER_LAUNCH);
         const unsigned blocks = (unsigned)describe(sets, first, n, sh, top_k, &a);
         if (blocks) {
-            const bool count_only = balance == nullptr;
-            ForwardKernel kernel = dtype == DM_F32    ? forward_for<float>((unsigned)E, count_only)
-                                   : dtype == DM_BF16 ? forward_for<dm::bf16_t>((unsigned)E, count_only)
-                                                      : forward_for<dm::half_t>((unsigned)E, count_only);
-            hipLaunchKernelGGL(kernel, dim3(blocks), dim3(RT_THREADS), 0, st, a, scores == DM_SCORES_SIGMOID ? 1 : 0, slots, status);
+            hipLaunchKernelGGL(forward_for((unsigned)E, given == 1 ? 1u : (unsigned)top_k, dtype == DM_F32, balance == nullptr), dim3(blocks), dim3(RT_THREADS), 0,
+                               st, a, dtype, scores == DM_SCORES_SIGMOID ? 1 : 0, slots, status);
             rc = dm::check_hip(hipGetLastError(), "router_forward_kernel launch");
             if (rc != DM_OK) return rc;
         }
         const size_t g0 = (size_t)first * (per_image ? (size_t)B : 1);
         const unsigned gn = (unsigned)n * (per_image ? (unsigned)B : 1u);
-        hipLaunchKernelGGL(router_finish_kernel, dim3(gn), dim3(FINISH_THREADS), 0, st, a, slots, cols,
-                           given_counts ? given_counts + g0 * E : nullptr, balance ? balance + g0 : nullptr,
-                           z ? z + g0 : nullptr, counts + g0 * E, slope ? slope + g0 * E : nullptr,
-                           inv_rows ? inv_rows + g0 : nullptr);
+        unsigned cols = 1;
+        while (cols < 64 && cols < (unsigned)E) cols <<= 1;
+        auto finish = [&](auto kernel, unsigned parts, unsigned width) {
+            hipLaunchKernelGGL(kernel, dim3(gn, parts), dim3(FINISH_THREADS), 0, st, a, slots, width,
+                               given_counts ? given_counts + g0 * E : nullptr, means, balance ? balance + g0 : nullptr,
+                               z ? z + g0 : nullptr, counts + g0 * E, slope ? slope + g0 * E : nullptr,
+                               inv_rows ? inv_rows + g0 : nullptr);
+        };
+        // (by itself a workgroup adds some 64 slots of 64 experts a microsecond)
+        const bool few = gn <= 16 && E > 64 && (unsigned long long)blocks * (unsigned)E > 64ull * 1024 * gn;
+        const unsigned width = few ? 16u : cols, parts = few ? (unsigned)(E + 15) / 16 : 1u;
+        if (!balance) {
+            means = nullptr;
+            finish(router_finish_kernel<true, false>, parts, width);
+        } else if (few) {
+            finish(router_finish_kernel<true, false>, parts, width);
+            finish(router_finish_kernel<false, true>, 1u, cols);
+        } else {
+            finish(router_finish_kernel<true, true>, 1u, cols);
+        }
         rc = dm::check_hip(hipGetLastError(), "router_finish_kernel launch");
         if (rc != DM_OK) return rc;
     }
@@ -564,7 +749,7 @@ extern "C" int64_t dm_balance_workspace(const DmRouterSet *sets, int S, int B, i
     Shape sh;
     const int rc = check_shape(sets, S, B, E, per_image, &sh);
     if (rc != DM_OK) return rc;
-    return (int64_t)(std::max(1ull, most_blocks(sets, sh)) * slot_words((unsigned)E) * 4);
+    return workspace_of(sets, sh).bytes(E);
 }
 
 extern "C" int dm_balance_loss(const DmRouterSet *sets, int S, int B, int E, int top_k, int dtype, int scores, int per_image,
@@ -604,11 +789,8 @@ extern "C" int dm_balance_backward(const DmRouterSet *sets, int S, int B, int E,
         RouterSets a;
         const int n = std::min(S - first, DM_MAX_SETS_PER_LAUNCH);
         const unsigned blocks = (unsigned)describe(sets, first, n, sh, 0, &a);
-        BackwardKernel kernel = dtype == DM_F32    ? backward_for<float>((unsigned)E)
-                                : dtype == DM_BF16 ? backward_for<dm::bf16_t>((unsigned)E)
-                                                   : backward_for<dm::half_t>((unsigned)E);
         const size_t g0 = (size_t)first * (per_image ? (size_t)B : 1);
-        hipLaunchKernelGGL(kernel, dim3(blocks), dim3(RT_THREADS), 0, st, a, scores == DM_SCORES_SIGMOID ? 1 : 0,
+        hipLaunchKernelGGL(dtype == DM_F32 ? backward_for<true>((unsigned)E) : backward_for<false>((unsigned)E), dim3(blocks), dim3(RT_THREADS), 0, st, a, dtype, scores == DM_SCORES_SIGMOID ? 1 : 0,
                            slope + g0 * E, inv_rows + g0, grad_balance ? grad_balance + g0 : nullptr,
                            grad_z ? grad_z + g0 : nullptr);
         rc = dm::check_hip(hipGetLastError(), "router_backward_kernel launch");

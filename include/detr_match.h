@@ -416,7 +416,7 @@ int dm_balance_loss(const DmRouterSet *sets, int S, int B, int E, int top_k, int
 int dm_balance_backward(const DmRouterSet *sets, int S, int B, int E, int dtype, int scores, int per_image,
                         const float *slope, const float *inv_rows, const float *grad_balance, const float *grad_z,
                         void *stream);
-/* The counts alone: one pass that takes no exponentials. */
+/* The counts alone (of the logits: sets[s].experts NULL): one pass that takes no exponentials. */
 int dm_expert_counts(const DmRouterSet *sets, int S, int B, int E, int top_k, int dtype, int per_image, int64_t *counts,
                      void *workspace, int64_t workspace_bytes, int32_t *status, void *stream);
 
