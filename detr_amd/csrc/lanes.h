@@ -48,9 +48,10 @@ __device__ __forceinline__ void store_quad(T *row, unsigned c, unsigned n, const
 
 // A row that L lanes share; WIDE: of DM_F32, else of DM_BF16 or DM_F16 as `dtype` says.  A lane holds NQ quads of four
 // elements, the lanes' quads side by side.  `fetch_row` only asks for the memory, so that a kernel can ask for its next row
-// before it works on this one; `row_values` makes float32 of what came.  There is no branch between the loads (each would wait
-// for the one before it): a quad that reaches past the row is read at the row's last four elements and moved into place
-// afterwards, `fill` behind the row's end.  One lane with one quad also takes rows of fewer than four elements.
+// before it works on this one; `row_values` makes float32 of what came: `raw_values`, then `place_row`.  There is no branch
+// between the loads (each would wait for the one before it): a quad that reaches past the row is read at the row's last four
+// elements and moved into place afterwards.  One lane with one quad also takes rows of fewer than four elements.  (What is read
+// is of the row in every case.)
 template <int NQ, bool WIDE>
 struct RawRow {
     unsigned q[NQ][WIDE ? 4 : 2];
@@ -69,7 +70,7 @@ __device__ __forceinline__ RawRow<NQ, WIDE> fetch_row(const void *base, size_t f
         } else {
             const uint16_t *row = static_cast<const uint16_t *>(base) + first;
             raw.q[0][0] = row[0] | (unsigned)row[min(1u, n - 1)] << 16;
-            raw.q[0][1] = row[n - 1];
+            raw.q[0][1] = row[n - 1] | (unsigned)row[n - 1] << 16;
         }
         return raw;
     }
@@ -91,8 +92,8 @@ __device__ __forceinline__ RawRow<NQ, WIDE> fetch_row(const void *base, size_t f
     return raw;
 }
 
-template <int NQ, int L, bool WIDE>
-__device__ __forceinline__ void row_values(const RawRow<NQ, WIDE> &raw, int dtype, unsigned sub, unsigned n, float fill, float (&x)[4 * NQ])
+template <int NQ, bool WIDE>
+__device__ __forceinline__ void raw_values(const RawRow<NQ, WIDE> &raw, int dtype, float (&x)[4 * NQ])
 {
     if (WIDE) {
 #pragma unroll
@@ -118,6 +119,12 @@ __device__ __forceinline__ void row_values(const RawRow<NQ, WIDE> &raw, int dtyp
                 x[4 * q + 2 * k + 1] = (float)h.y;
             }
     }
+}
+
+// Quads that were read further to the left into their places, `fill` behind the row's end.
+template <int NQ, int L>
+__device__ __forceinline__ void place_row(float (&x)[4 * NQ], unsigned sub, unsigned n, float fill)
+{
 #pragma unroll
     for (int q = 0; q < NQ; ++q) {
         if (4 * (q + 1) * L <= n) continue;                    // (the same for all lanes)
@@ -137,6 +144,13 @@ __device__ __forceinline__ void row_values(const RawRow<NQ, WIDE> &raw, int dtyp
             v[3] = out || two ? fill : a3;
         }
     }
+}
+
+template <int NQ, int L, bool WIDE>
+__device__ __forceinline__ void row_values(const RawRow<NQ, WIDE> &raw, int dtype, unsigned sub, unsigned n, float fill, float (&x)[4 * NQ])
+{
+    raw_values<NQ, WIDE>(raw, dtype, x);
+    place_row<NQ, L>(x, sub, n, fill);
 }
 
 template <int NQ, int L, bool WIDE>

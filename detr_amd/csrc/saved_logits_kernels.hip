@@ -28,6 +28,12 @@ constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr int FINEST = -16, FOCAL_COARSEST = -2, CE_COARSEST = -3, NOT_A_NUMBER = -128;
 constexpr float FOCAL_CLAMP = 20.0f, CE_CLAMP = 1048576.0f;
 
+// A byte (a whole number from 0 to 255) into place k of a word.
+__device__ __forceinline__ unsigned pack_code(unsigned word, unsigned k, float code)
+{
+    return __builtin_amdgcn_cvt_pk_u8_f32(code, k, word);
+}
+
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((unsigned)(127 + e) << 23); }
 
 // The exponent of the step of a block whose logits lie in [low, high].  With high - low in [2^E, 2^(E+1)) the span at
@@ -56,26 +62,17 @@ __device__ __forceinline__ FocalParts focal_parts(float z, float gamma)
 {
     FocalParts f;
     const float e = __builtin_amdgcn_exp2f(-__builtin_fabsf(z) * LOG2E);
-    const float one_e = 1.0f + e, r = __builtin_amdgcn_rcpf(one_e), er = e * r;
+    const float one_e = 1.0f + e, r = __builtin_amdgcn_rcpf(one_e);
     const bool up = z >= 0.0f;
-    f.sigmoid = up ? r : er;
-    f.rest = up ? er : r;
+    f.sigmoid = (up ? 1.0f : e) * r;
+    f.rest = (up ? e : 1.0f) * r;
     // log1p(e) = log(1 + e) + what the rounding of 1 + e dropped, over 1 + e
-    const float l1p = __builtin_amdgcn_logf(one_e) * LN2 + (e - (one_e - 1.0f)) * r;
-    f.softplus = __builtin_fmaxf(z, 0.0f) + l1p;
+    const float l1p = __builtin_fmaf(e - (one_e - 1.0f), r, __builtin_amdgcn_logf(one_e) * LN2);
+    f.softplus = (up ? z : 0.0f) + l1p;
     // (NaN: fminf passes it over, e carries it)
     if (GAMMA2) f.power = f.sigmoid * f.sigmoid;
-    else f.power = __builtin_amdgcn_exp2f(-gamma * LOG2E * __builtin_fminf(__builtin_fmaxf(-z, 0.0f) + l1p, 1e30f));      // (0 x infinity)
+    else f.power = __builtin_amdgcn_exp2f(-gamma * LOG2E * __builtin_fminf((up ? 0.0f : -z) + l1p, 1e30f));      // (0 x infinity)
     return f;
-}
-
-__device__ __forceinline__ float flip(float x, bool positive)
-{
-    return __uint_as_float(__float_as_uint(x) ^ (positive ? 0x80000000u : 0u));
-}
-__device__ __forceinline__ float focal_alpha(const FocalParams &fp, bool positive)
-{
-    return fp.alpha >= 0.0f ? (positive ? fp.alpha : 1.0f - fp.alpha) : 1.0f;
 }
 
 // Rows and columns of a thread's quads of four consecutive logits, `stride` quads apart, walked by additions.
@@ -97,30 +94,53 @@ struct Walk {
     }
 };
 
-// The class codes of a quad's logits: with two or more classes four consecutive logits lie in at most two rows (the flat
-// array's quads start at multiples of four, so that also holds for two classes); with one, each is a row.
+// The rows of a quad: with two or more classes four consecutive logits lie in at most two (the flat array's quads start at
+// multiples of four, so that also holds for two classes); with one, each is a row.  `ask` loads their classes, `settle` makes
+// of them which logits are positive and which count.
 template <bool ONE_CLASS>
 struct QuadRows {
-    int code[ONE_CLASS ? 4 : 2];
-    unsigned col, C;
-    __device__ __forceinline__ QuadRows(const int64_t *cls, unsigned row, unsigned col_, unsigned C_, unsigned rows,
-                                        const FocalParams &fp) : col(col_), C(C_)
+    static constexpr unsigned ROWS = ONE_CLASS ? 4 : 2;
+    int64_t label[ROWS];
+    unsigned col;
+    int code[ROWS];
+    int hot[ROWS];        // place of the row's positive logit in the quad, if it is there
+    bool skipped;         // a row is ignored (or bad): the general answer of `counts` is needed
+
+    __device__ __forceinline__ void ask(const int64_t *cls, unsigned row, unsigned col_, unsigned rows)
     {
+        col = col_;
 #pragma unroll
-        for (unsigned k = 0; k < (ONE_CLASS ? 4u : 2u); ++k) code[k] = row_code(cls[min(row + k, rows - 1)], C, fp);
+        for (unsigned k = 0; k < ROWS; ++k) label[k] = cls[min(row + k, rows - 1)];
     }
-    // class code of logit k's row, and whether k is the row's positive logit
-    __device__ __forceinline__ int row_class(unsigned k, bool *positive) const
+    __device__ __forceinline__ void settle(unsigned C, const FocalParams &fp, bool *bad)
     {
-        const bool wrapped = !ONE_CLASS && col + k >= C;
-        const int c = ONE_CLASS ? code[k] : (wrapped ? code[1] : code[0]);
-        const unsigned column = ONE_CLASS ? 0u : (wrapped ? col + k - C : col + k);
-        *positive = c == (int)column;
-        return c;
+        skipped = false;
+#pragma unroll
+        for (unsigned k = 0; k < ROWS; ++k) {
+            code[k] = row_code(label[k], C, fp);
+            skipped |= code[k] < 0;
+            *bad |= code[k] == ROW_BAD;
+            const int start = ONE_CLASS ? (int)k : (k ? (int)(C - col) : -(int)col);      // place of the row's first logit
+            hot[k] = (unsigned)code[k] < C ? start + code[k] : -1;
+        }
+    }
+    __device__ __forceinline__ bool positive(unsigned k) const
+    {
+        if (ONE_CLASS) return hot[k] == (int)k;
+        return hot[0] == (int)k || hot[1] == (int)k;
+    }
+    __device__ __forceinline__ bool counts(unsigned k, unsigned C) const
+    {
+        return (ONE_CLASS ? code[k] : col + k >= C ? code[1] : code[0]) >= 0;
     }
 };
 
 constexpr unsigned BLOCK_QUADS = 32;      // 128 logits: 32 lanes with four each
+constexpr int FORWARD_QUADS = 2, BACKWARD_QUADS = 4;      // quads a thread asks for before it works on them
+
+struct Quad4 {
+    float v[4];
+};
 
 // Loss, bytes and heads.  codes NULL: the loss alone.
 template <typename T, bool GAMMA2, bool ONE_CLASS>
@@ -131,48 +151,79 @@ __global__ __launch_bounds__(CLS_THREADS) void focal_saved_kernel(const T *__res
                                                                   int32_t *__restrict__ status)
 {
     __shared__ double lds[CLS_THREADS / 64];
-    const unsigned quads = (n + 127) / 128 * BLOCK_QUADS;             // whole blocks
+    const unsigned whole = n / 128 * BLOCK_QUADS;                     // quads of whole blocks
     const unsigned stride = gridDim.x * CLS_THREADS;
-    unsigned i = blockIdx.x * CLS_THREADS + threadIdx.x;
-    Walk at(i, stride, C);
+    const float alpha1 = fp.alpha >= 0.0f ? fp.alpha : 1.0f, alpha0 = fp.alpha >= 0.0f ? 1.0f - fp.alpha : 1.0f;
     float acc = 0.0f;
     bool bad = false;
-    // (the 32 lanes of a block run the same trips: the stride is a multiple of 32)
-    for (; i < quads; i += stride) {
-        const unsigned first = i << 2;
-        float v[4];
-        dm::load_quad(x, first, n, 0.0f, v);
-        const QuadRows<ONE_CLASS> q(cls, ONE_CLASS ? first : at.row, at.col, C, rows, fp);
-        float high = -__builtin_huge_valf(), low = __builtin_huge_valf(), c[4];
+
+    // the quad i, whose first logit is `first`; `there`: how many of its logits there are
+    auto work = [&](unsigned i, const float (&v)[4], QuadRows<ONE_CLASS> &q, unsigned there) {
+        q.settle(C, fp, &bad);
+        float term[4], c[4];
+        float high = -FOCAL_CLAMP, low = FOCAL_CLAMP;
+        bool nan = false;
 #pragma unroll
         for (unsigned k = 0; k < 4; ++k) {
-            bool positive;
-            const int row_class = q.row_class(k, &positive);
-            const bool inside = first + k < n;
-            const FocalParts f = focal_parts<GAMMA2>(flip(v[k], positive), fp.gamma);
-            acc += inside && row_class >= 0 ? focal_alpha(fp, positive) * (f.softplus * f.power) : 0.0f;
-            bad |= inside && row_class == ROW_BAD;
-            c[k] = fminf(fmaxf(v[k], -FOCAL_CLAMP), FOCAL_CLAMP);
-            low = inside ? fminf(low, c[k]) : low;
-            high = inside ? fmaxf(high, v[k] != v[k] ? __builtin_huge_valf() : c[k]) : high;      // (infinity: a NaN)
+            const bool positive = q.positive(k);
+            const FocalParts f = focal_parts<GAMMA2>(positive ? -v[k] : v[k], fp.gamma);
+            term[k] = (positive ? alpha1 : alpha0) * (f.softplus * f.power);
+            c[k] = __builtin_amdgcn_fmed3f(v[k], -FOCAL_CLAMP, FOCAL_CLAMP);
+            nan |= k < there && v[k] != v[k];
+            if (k < there) {
+                low = __builtin_amdgcn_fmed3f(low, c[k], -FOCAL_CLAMP);
+                high = __builtin_amdgcn_fmed3f(high, c[k], FOCAL_CLAMP);
+            }
         }
+        if (q.skipped || there < 4) {
+#pragma unroll
+            for (unsigned k = 0; k < 4; ++k) term[k] = k < there && q.counts(k, C) ? term[k] : 0.0f;
+        }
+        acc += (term[0] + term[1]) + (term[2] + term[3]);
         if (codes) {
-            high = dm::over_group<32>(high, dm::Max());
-            low = dm::over_group<32>(low, dm::Min());
-            const bool nan = high > FOCAL_CLAMP;
-            const int e = step_exponent(nan ? low : high, low, FOCAL_COARSEST);
+            high = dm::largest<32>(high);
+            low = -dm::largest<32>(-low);
+            const unsigned long long nans = __ballot(nan);
+            const bool block_nan = (unsigned)(nans >> (threadIdx.x & 32)) != 0;
+            const int e = step_exponent(high, low, FOCAL_COARSEST);
             const float inverse = power_of_two(-e);
             const float top = __builtin_rintf(high * inverse);
             unsigned packed = 0;
 #pragma unroll
-            for (unsigned k = 0; k < 4; ++k) {
-                const float code = fminf(top - __builtin_rintf(c[k] * inverse), 255.0f);
-                packed |= ((unsigned)(int)fmaxf(code, 0.0f) & 255u) << (8 * k);
-            }
+            for (unsigned k = 0; k < 4; ++k)
+                packed = pack_code(packed, k, k < there ? top - __builtin_rintf(c[k] * inverse) : 0.0f);
             codes[i] = packed;
-            if ((threadIdx.x & 31) == 0) heads[i / BLOCK_QUADS] = nan ? (NOT_A_NUMBER & 255) : (int)top * 256 | (e & 255);
+            if ((threadIdx.x & 31) == 0) heads[i / BLOCK_QUADS] = block_nan ? (NOT_A_NUMBER & 255) : (int)top * 256 | (e & 255);
         }
-        if (!ONE_CLASS) at.next();
+    };
+
+    unsigned i = blockIdx.x * CLS_THREADS + threadIdx.x;
+    Walk at(i, stride, C);
+    // (the 32 lanes of a block run the same trips: the strides are multiples of 32)
+    for (; i < whole; i += FORWARD_QUADS * stride) {
+        Quad4 v[FORWARD_QUADS];
+        QuadRows<ONE_CLASS> q[FORWARD_QUADS];
+#pragma unroll
+        for (int u = 0; u < FORWARD_QUADS; ++u) {
+            const unsigned j = min(i + u * stride, whole - 1);
+            const typename dm::Quad<T>::type t = *reinterpret_cast<const typename dm::Quad<T>::type *>(x + (size_t)(j << 2));
+            v[u].v[0] = (float)t.x; v[u].v[1] = (float)t.y; v[u].v[2] = (float)t.z; v[u].v[3] = (float)t.w;
+            q[u].ask(cls, ONE_CLASS ? j << 2 : at.row, at.col, rows);
+            if (!ONE_CLASS) at.next();
+        }
+#pragma unroll
+        for (int u = 0; u < FORWARD_QUADS; ++u)
+            if (i + u * stride < whole) work(i + u * stride, v[u].v, q[u], 4);
+    }
+    // the last block, if it is not a whole one
+    if (blockIdx.x == gridDim.x - 1 && threadIdx.x < BLOCK_QUADS && (n & 127)) {
+        const unsigned j = whole + threadIdx.x, first = j << 2;
+        float v[4];
+        dm::load_quad(x, min(first, n), n, 0.0f, v);
+        QuadRows<ONE_CLASS> q;
+        const unsigned row = min(first, n - 1) / C;
+        q.ask(cls, row, min(first, n - 1) - row * C, rows);
+        work(j, v, q, first < n ? min(4u, n - first) : 0u);
     }
     if (bad) dm::raise_status(status, DM_ST_LABEL_RANGE);
     const double total = block_sum((double)acc, lds);
@@ -188,30 +239,47 @@ __global__ __launch_bounds__(CLS_THREADS) void focal_from_saved_kernel(const uns
 {
     const unsigned quads = (n + 3) / 4;
     const unsigned stride = gridDim.x * CLS_THREADS;
+    const float scale = fp.scale * grad_loss[0];
+    const float gamma = GAMMA2 ? 2.0f : fp.gamma;
+    // (the gradient of a positive logit has the other sign)
+    const float alpha1 = -scale * (fp.alpha >= 0.0f ? fp.alpha : 1.0f), alpha0 = scale * (fp.alpha >= 0.0f ? 1.0f - fp.alpha : 1.0f);
     unsigned i = blockIdx.x * CLS_THREADS + threadIdx.x;
     Walk at(i, stride, C);
-    const float scale = fp.scale * grad_loss[0];
-    for (; i < quads; i += stride) {
-        const unsigned first = i << 2;
-        const unsigned packed = codes[i];
-        const int head = heads[i / BLOCK_QUADS];
-        const QuadRows<ONE_CLASS> q(cls, ONE_CLASS ? first : at.row, at.col, C, rows, fp);
-        const int e = (int)(int8_t)(head & 255);
-        const float step = e == NOT_A_NUMBER ? __builtin_nanf("") : power_of_two(e);
-        const float top = (float)(head >> 8);
-        float g[4];
+    for (; i < quads; i += BACKWARD_QUADS * stride) {
+        unsigned packed[BACKWARD_QUADS];
+        int head[BACKWARD_QUADS];
+        QuadRows<ONE_CLASS> q[BACKWARD_QUADS];
 #pragma unroll
-        for (unsigned k = 0; k < 4; ++k) {
-            bool positive;
-            const int row_class = q.row_class(k, &positive);
-            const float x = (top - (float)((packed >> (8 * k)) & 255u)) * step;
-            const FocalParts f = focal_parts<GAMMA2>(flip(x, positive), fp.gamma);
-            const float gamma = GAMMA2 ? 2.0f : fp.gamma;
-            const float slope = f.power * (f.sigmoid + gamma * (f.softplus * f.rest));
-            g[k] = row_class >= 0 ? flip(focal_alpha(fp, positive) * scale * slope, positive) : 0.0f;
+        for (int u = 0; u < BACKWARD_QUADS; ++u) {
+            const unsigned j = min(i + u * stride, quads - 1);
+            packed[u] = codes[j];
+            head[u] = heads[j / BLOCK_QUADS];
+            q[u].ask(cls, ONE_CLASS ? j << 2 : at.row, at.col, rows);
+            if (!ONE_CLASS) at.next();
         }
-        dm::store_quad(grad, first, n, g);
-        if (!ONE_CLASS) at.next();
+#pragma unroll
+        for (int u = 0; u < BACKWARD_QUADS; ++u) {
+            if (i + u * stride >= quads) continue;
+            bool bad = false;
+            q[u].settle(C, fp, &bad);
+            const int e = (int)(int8_t)(head[u] & 255);
+            const float step = e == NOT_A_NUMBER ? __builtin_nanf("") : power_of_two(e);
+            const float top = (float)(head[u] >> 8) * step;
+            float g[4];
+#pragma unroll
+            for (unsigned k = 0; k < 4; ++k) {
+                const bool positive = q[u].positive(k);
+                const float x = __builtin_fmaf((float)((packed[u] >> (8 * k)) & 255u), -step, top);      // (exact)
+                const FocalParts f = focal_parts<GAMMA2>(positive ? -x : x, fp.gamma);
+                const float slope = f.power * __builtin_fmaf(gamma, f.softplus * f.rest, f.sigmoid);
+                g[k] = (positive ? alpha1 : alpha0) * slope;
+            }
+            if (q[u].skipped) {
+#pragma unroll
+                for (unsigned k = 0; k < 4; ++k) g[k] = q[u].counts(k, C) ? g[k] : 0.0f;
+            }
+            dm::store_quad(grad, (i + u * stride) << 2, n, g);
+        }
     }
 }
 
@@ -226,77 +294,92 @@ __device__ __forceinline__ float row_weight(int64_t y, unsigned C, int64_t ignor
     return weight ? weight[y] : 1.0f;
 }
 
-// L lanes share a row and keep it in registers, NQ quads of four logits each.
-template <typename T, int NQ, int L>
-__global__ __launch_bounds__(CLS_THREADS) void ce_saved_kernel(const T *__restrict__ x, const int64_t *__restrict__ cls,
+// L lanes share a row and keep it in registers, NQ quads of four logits each; the next row is asked for before this one is
+// worked on.
+template <int NQ, int L, bool WIDE>
+__global__ __launch_bounds__(CLS_THREADS) void ce_saved_kernel(const void *__restrict__ x, const int dtype, const int64_t *__restrict__ cls,
                                                                const float *__restrict__ weight, const unsigned rows,
                                                                const unsigned C, const int64_t ignore_index,
                                                                uint8_t *__restrict__ codes, int8_t *__restrict__ steps,
                                                                double *__restrict__ partials, int32_t *__restrict__ status)
 {
     __shared__ double lds[CLS_THREADS / 64];
+    constexpr int N = 4 * NQ;
     const unsigned sub = threadIdx.x & (L - 1);
     constexpr unsigned ROWS = CLS_THREADS / L;
+    const unsigned stride = gridDim.x * ROWS;
     const float inf = __builtin_huge_valf();
     float num = 0.0f, den = 0.0f;
     bool bad = false;
+    dm::RawRow<NQ, WIDE> next;
+    int64_t next_y = 0;
+    auto fetch = [&](unsigned row) {
+        const unsigned r = min(row, rows - 1);
+        next_y = cls[r];
+        next = dm::fetch_row<NQ, L, WIDE>(x, (size_t)r * C, sub, C);
+    };
+    if (blockIdx.x * ROWS < rows) fetch(blockIdx.x * ROWS + threadIdx.x / L);
     // (every lane makes the same trips: the reductions need all lanes of a row)
-    for (unsigned r0 = blockIdx.x * ROWS; r0 < rows; r0 += gridDim.x * ROWS) {
+    for (unsigned r0 = blockIdx.x * ROWS; r0 < rows; r0 += stride) {
         const unsigned row = r0 + threadIdx.x / L;
         const bool live = row < rows;
-        const T *lg = x + (size_t)(live ? row : 0) * C;
-        float v[4 * NQ];
-        float mx = -inf, mn = inf;
+        const dm::RawRow<NQ, WIDE> raw = next;
+        const int64_t y = next_y;
+        const float w = live ? row_weight(y, C, ignore_index, weight, &bad) : 0.0f;
+        // the row's own logit, once more (by all its lanes, before the next row is asked for: it is waited for first)
+        const size_t own_at = (size_t)(live ? row : 0) * C + (w != 0.0f ? (unsigned)y : 0u);
+        const float own = WIDE ? static_cast<const float *>(x)[own_at]
+                          : dtype == DM_BF16 ? (float)static_cast<const dm::bf16_t *>(x)[own_at] : (float)static_cast<const dm::half_t *>(x)[own_at];
+        if (r0 + stride < rows) fetch(row + stride);
+        float v[N];
+        dm::raw_values<NQ, WIDE>(raw, dtype, v);
+        float mx = -inf, low = inf;
+        if (codes) {
+            // (logits of the row that were read twice do not change its smallest)
 #pragma unroll
-        for (int q = 0; q < NQ; ++q) {
-            const unsigned c = 4 * (q * L + sub);
-            float t[4];
-            dm::load_quad(lg, c, C, -inf, t);
-#pragma unroll
-            for (unsigned k = 0; k < 4; ++k) {
-                v[4 * q + k] = t[k];
-                mx = fmaxf(mx, t[k]);
-                mn = c + k < C ? fminf(mn, t[k]) : mn;
-            }
+            for (int j = 0; j < N; ++j) low = __builtin_amdgcn_fmed3f(low, v[j], -inf);
+            low = -dm::largest<L>(-low);
         }
-        mx = dm::over_group<L>(mx, dm::Max());
-        mn = dm::over_group<L>(mn, dm::Min());
+        dm::place_row<NQ, L>(v, sub, C, -inf);
+#pragma unroll
+        for (int j = 0; j < N; j += 2) mx = dm::max3(mx, v[j], v[j + 1]);      // (a NaN makes the sum NaN, whatever is found here)
+        mx = dm::largest<L>(mx);
         float sum = 0.0f;
 #pragma unroll
-        for (int k = 0; k < 4 * NQ; ++k) sum += __builtin_amdgcn_exp2f((v[k] - mx) * LOG2E);      // (past the row: exp2(-inf) = 0)
+        for (int j = 0; j < N; ++j) sum += __builtin_amdgcn_exp2f((v[j] - mx) * LOG2E);      // (past the row: exp2(-inf) = 0)
         sum = dm::over_group<L>(sum, dm::Add());
-        if (!live) continue;
-        const int64_t y = cls[row];
-        const float w = row_weight(y, C, ignore_index, weight, &bad);
         if (sub == 0 && w != 0.0f) {
-            num += w * ((mx + __builtin_amdgcn_logf(sum) * LN2) - (float)lg[y]);
+            num += w * ((mx + __builtin_amdgcn_logf(sum) * LN2) - own);
             den += w;
         }
         if (!codes) continue;
-        const float high = fminf(fmaxf(mx, -CE_CLAMP), CE_CLAMP), low = fminf(fmaxf(mn, -CE_CLAMP), CE_CLAMP);
+        const float high = __builtin_amdgcn_fmed3f(mx, -CE_CLAMP, CE_CLAMP);
+        low = __builtin_amdgcn_fmed3f(low, -CE_CLAMP, CE_CLAMP);
         const int e = step_exponent(high, low, CE_COARSEST);
         const float inverse = power_of_two(-e), top = __builtin_rintf(high * inverse);
+        // (the clamp changes no byte while the largest lies well inside it: what is below -2^20 is cut off at 255 anyway)
+        if (__any(!(__builtin_fabsf(mx) < CE_CLAMP / 2))) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) v[j] = __builtin_amdgcn_fmed3f(v[j], -CE_CLAMP, CE_CLAMP);
+        }
         uint8_t *out = codes + (size_t)row * C;
 #pragma unroll
         for (int q = 0; q < NQ; ++q) {
+            unsigned packed = 0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                packed = pack_code(packed, k, __builtin_amdgcn_fmed3f(top - __builtin_rintf(v[4 * q + k] * inverse), 0.0f, 255.0f));
             const unsigned c = 4 * (q * L + sub);
-            unsigned code[4];
+            if (live && c + 4 <= C) {
+                typedef unsigned Word __attribute__((aligned(1)));
+                *reinterpret_cast<Word *>(out + c) = packed;
+            } else if (live) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float z = fminf(fmaxf(v[4 * q + k], -CE_CLAMP), CE_CLAMP);
-                code[k] = (unsigned)fminf(top - __builtin_rintf(z * inverse), 255.0f);
-            }
-            if (c + 4 <= C) {
-                dm::Quad<uint8_t>::type t;
-                t.x = (uint8_t)code[0]; t.y = (uint8_t)code[1]; t.z = (uint8_t)code[2]; t.w = (uint8_t)code[3];
-                *reinterpret_cast<dm::Quad<uint8_t>::type *>(out + c) = t;
-            } else {
-#pragma unroll
-                for (unsigned k = 0; k < 4; ++k)
-                    if (c + k < C) out[c + k] = (uint8_t)code[k];
+                for (unsigned k = 0; k < 3; ++k)
+                    if (c + k < C) out[c + k] = (uint8_t)(packed >> (8 * k));
             }
         }
-        if (sub == 0) steps[row] = (int8_t)(sum == sum ? e : NOT_A_NUMBER);
+        if (sub == 0 && live) steps[row] = (int8_t)(sum == sum ? e : NOT_A_NUMBER);
     }
     if (bad) dm::raise_status(status, DM_ST_LABEL_RANGE);
     const double a = block_sum((double)num, lds);
@@ -307,49 +390,68 @@ __global__ __launch_bounds__(CLS_THREADS) void ce_saved_kernel(const T *__restri
     }
 }
 
-template <typename T, int NQ, int L>
+template <int NQ, int L, bool WIDE>
 __global__ __launch_bounds__(CLS_THREADS) void ce_from_saved_kernel(const uint8_t *__restrict__ codes, const int8_t *__restrict__ steps,
                                                                     const int64_t *__restrict__ cls, const float *__restrict__ weight,
                                                                     const unsigned rows, const unsigned C,
                                                                     const int64_t ignore_index, const float *__restrict__ inv_weight,
-                                                                    const float *__restrict__ grad_loss, T *__restrict__ grad)
+                                                                    const float *__restrict__ grad_loss, const int dtype,
+                                                                    void *__restrict__ grad)
 {
+    typedef unsigned Word __attribute__((aligned(1)));
+    constexpr int N = 4 * NQ;
     const unsigned sub = threadIdx.x & (L - 1);
     constexpr unsigned ROWS = CLS_THREADS / L;
+    const unsigned stride = gridDim.x * ROWS;
     const float scale = inv_weight[0] * grad_loss[0];
-    for (unsigned r0 = blockIdx.x * ROWS; r0 < rows; r0 += gridDim.x * ROWS) {
+    unsigned next[NQ];
+    int next_e = 0;
+    int64_t next_y = 0;
+    auto fetch = [&](unsigned row) {
+        const unsigned r = min(row, rows - 1);
+        next_y = cls[r];
+        next_e = steps[r];
+        const uint8_t *in = codes + (size_t)r * C;
+        if (NQ == 1 && L == 1 && C < 4) {
+            next[0] = in[0] | (unsigned)in[min(1u, C - 1)] << 8 | (unsigned)in[C - 1] << 16;
+            return;
+        }
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) next[q] = *reinterpret_cast<const Word *>(in + min(4 * (q * L + sub), C - 4));
+    };
+    if (blockIdx.x * ROWS < rows) fetch(blockIdx.x * ROWS + threadIdx.x / L);
+    for (unsigned r0 = blockIdx.x * ROWS; r0 < rows; r0 += stride) {
         const unsigned row = r0 + threadIdx.x / L;
         const bool live = row < rows;
-        const size_t base = (size_t)(live ? row : 0) * C;
-        const int e = steps[live ? row : 0];
+        const int64_t y = next_y;
+        const int e = next_e;
+        float p[N];
+#pragma unroll
+        for (int q = 0; q < NQ; ++q)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) p[4 * q + k] = (float)((next[q] >> (8 * k)) & 255u);
+        if (r0 + stride < rows) fetch(row + stride);
+        bool bad = false;
+        const float w = row_weight(y, C, ignore_index, weight, &bad);
+        dm::place_row<NQ, L>(p, sub, C, __builtin_huge_valf());
         const float step = e == NOT_A_NUMBER ? __builtin_nanf("") : -power_of_two(e) * LOG2E;
-        float p[4 * NQ];
         float sum = 0.0f;
 #pragma unroll
-        for (int q = 0; q < NQ; ++q) {
-            float t[4];
-            dm::load_quad(codes + base, 4 * (q * L + sub), C, __builtin_huge_valf(), t);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                p[4 * q + k] = __builtin_amdgcn_exp2f(t[k] * step);
-                sum += p[4 * q + k];
-            }
+        for (int j = 0; j < N; ++j) {
+            p[j] = __builtin_amdgcn_exp2f(p[j] * step);
+            sum += p[j];
         }
         sum = dm::over_group<L>(sum, dm::Add());
-        if (!live) continue;
-        bool bad = false;
-        const int64_t y = cls[row];
-        const float w = row_weight(y, C, ignore_index, weight, &bad);
         const float inv = __builtin_amdgcn_rcpf(sum), ws = w * scale;
+        // the place of the row's own logit in the lane's quads (its first is at 4 sub)
+        const unsigned hot = w != 0.0f ? (unsigned)y - 4 * sub : 0xFFFFFFFFu;
 #pragma unroll
-        for (int q = 0; q < NQ; ++q) {
-            const unsigned c = 4 * (q * L + sub);
-            float g[4];
+        for (int j = 0; j < N; ++j) p[j] = (p[j] * inv - (hot == (unsigned)(4 * (j >> 2) * L + (j & 3)) ? 1.0f : 0.0f)) * ws;
+        if (w == 0.0f) {
 #pragma unroll
-            for (unsigned k = 0; k < 4; ++k)
-                g[k] = w == 0.0f ? 0.0f : (p[4 * q + k] * inv - ((int64_t)(c + k) == y ? 1.0f : 0.0f)) * ws;
-            dm::store_quad(grad + base, c, C, g);
+            for (int j = 0; j < N; ++j) p[j] = 0.0f;
         }
+        if (live) dm::store_row<NQ, L, WIDE>(grad, dtype, (size_t)row * C, sub, C, p);
     }
 }
 
@@ -509,29 +611,79 @@ void launch_focal_from_saved(const uint8_t *codes, const int32_t *heads, const i
 
 constexpr unsigned WIDEST = 2048;      // logits of a row that a wavefront keeps in registers
 
+// Lanes per row and quads per lane.
+struct Form {
+    int NQ, L;
+};
+Form ce_form(unsigned C)
+{
+    if (C <= 8) return {C <= 4 ? 1 : 2, 1};
+    if (C <= 16) return {2, 2};
+    if (C <= 32) return {2, 4};
+    if (C <= 64) return {2, 8};
+    if (C <= 128) return {C <= 96 ? 3 : 4, 8};
+    if (C <= 256) return {C <= 192 ? 3 : 4, 16};
+    if (C <= 512) return {C <= 384 ? 3 : 4, 32};
+    if (C <= 1024) return {C <= 768 ? 3 : 4, 64};
+    return {C <= 1280 ? 5 : C <= 1536 ? 6 : 8, 64};
+}
+template <typename F>
+void with_ce_form(unsigned C, F &&f)
+{
+    auto as = [&](auto nq, auto l) { f(nq, l); };
+#define DM_FORM(NQ_, L_) as(std::integral_constant<int, NQ_>(), std::integral_constant<int, L_>())
+    const Form form = ce_form(C);
+    switch (form.L) {
+    case 1: return form.NQ == 1 ? DM_FORM(1, 1) : DM_FORM(2, 1);
+    case 2: return DM_FORM(2, 2);
+    case 4: return DM_FORM(2, 4);
+    case 8: return form.NQ == 2 ? DM_FORM(2, 8) : form.NQ == 3 ? DM_FORM(3, 8) : DM_FORM(4, 8);
+    case 16: return form.NQ == 3 ? DM_FORM(3, 16) : DM_FORM(4, 16);
+    case 32: return form.NQ == 3 ? DM_FORM(3, 32) : DM_FORM(4, 32);
+    default:
+        switch (form.NQ) {
+        case 3: return DM_FORM(3, 64);
+        case 4: return DM_FORM(4, 64);
+        case 5: return DM_FORM(5, 64);
+        case 6: return DM_FORM(6, 64);
+        default: return DM_FORM(8, 64);
+        }
+    }
+#undef DM_FORM
+}
 unsigned ce_blocks(unsigned rows, unsigned C)
 {
-    const unsigned rows_per_block = C <= WIDEST ? CLS_THREADS / 64 : 1;
+    const unsigned rows_per_block = C <= WIDEST ? (unsigned)(CLS_THREADS / ce_form(C).L) : 1u;
     return std::max(1u, std::min((unsigned)CLS_MAX_BLOCKS, (rows + rows_per_block - 1) / rows_per_block));
 }
 template <typename T>
-void launch_ce_saved(const void *logits, const int64_t *cls, const float *weight, unsigned rows, unsigned C, int64_t ignore_index,
+void launch_ce_saved(const void *logits, int dtype, const int64_t *cls, const float *weight, unsigned rows, unsigned C, int64_t ignore_index,
                      uint8_t *codes, int8_t *steps, double *partials, int32_t *status, unsigned blocks, hipStream_t st)
 {
-    auto kernel = C <= 256 ? ce_saved_kernel<T, 1, 64> : C <= 512 ? ce_saved_kernel<T, 2, 64> : C <= 1024 ? ce_saved_kernel<T, 4, 64>
-                  : C <= WIDEST ? ce_saved_kernel<T, 8, 64> : ce_saved_wide_kernel<T>;
-    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(CLS_THREADS), 0, st, static_cast<const T *>(logits), cls, weight, rows, C,
-                       ignore_index, codes, steps, partials, status);
+    if (C > WIDEST) {
+        hipLaunchKernelGGL(ce_saved_wide_kernel<T>, dim3(blocks), dim3(CLS_THREADS), 0, st, static_cast<const T *>(logits), cls, weight,
+                           rows, C, ignore_index, codes, steps, partials, status);
+        return;
+    }
+    with_ce_form(C, [&](auto nq, auto l) {
+        hipLaunchKernelGGL((ce_saved_kernel<decltype(nq)::value, decltype(l)::value, sizeof(T) == 4>), dim3(blocks), dim3(CLS_THREADS), 0,
+                           st, logits, dtype, cls, weight, rows, C, ignore_index, codes, steps, partials, status);
+    });
 }
 template <typename T>
-void launch_ce_from_saved(const uint8_t *codes, const int8_t *steps, const int64_t *cls, const float *weight, unsigned rows, unsigned C,
-                          int64_t ignore_index, const float *inv_weight, const float *grad_loss, void *grad, unsigned blocks,
+void launch_ce_from_saved(const uint8_t *codes, const int8_t *steps, int dtype, const int64_t *cls, const float *weight, unsigned rows,
+                          unsigned C, int64_t ignore_index, const float *inv_weight, const float *grad_loss, void *grad, unsigned blocks,
                           hipStream_t st)
 {
-    auto kernel = C <= 256 ? ce_from_saved_kernel<T, 1, 64> : C <= 512 ? ce_from_saved_kernel<T, 2, 64>
-                  : C <= 1024 ? ce_from_saved_kernel<T, 4, 64> : C <= WIDEST ? ce_from_saved_kernel<T, 8, 64> : ce_from_saved_wide_kernel<T>;
-    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(CLS_THREADS), 0, st, codes, steps, cls, weight, rows, C, ignore_index, inv_weight,
-                       grad_loss, static_cast<T *>(grad));
+    if (C > WIDEST) {
+        hipLaunchKernelGGL(ce_from_saved_wide_kernel<T>, dim3(blocks), dim3(CLS_THREADS), 0, st, codes, steps, cls, weight, rows, C,
+                           ignore_index, inv_weight, grad_loss, static_cast<T *>(grad));
+        return;
+    }
+    with_ce_form(C, [&](auto nq, auto l) {
+        hipLaunchKernelGGL((ce_from_saved_kernel<decltype(nq)::value, decltype(l)::value, sizeof(T) == 4>), dim3(blocks), dim3(CLS_THREADS),
+                           0, st, codes, steps, cls, weight, rows, C, ignore_index, inv_weight, grad_loss, dtype, grad);
+    });
 }
 
 bool known(int dtype) { return dtype == DM_F32 || dtype == DM_BF16 || dtype == DM_F16; }
@@ -557,8 +709,8 @@ extern "C" int dm_focal_loss_saved(const void *logits, int dtype, const int64_t 
     if (((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(heads)) & 3) != 0) return DM_E_INVALID_ARG;
     hipStream_t st = static_cast<hipStream_t>(stream);
     const unsigned n = (unsigned)(rows * C);
-    const unsigned quads = (n + 127) / 128 * BLOCK_QUADS;
-    const int blocks = (int)std::max(1u, std::min((unsigned)CLS_MAX_BLOCKS, (quads + CLS_THREADS - 1) / CLS_THREADS));
+    const unsigned quads = (n + 127) / 128 * BLOCK_QUADS, per_block = CLS_THREADS * FORWARD_QUADS;
+    const int blocks = (int)std::max(1u, std::min((unsigned)CLS_MAX_BLOCKS, (quads + per_block - 1) / per_block));
     const FocalParams fp{alpha, gamma, scale, ignore_index, use_ignore};
     auto launch = dtype == DM_F32 ? launch_focal_saved<float> : dtype == DM_BF16 ? launch_focal_saved<dm::bf16_t> : launch_focal_saved<dm::half_t>;
     launch(logits, target_cls, n, (unsigned)C, (unsigned)rows, fp, codes, heads, partials, status, blocks, st);
@@ -577,8 +729,8 @@ extern "C" int dm_focal_loss_from_saved(const uint8_t *codes, const int32_t *hea
     if (((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(heads)) & 3) != 0) return DM_E_INVALID_ARG;
     if (rows == 0) return DM_OK;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    const unsigned n = (unsigned)(rows * C), quads = (n + 3) / 4;
-    const int blocks = (int)std::min((unsigned)CLS_MAX_BLOCKS, (quads + CLS_THREADS - 1) / CLS_THREADS);
+    const unsigned n = (unsigned)(rows * C), quads = (n + 3) / 4, per_block = CLS_THREADS * BACKWARD_QUADS;
+    const int blocks = (int)std::min((unsigned)CLS_MAX_BLOCKS, (quads + per_block - 1) / per_block);
     const FocalParams fp{alpha, gamma, scale, ignore_index, use_ignore};
     auto launch = dtype == DM_F32 ? launch_focal_from_saved<float>
                   : dtype == DM_BF16 ? launch_focal_from_saved<dm::bf16_t> : launch_focal_from_saved<dm::half_t>;
@@ -596,7 +748,7 @@ extern "C" int dm_cross_entropy_saved(const void *logits, int dtype, const int64
     hipStream_t st = static_cast<hipStream_t>(stream);
     const unsigned blocks = ce_blocks((unsigned)rows, (unsigned)C);
     auto launch = dtype == DM_F32 ? launch_ce_saved<float> : dtype == DM_BF16 ? launch_ce_saved<dm::bf16_t> : launch_ce_saved<dm::half_t>;
-    launch(logits, target_cls, weight, (unsigned)rows, (unsigned)C, ignore_index, codes, steps, partials, status, blocks, st);
+    launch(logits, dtype, target_cls, weight, (unsigned)rows, (unsigned)C, ignore_index, codes, steps, partials, status, blocks, st);
     rc = dm::check_hip(hipGetLastError(), "ce_saved_kernel launch");
     if (rc != DM_OK) return rc;
     hipLaunchKernelGGL(cls_loss_finish_kernel<false>, dim3(1), dim3(CLS_THREADS), 0, st, partials, (int)blocks, 1.0f, loss_out);
@@ -613,7 +765,7 @@ extern "C" int dm_cross_entropy_from_saved(const uint8_t *codes, const int8_t *s
     if (!inv_weight) return DM_E_INVALID_ARG;
     auto launch = dtype == DM_F32 ? launch_ce_from_saved<float>
                   : dtype == DM_BF16 ? launch_ce_from_saved<dm::bf16_t> : launch_ce_from_saved<dm::half_t>;
-    launch(codes, steps, target_cls, weight, (unsigned)rows, (unsigned)C, ignore_index, inv_weight, grad_loss, grad_out,
+    launch(codes, steps, dtype, target_cls, weight, (unsigned)rows, (unsigned)C, ignore_index, inv_weight, grad_loss, grad_out,
            ce_blocks((unsigned)rows, (unsigned)C), static_cast<hipStream_t>(stream));
     return dm::check_hip(hipGetLastError(), "ce_from_saved_kernel launch");
 }
