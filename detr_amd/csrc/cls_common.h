@@ -49,6 +49,7 @@ __global__ __launch_bounds__(CLS_THREADS) void cls_loss_finish_kernel(const doub
 {
     __shared__ double lds[CLS_THREADS / 64];
     double a = 0.0, b = 0.0;
+#pragma unroll 8
     for (int i = threadIdx.x; i < blocks; i += CLS_THREADS) {
         if (FOCAL) a += partials[i];
         else { a += partials[2 * i]; b += partials[2 * i + 1]; }

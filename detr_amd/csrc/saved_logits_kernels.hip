@@ -18,6 +18,7 @@
 //
 // The gradient is that of the loss at the decoded logits; the loss itself is of the logits as they came.
 #include <algorithm>
+#include <climits>
 
 #include "cls_common.h"
 #include "lanes.h"
@@ -75,71 +76,90 @@ __device__ __forceinline__ FocalParts focal_parts(float z, float gamma)
     return f;
 }
 
-// Rows and columns of a thread's quads of four consecutive logits, `stride` quads apart, walked by additions.
+// A row's class as the focal loss needs it, 64 bits looked at once: the place of its positive logit counted from the row's
+// first, or none; and whether the row may not count (ignored, or a class that is none), which `row_code` then settles.
+__device__ __forceinline__ bool class_place(int64_t label, unsigned C, const FocalParams &fp, int *place)
+{
+    const unsigned low = (unsigned)label;
+    const bool small = (unsigned)((uint64_t)label >> 32) == 0;
+    *place = small && low < C ? (int)low : INT_MIN / 2;
+    return !(small && low <= C) || (fp.use_ignore && label == fp.ignore_index);
+}
+
+// The focal kernels' share of the flat array: 8 lanes take a block of 128 logits, each four quads of four consecutive ones,
+// 32 logits apart (a load of the 8 lanes is 128 bytes of float32).  With four logits per lane, and 32 lanes to agree on a
+// block's step, the agreement cost as much as half of the loss itself.
+constexpr unsigned BLOCK = 128, LANES = 8, QUADS = 4, BLOCKS_AT_A_TIME = CLS_THREADS / LANES;
+
+// Rows and columns of a lane's quads, walked by additions: from quad to quad of a block, and from block to block.
 struct Walk {
-    unsigned row, col, step_row, step_col, C;
-    __device__ __forceinline__ Walk(unsigned quad, unsigned stride, unsigned C_) : C(C_)
+    unsigned row, col, C, quad_row, quad_col, block_row, block_col;
+    __device__ __forceinline__ Walk(unsigned block, unsigned stride, unsigned sub, unsigned C_) : C(C_)
     {
-        step_row = (stride << 2) / C;
-        step_col = (stride << 2) - step_row * C;
-        row = (quad << 2) / C;
-        col = (quad << 2) - row * C;
+        const unsigned first = block * BLOCK + 4 * sub, apart = 4 * LANES, far = stride * BLOCK;
+        row = first / C;
+        col = first - row * C;
+        quad_row = apart / C;
+        quad_col = apart - quad_row * C;
+        block_row = far / C;
+        block_col = far - block_row * C;
     }
-    __device__ __forceinline__ void next()
+    __device__ __forceinline__ void step(unsigned &r, unsigned &c, unsigned rows, unsigned cols) const
     {
-        col += step_col;
-        const bool over = col >= C;
-        col = over ? col - C : col;
-        row += step_row + (over ? 1u : 0u);
+        c += cols;
+        const bool over = c >= C;
+        c = over ? c - C : c;
+        r += rows + (over ? 1u : 0u);
     }
+    __device__ __forceinline__ void next_quad(unsigned &r, unsigned &c) const { step(r, c, quad_row, quad_col); }
+    __device__ __forceinline__ void next_block() { step(row, col, block_row, block_col); }
 };
 
-// The rows of a quad: with two or more classes four consecutive logits lie in at most two (the flat array's quads start at
-// multiples of four, so that also holds for two classes); with one, each is a row.  `ask` loads their classes, `settle` makes
-// of them which logits are positive and which count.
+// The rows of a lane's quads.  With two or more classes four consecutive logits lie in at most two rows (quads start at
+// multiples of four of the flat array, so that also holds for two classes); with one, each is a row.
 template <bool ONE_CLASS>
-struct QuadRows {
+struct BlockRows {
     static constexpr unsigned ROWS = ONE_CLASS ? 4 : 2;
-    int64_t label[ROWS];
-    unsigned col;
-    int code[ROWS];
-    int hot[ROWS];        // place of the row's positive logit in the quad, if it is there
-    bool skipped;         // a row is ignored (or bad): the general answer of `counts` is needed
+    int64_t label[QUADS][ROWS];
+    unsigned col[QUADS];
+    int hot[QUADS][ROWS];       // place of the row's positive logit in the quad, if it is there
+    bool skipped;               // some row may not count: `counts` has to be asked
 
-    __device__ __forceinline__ void ask(const int64_t *cls, unsigned row, unsigned col_, unsigned rows)
+    // (first: of the lane's logits in the flat array)
+    __device__ __forceinline__ void ask(const int64_t *cls, const Walk &at, unsigned first, unsigned rows)
     {
-        col = col_;
+        unsigned r = at.row, c = at.col;
 #pragma unroll
-        for (unsigned k = 0; k < ROWS; ++k) label[k] = cls[min(row + k, rows - 1)];
+        for (unsigned q = 0; q < QUADS; ++q) {
+            col[q] = c;
+#pragma unroll
+            for (unsigned k = 0; k < ROWS; ++k) label[q][k] = cls[min((ONE_CLASS ? first + 4 * LANES * q : r) + k, rows - 1)];
+            if (!ONE_CLASS) at.next_quad(r, c);
+        }
     }
-    __device__ __forceinline__ void settle(unsigned C, const FocalParams &fp, bool *bad)
+    __device__ __forceinline__ void settle(unsigned C, const FocalParams &fp)
     {
         skipped = false;
 #pragma unroll
-        for (unsigned k = 0; k < ROWS; ++k) {
-            code[k] = row_code(label[k], C, fp);
-            skipped |= code[k] < 0;
-            *bad |= code[k] == ROW_BAD;
-            const int start = ONE_CLASS ? (int)k : (k ? (int)(C - col) : -(int)col);      // place of the row's first logit
-            hot[k] = (unsigned)code[k] < C ? start + code[k] : -1;
-        }
+        for (unsigned q = 0; q < QUADS; ++q)
+#pragma unroll
+            for (unsigned k = 0; k < ROWS; ++k) {
+                int place;
+                skipped |= class_place(label[q][k], C, fp, &place);
+                hot[q][k] = place + (ONE_CLASS ? (int)k : k ? (int)(C - col[q]) : -(int)col[q]);
+            }
     }
-    __device__ __forceinline__ bool positive(unsigned k) const
+    __device__ __forceinline__ bool positive(unsigned q, unsigned k) const
     {
-        if (ONE_CLASS) return hot[k] == (int)k;
-        return hot[0] == (int)k || hot[1] == (int)k;
+        if (ONE_CLASS) return hot[q][k] == (int)k;
+        return hot[q][0] == (int)k || hot[q][1] == (int)k;
     }
-    __device__ __forceinline__ bool counts(unsigned k, unsigned C) const
+    __device__ __forceinline__ bool counts(unsigned q, unsigned k, unsigned C, const FocalParams &fp, bool *bad) const
     {
-        return (ONE_CLASS ? code[k] : col + k >= C ? code[1] : code[0]) >= 0;
+        const int code = row_code(ONE_CLASS ? label[q][k] : col[q] + k >= C ? label[q][1] : label[q][0], C, fp);
+        *bad |= code == ROW_BAD;
+        return code >= 0;
     }
-};
-
-constexpr unsigned BLOCK_QUADS = 32;      // 128 logits: 32 lanes with four each
-constexpr int FORWARD_QUADS = 2, BACKWARD_QUADS = 4;      // quads a thread asks for before it works on them
-
-struct Quad4 {
-    float v[4];
 };
 
 // Loss, bytes and heads.  codes NULL: the loss alone.
@@ -150,80 +170,95 @@ __global__ __launch_bounds__(CLS_THREADS) void focal_saved_kernel(const T *__res
                                                                   int32_t *__restrict__ heads, double *__restrict__ partials,
                                                                   int32_t *__restrict__ status)
 {
+    typedef typename dm::Quad<T>::type Four;
     __shared__ double lds[CLS_THREADS / 64];
-    const unsigned whole = n / 128 * BLOCK_QUADS;                     // quads of whole blocks
-    const unsigned stride = gridDim.x * CLS_THREADS;
+    const unsigned blocks = n / BLOCK, stride = gridDim.x * BLOCKS_AT_A_TIME;      // whole blocks
+    const unsigned sub = threadIdx.x & (LANES - 1), lane = threadIdx.x & 63;
     const float alpha1 = fp.alpha >= 0.0f ? fp.alpha : 1.0f, alpha0 = fp.alpha >= 0.0f ? 1.0f - fp.alpha : 1.0f;
     float acc = 0.0f;
     bool bad = false;
 
-    // the quad i, whose first logit is `first`; `there`: how many of its logits there are
-    auto work = [&](unsigned i, const float (&v)[4], QuadRows<ONE_CLASS> &q, unsigned there) {
-        q.settle(C, fp, &bad);
-        float term[4], c[4];
-        float high = -FOCAL_CLAMP, low = FOCAL_CLAMP;
+    // a block with its logits and rows; `end`: logits of the flat array (whole blocks lie before it)
+    auto work = [&](unsigned block, const float (&v)[4 * QUADS], BlockRows<ONE_CLASS> &rows_of, bool whole) {
+        const unsigned first = block * BLOCK + 4 * sub;
+        auto inside = [&](unsigned q, unsigned k) { return whole || first + 4 * LANES * q + k < n; };
+        rows_of.settle(C, fp);
+        float c[4 * QUADS], high = -FOCAL_CLAMP, low = FOCAL_CLAMP, sum = 0.0f;
         bool nan = false;
 #pragma unroll
-        for (unsigned k = 0; k < 4; ++k) {
-            const bool positive = q.positive(k);
-            const FocalParts f = focal_parts<GAMMA2>(positive ? -v[k] : v[k], fp.gamma);
-            term[k] = (positive ? alpha1 : alpha0) * (f.softplus * f.power);
-            c[k] = __builtin_amdgcn_fmed3f(v[k], -FOCAL_CLAMP, FOCAL_CLAMP);
-            nan |= k < there && v[k] != v[k];
-            if (k < there) {
-                low = __builtin_amdgcn_fmed3f(low, c[k], -FOCAL_CLAMP);
-                high = __builtin_amdgcn_fmed3f(high, c[k], FOCAL_CLAMP);
-            }
-        }
-        if (q.skipped || there < 4) {
+        for (unsigned q = 0; q < QUADS; ++q) {
+            float term[4];
 #pragma unroll
-            for (unsigned k = 0; k < 4; ++k) term[k] = k < there && q.counts(k, C) ? term[k] : 0.0f;
+            for (unsigned k = 0; k < 4; ++k) {
+                const float x = v[4 * q + k];
+                const bool positive = rows_of.positive(q, k);
+                const FocalParts f = focal_parts<GAMMA2>(positive ? -x : x, fp.gamma);
+                term[k] = (positive ? alpha1 : alpha0) * (f.softplus * f.power);
+                c[4 * q + k] = __builtin_amdgcn_fmed3f(x, -FOCAL_CLAMP, FOCAL_CLAMP);
+                if (inside(q, k)) {
+                    nan |= x != x;
+                    low = __builtin_amdgcn_fmed3f(low, c[4 * q + k], -FOCAL_CLAMP);
+                    high = __builtin_amdgcn_fmed3f(high, c[4 * q + k], FOCAL_CLAMP);
+                }
+            }
+            if (rows_of.skipped || !whole) {
+#pragma unroll
+                for (unsigned k = 0; k < 4; ++k) term[k] = inside(q, k) && rows_of.counts(q, k, C, fp, &bad) ? term[k] : 0.0f;
+            }
+            sum += (term[0] + term[1]) + (term[2] + term[3]);
         }
-        acc += (term[0] + term[1]) + (term[2] + term[3]);
-        if (codes) {
-            high = dm::largest<32>(high);
-            low = -dm::largest<32>(-low);
-            const unsigned long long nans = __ballot(nan);
-            const bool block_nan = (unsigned)(nans >> (threadIdx.x & 32)) != 0;
-            const int e = step_exponent(high, low, FOCAL_COARSEST);
-            const float inverse = power_of_two(-e);
-            const float top = __builtin_rintf(high * inverse);
+        acc += sum;
+        if (!codes) return;
+        high = dm::largest<LANES>(high);
+        low = -dm::largest<LANES>(-low);
+        const bool block_nan = ((__ballot(nan) >> (lane & ~(LANES - 1))) & ((1u << LANES) - 1)) != 0;
+        const int e = step_exponent(high, low, FOCAL_COARSEST);
+        const float inverse = power_of_two(-e);
+        const float top = __builtin_rintf(high * inverse);
+#pragma unroll
+        for (unsigned q = 0; q < QUADS; ++q) {
             unsigned packed = 0;
 #pragma unroll
             for (unsigned k = 0; k < 4; ++k)
-                packed = pack_code(packed, k, k < there ? top - __builtin_rintf(c[k] * inverse) : 0.0f);
-            codes[i] = packed;
-            if ((threadIdx.x & 31) == 0) heads[i / BLOCK_QUADS] = block_nan ? (NOT_A_NUMBER & 255) : (int)top * 256 | (e & 255);
+                packed = pack_code(packed, k, inside(q, k) ? top - __builtin_rintf(c[4 * q + k] * inverse) : 0.0f);
+            codes[block * (BLOCK / 4) + LANES * q + sub] = packed;
         }
+        if (sub == 0) heads[block] = block_nan ? (NOT_A_NUMBER & 255) : (int)top * 256 | (e & 255);
     };
 
-    unsigned i = blockIdx.x * CLS_THREADS + threadIdx.x;
-    Walk at(i, stride, C);
-    // (the 32 lanes of a block run the same trips: the strides are multiples of 32)
-    for (; i < whole; i += FORWARD_QUADS * stride) {
-        Quad4 v[FORWARD_QUADS];
-        QuadRows<ONE_CLASS> q[FORWARD_QUADS];
+    unsigned block = blockIdx.x * BLOCKS_AT_A_TIME + threadIdx.x / LANES;
+    Walk at(block, stride, sub, C);
+    // (the lanes of a block run the same trips)
+    for (; block < blocks; block += stride) {
+        const unsigned first = block * BLOCK + 4 * sub;
+        Four t[QUADS];
 #pragma unroll
-        for (int u = 0; u < FORWARD_QUADS; ++u) {
-            const unsigned j = min(i + u * stride, whole - 1);
-            const typename dm::Quad<T>::type t = *reinterpret_cast<const typename dm::Quad<T>::type *>(x + (size_t)(j << 2));
-            v[u].v[0] = (float)t.x; v[u].v[1] = (float)t.y; v[u].v[2] = (float)t.z; v[u].v[3] = (float)t.w;
-            q[u].ask(cls, ONE_CLASS ? j << 2 : at.row, at.col, rows);
-            if (!ONE_CLASS) at.next();
+        for (unsigned q = 0; q < QUADS; ++q) t[q] = *reinterpret_cast<const Four *>(x + first + 4 * LANES * q);
+        BlockRows<ONE_CLASS> rows_of;
+        rows_of.ask(cls, at, first, rows);
+        at.next_block();
+        float v[4 * QUADS];
+#pragma unroll
+        for (unsigned q = 0; q < QUADS; ++q) {
+            v[4 * q] = (float)t[q].x;
+            v[4 * q + 1] = (float)t[q].y;
+            v[4 * q + 2] = (float)t[q].z;
+            v[4 * q + 3] = (float)t[q].w;
         }
-#pragma unroll
-        for (int u = 0; u < FORWARD_QUADS; ++u)
-            if (i + u * stride < whole) work(i + u * stride, v[u].v, q[u], 4);
+        work(block, v, rows_of, true);
     }
     // the last block, if it is not a whole one
-    if (blockIdx.x == gridDim.x - 1 && threadIdx.x < BLOCK_QUADS && (n & 127)) {
-        const unsigned j = whole + threadIdx.x, first = j << 2;
-        float v[4];
-        dm::load_quad(x, min(first, n), n, 0.0f, v);
-        QuadRows<ONE_CLASS> q;
-        const unsigned row = min(first, n - 1) / C;
-        q.ask(cls, row, min(first, n - 1) - row * C, rows);
-        work(j, v, q, first < n ? min(4u, n - first) : 0u);
+    if (blockIdx.x == gridDim.x - 1 && threadIdx.x < LANES && n % BLOCK != 0) {
+        const unsigned first = blocks * BLOCK + 4 * sub;
+        float v[4 * QUADS];
+#pragma unroll
+        for (unsigned q = 0; q < QUADS; ++q)
+#pragma unroll
+            for (unsigned k = 0; k < 4; ++k) v[4 * q + k] = (float)x[min(first + 4 * LANES * q + k, n - 1)];
+        const Walk last(blocks, 0, sub, C);
+        BlockRows<ONE_CLASS> rows_of;
+        rows_of.ask(cls, last, first, rows);
+        work(blocks, v, rows_of, false);
     }
     if (bad) dm::raise_status(status, DM_ST_LABEL_RANGE);
     const double total = block_sum((double)acc, lds);
@@ -237,48 +272,51 @@ __global__ __launch_bounds__(CLS_THREADS) void focal_from_saved_kernel(const uns
                                                                        const unsigned C, const unsigned rows, const FocalParams fp,
                                                                        const float *__restrict__ grad_loss, T *__restrict__ grad)
 {
-    const unsigned quads = (n + 3) / 4;
-    const unsigned stride = gridDim.x * CLS_THREADS;
+    typedef typename dm::Quad<T>::type Four;
+    const unsigned blocks = (n + BLOCK - 1) / BLOCK, whole = n / BLOCK, stride = gridDim.x * BLOCKS_AT_A_TIME;
+    const unsigned sub = threadIdx.x & (LANES - 1);
     const float scale = fp.scale * grad_loss[0];
     const float gamma = GAMMA2 ? 2.0f : fp.gamma;
     // (the gradient of a positive logit has the other sign)
     const float alpha1 = -scale * (fp.alpha >= 0.0f ? fp.alpha : 1.0f), alpha0 = scale * (fp.alpha >= 0.0f ? 1.0f - fp.alpha : 1.0f);
-    unsigned i = blockIdx.x * CLS_THREADS + threadIdx.x;
-    Walk at(i, stride, C);
-    for (; i < quads; i += BACKWARD_QUADS * stride) {
-        unsigned packed[BACKWARD_QUADS];
-        int head[BACKWARD_QUADS];
-        QuadRows<ONE_CLASS> q[BACKWARD_QUADS];
+    unsigned block = blockIdx.x * BLOCKS_AT_A_TIME + threadIdx.x / LANES;
+    Walk at(block, stride, sub, C);
+    for (; block < blocks; block += stride) {
+        const unsigned first = block * BLOCK + 4 * sub;
+        unsigned packed[QUADS];
 #pragma unroll
-        for (int u = 0; u < BACKWARD_QUADS; ++u) {
-            const unsigned j = min(i + u * stride, quads - 1);
-            packed[u] = codes[j];
-            head[u] = heads[j / BLOCK_QUADS];
-            q[u].ask(cls, ONE_CLASS ? j << 2 : at.row, at.col, rows);
-            if (!ONE_CLASS) at.next();
-        }
+        for (unsigned q = 0; q < QUADS; ++q) packed[q] = codes[block * (BLOCK / 4) + LANES * q + sub];
+        const int head = heads[block];
+        BlockRows<ONE_CLASS> rows_of;
+        rows_of.ask(cls, at, first, rows);
+        at.next_block();
+        rows_of.settle(C, fp);
+        const int e = (int)(int8_t)(head & 255);
+        const float step = e == NOT_A_NUMBER ? __builtin_nanf("") : power_of_two(e);
+        const float top = (float)(head >> 8) * step;
 #pragma unroll
-        for (int u = 0; u < BACKWARD_QUADS; ++u) {
-            if (i + u * stride >= quads) continue;
-            bool bad = false;
-            q[u].settle(C, fp, &bad);
-            const int e = (int)(int8_t)(head[u] & 255);
-            const float step = e == NOT_A_NUMBER ? __builtin_nanf("") : power_of_two(e);
-            const float top = (float)(head[u] >> 8) * step;
+        for (unsigned q = 0; q < QUADS; ++q) {
             float g[4];
 #pragma unroll
             for (unsigned k = 0; k < 4; ++k) {
-                const bool positive = q[u].positive(k);
-                const float x = __builtin_fmaf((float)((packed[u] >> (8 * k)) & 255u), -step, top);      // (exact)
+                const bool positive = rows_of.positive(q, k);
+                const float x = __builtin_fmaf((float)((packed[q] >> (8 * k)) & 255u), -step, top);      // (exact)
                 const FocalParts f = focal_parts<GAMMA2>(positive ? -x : x, fp.gamma);
                 const float slope = f.power * __builtin_fmaf(gamma, f.softplus * f.rest, f.sigmoid);
                 g[k] = (positive ? alpha1 : alpha0) * slope;
             }
-            if (q[u].skipped) {
+            if (rows_of.skipped) {
+                bool bad;
 #pragma unroll
-                for (unsigned k = 0; k < 4; ++k) g[k] = q[u].counts(k, C) ? g[k] : 0.0f;
+                for (unsigned k = 0; k < 4; ++k) g[k] = rows_of.counts(q, k, C, fp, &bad) ? g[k] : 0.0f;
             }
-            dm::store_quad(grad, (i + u * stride) << 2, n, g);
+            if (block < whole) {
+                Four t;
+                t.x = (T)g[0]; t.y = (T)g[1]; t.z = (T)g[2]; t.w = (T)g[3];
+                *reinterpret_cast<Four *>(grad + first + 4 * LANES * q) = t;
+            } else {
+                dm::store_quad(grad, first + 4 * LANES * q, n, g);
+            }
         }
     }
 }
@@ -609,6 +647,12 @@ void launch_focal_from_saved(const uint8_t *codes, const int32_t *heads, const i
                        rows, fp, grad_loss, static_cast<T *>(grad));
 }
 
+int focal_blocks(unsigned n)
+{
+    const unsigned per_block = BLOCK * BLOCKS_AT_A_TIME;
+    return (int)std::max(1u, std::min((unsigned)CLS_MAX_BLOCKS, n / per_block + (n % per_block != 0)));
+}
+
 constexpr unsigned WIDEST = 2048;      // logits of a row that a wavefront keeps in registers
 
 // Lanes per row and quads per lane.
@@ -709,8 +753,7 @@ extern "C" int dm_focal_loss_saved(const void *logits, int dtype, const int64_t 
     if (((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(heads)) & 3) != 0) return DM_E_INVALID_ARG;
     hipStream_t st = static_cast<hipStream_t>(stream);
     const unsigned n = (unsigned)(rows * C);
-    const unsigned quads = (n + 127) / 128 * BLOCK_QUADS, per_block = CLS_THREADS * FORWARD_QUADS;
-    const int blocks = (int)std::max(1u, std::min((unsigned)CLS_MAX_BLOCKS, (quads + per_block - 1) / per_block));
+    const int blocks = focal_blocks(n);
     const FocalParams fp{alpha, gamma, scale, ignore_index, use_ignore};
     auto launch = dtype == DM_F32 ? launch_focal_saved<float> : dtype == DM_BF16 ? launch_focal_saved<dm::bf16_t> : launch_focal_saved<dm::half_t>;
     launch(logits, target_cls, n, (unsigned)C, (unsigned)rows, fp, codes, heads, partials, status, blocks, st);
@@ -729,8 +772,8 @@ extern "C" int dm_focal_loss_from_saved(const uint8_t *codes, const int32_t *hea
     if (((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(heads)) & 3) != 0) return DM_E_INVALID_ARG;
     if (rows == 0) return DM_OK;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    const unsigned n = (unsigned)(rows * C), quads = (n + 3) / 4, per_block = CLS_THREADS * BACKWARD_QUADS;
-    const int blocks = (int)std::min((unsigned)CLS_MAX_BLOCKS, (quads + per_block - 1) / per_block);
+    const unsigned n = (unsigned)(rows * C);
+    const int blocks = focal_blocks(n);
     const FocalParams fp{alpha, gamma, scale, ignore_index, use_ignore};
     auto launch = dtype == DM_F32 ? launch_focal_from_saved<float>
                   : dtype == DM_BF16 ? launch_focal_from_saved<dm::bf16_t> : launch_focal_from_saved<dm::half_t>;
