@@ -61,6 +61,21 @@ __device__ __forceinline__ Place place_of(const RouterSets &a, unsigned block)
 // Sigmoid: sigmoid(x) times a constant of the row that keeps the largest from underflowing: with c = min(max x, 0),
 // t = exp(-|x| - c), sigmoid(x) exp(-c) = (x >= 0 ? 1 : t) / (1 + t exp(c)).  `rest` = 1 - sigmoid(x).
 __device__ __forceinline__ float softmax_weight(float x, float mx) { return __builtin_amdgcn_exp2f((x - mx) * LOG2E); }
+// All of a lane's.  exp(x - max) as 2^(x log2 e - (max log2 e)): the rounding of the product with the row's largest is the
+// same for the whole row, it drops out of p and is within the rounding of the logarithm of the sum.  Not so far from zero,
+// where that rounding is a step of the exponent and more.
+template <int N>
+__device__ __forceinline__ void softmax_weights(float (&x)[N], float mx)
+{
+    if (__any(!(__builtin_fabsf(mx) < 1024.0f))) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) x[j] = softmax_weight(x[j], mx);
+        return;
+    }
+    const float base = mx * LOG2E;
+#pragma unroll
+    for (int j = 0; j < N; ++j) x[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[j], LOG2E, -base));
+}
 __device__ __forceinline__ float sigmoid_weight(float x, float c, float exp_c, float *rest)
 {
     const float t = __builtin_amdgcn_exp2f((-__builtin_fabsf(x) - c) * LOG2E);
@@ -74,7 +89,7 @@ __device__ __forceinline__ float sigmoid_weight(float x, float c, float exp_c, f
 // number goes into the low ten (1023 - e for positive logits, e for negative ones, where a longer mantissa means smaller).  No
 // two are equal then, and the order is that of (logit, lowest index).  +infinity becomes a number that is larger than any.
 constexpr unsigned ABOVE_ALL = 0x7F7F8000u;
-__device__ __forceinline__ float order_f32(float x) { return x > -__builtin_huge_valf() ? x : -__builtin_huge_valf(); }
+__device__ __forceinline__ float order_f32(float x) { return dm::max3(x, -__builtin_huge_valf(), -__builtin_huge_valf()); }
 __device__ __forceinline__ float order_16(float x, unsigned e)
 {
     const float finite = __builtin_amdgcn_fmed3f(x + 0.0f, -__builtin_huge_valf(), __uint_as_float(ABOVE_ALL));      // (-0 is +0)
@@ -181,11 +196,9 @@ __global__ __launch_bounds__(RT_THREADS) void router_forward_kernel(const Router
                     sum += x[j];
                 }
             } else {
+                softmax_weights(x, mx);
 #pragma unroll
-                for (int j = 0; j < N; ++j) {
-                    x[j] = softmax_weight(x[j], mx);
-                    sum += x[j];
-                }
+                for (int j = 0; j < N; ++j) sum += x[j];
             }
             sum = dm::over_group<L>(sum, dm::Add());
             live = sum != 0.0f;                                // (a NaN makes it NaN)
@@ -230,16 +243,20 @@ __global__ __launch_bounds__(RT_THREADS) void router_forward_kernel(const Router
                 }
             }
             last = __builtin_amdgcn_fmed3f(last, -__FLT_MAX__, __builtin_huge_valf());       // (fewer than k: all that can be)
-            if (WIDE) {
-                unsigned chosen = 0;
+            unsigned chosen = 0;
 #pragma unroll
-                for (int j = 0; j < N; ++j) chosen += y[j] >= last ? 1u : 0u;
+            for (int j = 0; j < N; ++j) {
+                const unsigned one = y[j] >= last ? 1u : 0u;
+                cnt[j] += one;
+                if (WIDE) chosen += one;
+            }
+            if (WIDE) {
                 chosen = dm::over_group<L>(chosen, dm::Add());
                 again = __any(chosen > k);
-            }
-            if (!again) {
+                if (again) {
 #pragma unroll
-                for (int j = 0; j < N; ++j) cnt[j] += y[j] >= last ? 1u : 0u;
+                    for (int j = 0; j < N; ++j) cnt[j] -= y[j] >= last ? 1u : 0u;
+                }
             }
         }
         if (again) {
@@ -323,21 +340,6 @@ __global__ __launch_bounds__(RT_THREADS) void router_forward_kernel(const Router
 constexpr int FINISH_THREADS = 1024, FINISH_WAVES = FINISH_THREADS / 64;
 static_assert(RT_MAX_EXPERTS <= FINISH_THREADS, "a thread per expert");
 
-// Sum over the workgroup, in every thread.
-template <typename V>
-__device__ __forceinline__ V finish_sum(V v, V *lds)
-{
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = lds[0];
-#pragma unroll
-    for (int w = 1; w < FINISH_WAVES; ++w) v += lds[w];
-    return v;
-}
-
 template <bool SUMS, bool LOSS>
 __global__ __launch_bounds__(FINISH_THREADS) void router_finish_kernel(const RouterSets a, const unsigned *__restrict__ slots,
                                                                        const unsigned cols, const int64_t *__restrict__ given_counts,
@@ -407,19 +409,42 @@ __global__ __launch_bounds__(FINISH_THREADS) void router_finish_kernel(const Rou
         }
     }
     if (!LOSS) return;
-    double *sums = &p_lds[0][0];
-    unsigned long long *whole = &c_lds[0][0];
     long long mine = 0;
-    double mean = 0.0;
+    double dot = 0.0;
     if (tid < E) {
         const int64_t *shares = given_counts ? given_counts : SUMS ? nullptr : counts;
         mine = shares ? shares[(size_t)group * E + tid] : C[tid];
-        mean = SUMS ? P[tid] : means[(size_t)group * E + tid];
+        dot = (double)mine * (SUMS ? P[tid] : means[(size_t)group * E + tid]);
     }
-    rows = finish_sum(rows, whole);
-    const long long all = (long long)finish_sum((unsigned long long)mine, whole);
-    zs = finish_sum(zs, sums);
-    const double dot = finish_sum((double)mine * mean, sums);
+    // the four sums over the workgroup, in every thread, in one exchange
+    unsigned long long total = (unsigned long long)mine;
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) {
+        rows += __shfl_xor(rows, off);
+        total += __shfl_xor(total, off);
+        zs += __shfl_xor(zs, off);
+        dot += __shfl_xor(dot, off);
+    }
+    if ((tid & 63) == 0) {
+        c_lds[tid >> 6][0] = rows;
+        c_lds[tid >> 6][1] = total;
+        p_lds[tid >> 6][0] = zs;
+        p_lds[tid >> 6][1] = dot;
+    }
+    __syncthreads();
+    const unsigned w = tid & (FINISH_WAVES - 1);
+    rows = c_lds[w][0];
+    total = c_lds[w][1];
+    zs = p_lds[w][0];
+    dot = p_lds[w][1];
+#pragma unroll
+    for (int off = FINISH_WAVES / 2; off >= 1; off >>= 1) {
+        rows += __shfl_xor(rows, off);
+        total += __shfl_xor(total, off);
+        zs += __shfl_xor(zs, off);
+        dot += __shfl_xor(dot, off);
+    }
+    const long long all = (long long)total;
     const double inv_n = rows ? 1.0 / (double)rows : 0.0;
     const double per_count = all > 0 ? (double)E / (double)all : 0.0;
     if (tid == 0) {
@@ -489,11 +514,9 @@ __global__ __launch_bounds__(RT_THREADS) void router_backward_kernel(const Route
                 x[j] = x[j] == ninf ? 0.0f : sigmoid_weight(x[j], c, exp_c, &rest[j]);
             }
         } else {
+            softmax_weights(x, mx);
 #pragma unroll
-            for (int j = 0; j < N; ++j) {
-                rest[j] = 1.0f;
-                x[j] = softmax_weight(x[j], mx);
-            }
+            for (int j = 0; j < N; ++j) rest[j] = 1.0f;
         }
 #pragma unroll
         for (int j = 0; j < N; ++j) {
@@ -571,18 +594,27 @@ Form backward_form(unsigned E)
     return {4, E <= 512 ? 32 : 64};
 }
 
-// Chunks per image of a set: enough workgroups to fill the chip over all sets of the call, none with less than one trip.
-unsigned chunks_of(const Shape &sh, int Q)
+// Chunks per image of a set, and their rows: over all sets of the call as many workgroups as the chip holds at once (three
+// per CU at the registers of the forward kernels: with 1020 workgroups a second round of a few of them doubled the time; eight
+// of the backward kernels), each with the same number of trips.
+constexpr long long FORWARD_RESIDENT = 3 * 256, BACKWARD_RESIDENT = 8 * 256;
+struct Chunks {
+    unsigned count, rows;
+};
+Chunks chunks_of(const Shape &sh, int Q, bool backward = false)
 {
     const long long images = sh.merged ? 1 : sh.B;
     const long long rows = sh.merged ? (long long)sh.B * Q : Q;
-    const long long trip = RT_THREADS / forward_form((unsigned)sh.E).L;
-    const long long want = std::max(1ll, 1024 / std::max(1ll, (long long)sh.S * images));
-    return (unsigned)std::max(1ll, std::min(want, (rows + trip - 1) / trip));
+    const long long trip = RT_THREADS / (backward ? backward_form((unsigned)sh.E) : forward_form((unsigned)sh.E)).L;
+    const long long resident = backward ? BACKWARD_RESIDENT : FORWARD_RESIDENT;
+    const long long trips = std::max(1ll, (rows + trip - 1) / trip);
+    const long long want = std::max(1ll, resident / std::max(1ll, std::min<long long>(sh.S, DM_MAX_SETS_PER_LAUNCH) * images));
+    const long long each = (trips + want - 1) / want;
+    return Chunks{(unsigned)((trips + each - 1) / each), (unsigned)(each * trip)};
 }
 
 // The kernel arguments of sets first .. first + n - 1; returns the launch's workgroups.
-unsigned long long describe(const DmRouterSet *sets, int first, int n, const Shape &sh, int k, RouterSets *a)
+unsigned long long describe(const DmRouterSet *sets, int first, int n, const Shape &sh, int k, bool backward, RouterSets *a)
 {
     a->S = n;
     a->E = (unsigned)sh.E;
@@ -599,8 +631,9 @@ unsigned long long describe(const DmRouterSet *sets, int first, int n, const Sha
         s.image_stride = in.image_stride ? in.image_stride : (int64_t)in.Q * sh.E;
         s.images = sh.merged ? 1u : (unsigned)sh.B;
         s.Q = sh.merged ? (unsigned)sh.B * (unsigned)in.Q : (unsigned)in.Q;
-        s.chunks = chunks_of(sh, in.Q);
-        s.chunk_rows = (s.Q + s.chunks - 1) / s.chunks;
+        const Chunks c = chunks_of(sh, in.Q, backward);
+        s.chunks = c.count;
+        s.chunk_rows = c.rows;
         s.first_block = (unsigned)blocks;
         a->first_group[i] = (unsigned)i * (sh.per_image ? (unsigned)sh.B : 1u);
         blocks += (unsigned long long)s.images * s.chunks;
@@ -609,13 +642,13 @@ unsigned long long describe(const DmRouterSet *sets, int first, int n, const Sha
 }
 
 // (the sets of a call go through launches of up to DM_MAX_SETS_PER_LAUNCH, one after the other, over the same workspace)
-unsigned long long most_blocks(const DmRouterSet *sets, const Shape &sh)
+unsigned long long most_blocks(const DmRouterSet *sets, const Shape &sh, bool backward = false)
 {
     unsigned long long most = 0;
     for (int first = 0; first < sh.S; first += DM_MAX_SETS_PER_LAUNCH) {
         unsigned long long blocks = 0;
         for (int s = first; s < std::min(sh.S, first + DM_MAX_SETS_PER_LAUNCH); ++s)
-            blocks += (unsigned long long)(sh.merged ? 1 : sh.B) * chunks_of(sh, sets[s].Q);
+            blocks += (unsigned long long)(sh.merged ? 1 : sh.B) * chunks_of(sh, sets[s].Q, backward).count;
         most = std::max(most, blocks);
     }
     return most;
@@ -707,7 +740,7 @@ int forward(const DmRouterSet *sets, int S, int B, int E, int top_k, int dtype, 
     for (int first = 0; first < S; first += DM_MAX_SETS_PER_LAUNCH) {
         RouterSets a;
         const int n = std::min(S - first, DM_MAX_SETS_PER_LAUNCH);
-        const unsigned blocks = (unsigned)describe(sets, first, n, sh, top_k, &a);
+        const unsigned blocks = (unsigned)describe(sets, first, n, sh, top_k, false, &a);
         if (blocks) {
             hipLaunchKernelGGL(forward_for((unsigned)E, given == 1 ? 1u : (unsigned)top_k, dtype == DM_F32, balance == nullptr), dim3(blocks), dim3(RT_THREADS), 0,
                                st, a, dtype, scores == DM_SCORES_SIGMOID ? 1 : 0, slots, status);
@@ -783,12 +816,12 @@ extern "C" int dm_balance_backward(const DmRouterSet *sets, int S, int B, int E,
     if (!slope || !inv_rows) return DM_E_INVALID_ARG;
     for (int s = 0; s < S; ++s)
         if (sets[s].Q > 0 && (!sets[s].logits || !sets[s].grad)) return DM_E_INVALID_ARG;
-    if (most_blocks(sets, sh) >= (1ull << 31)) return DM_E_UNSUPPORTED;
+    if (most_blocks(sets, sh, true) >= (1ull << 31)) return DM_E_UNSUPPORTED;
     hipStream_t st = static_cast<hipStream_t>(stream);
     for (int first = 0; first < S; first += DM_MAX_SETS_PER_LAUNCH) {
         RouterSets a;
         const int n = std::min(S - first, DM_MAX_SETS_PER_LAUNCH);
-        const unsigned blocks = (unsigned)describe(sets, first, n, sh, 0, &a);
+        const unsigned blocks = (unsigned)describe(sets, first, n, sh, 0, true, &a);
         const size_t g0 = (size_t)first * (per_image ? (size_t)B : 1);
         hipLaunchKernelGGL(dtype == DM_F32 ? backward_for<true>((unsigned)E) : backward_for<false>((unsigned)E), dim3(blocks), dim3(RT_THREADS), 0, st, a, dtype, scores == DM_SCORES_SIGMOID ? 1 : 0,
                            slope + g0 * E, inv_rows + g0, grad_balance ? grad_balance + g0 : nullptr,

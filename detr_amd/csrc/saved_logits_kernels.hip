@@ -647,10 +647,21 @@ void launch_focal_from_saved(const uint8_t *codes, const int32_t *heads, const i
                        rows, fp, grad_loss, static_cast<T *>(grad));
 }
 
+// Workgroups for a number of trips: as many as the chip holds at once (seven per CU at these kernels' registers), each with
+// the same number of trips.  (256 x 900 x 91 logits are 5119 trips of the focal kernels: with 2048 workgroups half of them
+// make three and the others wait for them.)
+unsigned even_blocks(unsigned trips)
+{
+    constexpr unsigned RESIDENT = 7 * 256;
+    static_assert(RESIDENT <= (unsigned)CLS_MAX_BLOCKS, "a partial sum for each");
+    const unsigned each = std::max(1u, (trips + RESIDENT - 1) / RESIDENT);
+    return std::max(1u, (trips + each - 1) / each);
+}
+
 int focal_blocks(unsigned n)
 {
     const unsigned per_block = BLOCK * BLOCKS_AT_A_TIME;
-    return (int)std::max(1u, std::min((unsigned)CLS_MAX_BLOCKS, n / per_block + (n % per_block != 0)));
+    return (int)even_blocks(n / per_block + (n % per_block != 0));
 }
 
 constexpr unsigned WIDEST = 2048;      // logits of a row that a wavefront keeps in registers
@@ -698,7 +709,7 @@ void with_ce_form(unsigned C, F &&f)
 unsigned ce_blocks(unsigned rows, unsigned C)
 {
     const unsigned rows_per_block = C <= WIDEST ? (unsigned)(CLS_THREADS / ce_form(C).L) : 1u;
-    return std::max(1u, std::min((unsigned)CLS_MAX_BLOCKS, (rows + rows_per_block - 1) / rows_per_block));
+    return even_blocks(rows / rows_per_block + (rows % rows_per_block != 0));
 }
 template <typename T>
 void launch_ce_saved(const void *logits, int dtype, const int64_t *cls, const float *weight, unsigned rows, unsigned C, int64_t ignore_index,
