@@ -194,6 +194,17 @@ __device__ __forceinline__ unsigned partner(unsigned v) { return (unsigned)partn
 template <int STEP>
 __device__ __forceinline__ float partner(float v) { return __int_as_float(partner<STEP>(__float_as_int(v))); }
 
+template <int STEP>
+__device__ __forceinline__ unsigned long long partner(unsigned long long v)
+{
+    return (unsigned long long)partner<STEP>((unsigned)(v >> 32)) << 32 | partner<STEP>((unsigned)v);
+}
+template <int STEP>
+__device__ __forceinline__ double partner(double v)
+{
+    return __builtin_bit_cast(double, partner<STEP>(__builtin_bit_cast(unsigned long long, v)));
+}
+
 struct Max { template <typename V> __device__ __forceinline__ V operator()(V a, V b) const { return a > b ? a : b; } };
 struct Min { template <typename V> __device__ __forceinline__ V operator()(V a, V b) const { return a < b ? a : b; } };
 struct Add { template <typename V> __device__ __forceinline__ V operator()(V a, V b) const { return a + b; } };

@@ -337,8 +337,7 @@ __global__ __launch_bounds__(RT_THREADS) void router_forward_kernel(const Router
 //   LOSS alone      a workgroup per group, from counts and means
 // Two launches are taken for few groups of many experts, where one workgroup would read a megabyte of slots by itself.  (One
 // launch in which the last of a group's workgroups makes the loss is slower: the fences it needs write the caches back.)
-constexpr int FINISH_THREADS = 1024, FINISH_WAVES = FINISH_THREADS / 64;
-static_assert(RT_MAX_EXPERTS <= FINISH_THREADS, "a thread per expert");
+constexpr int FINISH_THREADS = 1024, FINISH_WAVES = FINISH_THREADS / 64, LOSS_THREADS = 256;
 
 template <bool SUMS, bool LOSS>
 __global__ __launch_bounds__(FINISH_THREADS) void router_finish_kernel(const RouterSets a, const unsigned *__restrict__ slots,
@@ -358,15 +357,6 @@ __global__ __launch_bounds__(FINISH_THREADS) void router_finish_kernel(const Rou
     const unsigned image = group - a.first_group[set];                   // (0 unless per_image)
     const unsigned slots_of_group = a.per_image ? s.chunks : s.images * s.chunks;
     const unsigned *first = slots + (size_t)(s.first_block + image * s.chunks) * words;
-    // the rows that count and the sum of lse^2 are asked for first
-    double zs = 0.0;
-    unsigned long long rows = 0;
-    if (LOSS)
-        for (unsigned i = tid; i < slots_of_group; i += FINISH_THREADS) {
-            const unsigned *slot = first + (size_t)i * words;
-            zs += *reinterpret_cast<const double *>(slot + 2 * E);
-            rows += slot[2 * E + 2];
-        }
     if (SUMS) {
         const unsigned col = tid & (cols - 1), slice = tid / cols, slices = FINISH_THREADS / cols;
         const bool with_p = means != nullptr || LOSS;
@@ -374,14 +364,24 @@ __global__ __launch_bounds__(FINISH_THREADS) void router_finish_kernel(const Rou
             const unsigned e = e0 + col;
             double p = 0.0;
             unsigned long long c = 0;
-            if (e < E) {
-#pragma unroll 8
-                for (unsigned i = slice; i < slots_of_group; i += slices) {
-                    const unsigned *slot = first + (size_t)i * words;
-                    if (with_p) p += (double)__uint_as_float(slot[e]);
-                    c += slot[E + e];
+            // (eight slots are asked for before the first is added)
+            for (unsigned i = slice; i < slots_of_group; i += 8 * slices) {
+                float part[8];
+                unsigned times[8];
+#pragma unroll
+                for (unsigned u = 0; u < 8; ++u) {
+                    const bool there = e < E && i + u * slices < slots_of_group;
+                    const unsigned *slot = first + (size_t)(there ? i + u * slices : 0) * words + (there ? e : 0);
+                    part[u] = there && with_p ? __uint_as_float(slot[0]) : 0.0f;
+                    times[u] = there ? slot[E] : 0u;
+                }
+#pragma unroll
+                for (unsigned u = 0; u < 8; ++u) {
+                    p += (double)part[u];
+                    c += times[u];
                 }
             }
+            // (cols: 1 to 64; the lanes of an expert are cols apart)
             for (unsigned off = cols; off < 64; off <<= 1) {
                 p += __shfl_xor(p, off);
                 c += __shfl_xor(c, off);
@@ -408,23 +408,34 @@ __global__ __launch_bounds__(FINISH_THREADS) void router_finish_kernel(const Rou
             __syncthreads();
         }
     }
-    if (!LOSS) return;
-    long long mine = 0;
-    double dot = 0.0;
-    if (tid < E) {
-        const int64_t *shares = given_counts ? given_counts : SUMS ? nullptr : counts;
-        mine = shares ? shares[(size_t)group * E + tid] : C[tid];
-        dot = (double)mine * (SUMS ? P[tid] : means[(size_t)group * E + tid]);
-    }
-    // the four sums over the workgroup, in every thread, in one exchange
-    unsigned long long total = (unsigned long long)mine;
+    if (!LOSS || tid >= LOSS_THREADS) return;
+    // the rows that count and the sum of lse^2; the counts and sum_e c_e P_e
+    constexpr int EACH = RT_MAX_EXPERTS / LOSS_THREADS;
+    const int64_t *shares = given_counts ? given_counts : SUMS ? nullptr : counts;
+    long long mine[EACH];
+    double zs = 0.0, dot = 0.0;
+    unsigned long long rows = 0, total = 0;
 #pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) {
-        rows += __shfl_xor(rows, off);
-        total += __shfl_xor(total, off);
-        zs += __shfl_xor(zs, off);
-        dot += __shfl_xor(dot, off);
+    for (int j = 0; j < EACH; ++j) {
+        const unsigned e = tid + j * LOSS_THREADS;
+        mine[j] = 0;
+        if (e < E) {
+            mine[j] = shares ? shares[(size_t)group * E + e] : C[e];
+            dot += (double)mine[j] * (SUMS ? P[e] : means[(size_t)group * E + e]);
+            total += (unsigned long long)mine[j];
+        }
     }
+#pragma unroll 4
+    for (unsigned i = tid; i < slots_of_group; i += LOSS_THREADS) {
+        const unsigned *slot = first + (size_t)i * words;
+        zs += *reinterpret_cast<const double *>(slot + 2 * E);
+        rows += slot[2 * E + 2];
+    }
+    // over the wave, then over the waves, in every thread
+    rows = dm::over_group<64>(rows, dm::Add());
+    total = dm::over_group<64>(total, dm::Add());
+    zs = dm::over_group<64>(zs, dm::Add());
+    dot = dm::over_group<64>(dot, dm::Add());
     if ((tid & 63) == 0) {
         c_lds[tid >> 6][0] = rows;
         c_lds[tid >> 6][1] = total;
@@ -432,17 +443,16 @@ __global__ __launch_bounds__(FINISH_THREADS) void router_finish_kernel(const Rou
         p_lds[tid >> 6][1] = dot;
     }
     __syncthreads();
-    const unsigned w = tid & (FINISH_WAVES - 1);
-    rows = c_lds[w][0];
-    total = c_lds[w][1];
-    zs = p_lds[w][0];
-    dot = p_lds[w][1];
+    rows = c_lds[0][0];
+    total = c_lds[0][1];
+    zs = p_lds[0][0];
+    dot = p_lds[0][1];
 #pragma unroll
-    for (int off = FINISH_WAVES / 2; off >= 1; off >>= 1) {
-        rows += __shfl_xor(rows, off);
-        total += __shfl_xor(total, off);
-        zs += __shfl_xor(zs, off);
-        dot += __shfl_xor(dot, off);
+    for (int w = 1; w < LOSS_THREADS / 64; ++w) {
+        rows += c_lds[w][0];
+        total += c_lds[w][1];
+        zs += p_lds[w][0];
+        dot += p_lds[w][1];
     }
     const long long all = (long long)total;
     const double inv_n = rows ? 1.0 / (double)rows : 0.0;
@@ -452,7 +462,11 @@ __global__ __launch_bounds__(FINISH_THREADS) void router_finish_kernel(const Rou
         if (z) z[group] = (float)(zs * inv_n);
         inv_rows[group] = (float)inv_n;
     }
-    if (tid < E) slope[(size_t)group * E + tid] = all > 0 ? (float)((double)mine * per_count - 1.0) : 0.0f;
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+        const unsigned e = tid + j * LOSS_THREADS;
+        if (e < E) slope[(size_t)group * E + e] = all > 0 ? (float)((double)mine[j] * per_count - 1.0) : 0.0f;
+    }
 }
 
 template <int NQ, int L, bool WIDE>
@@ -751,23 +765,23 @@ int forward(const DmRouterSet *sets, int S, int B, int E, int top_k, int dtype, 
         const unsigned gn = (unsigned)n * (per_image ? (unsigned)B : 1u);
         unsigned cols = 1;
         while (cols < 64 && cols < (unsigned)E) cols <<= 1;
-        auto finish = [&](auto kernel, unsigned parts, unsigned width) {
-            hipLaunchKernelGGL(kernel, dim3(gn, parts), dim3(FINISH_THREADS), 0, st, a, slots, width,
+        auto finish = [&](auto kernel, unsigned parts, unsigned width, int threads) {
+            hipLaunchKernelGGL(kernel, dim3(gn, parts), dim3(threads), 0, st, a, slots, width,
                                given_counts ? given_counts + g0 * E : nullptr, means, balance ? balance + g0 : nullptr,
                                z ? z + g0 : nullptr, counts + g0 * E, slope ? slope + g0 * E : nullptr,
                                inv_rows ? inv_rows + g0 : nullptr);
         };
-        // (by itself a workgroup adds some 64 slots of 64 experts a microsecond)
-        const bool few = gn <= 16 && E > 64 && (unsigned long long)blocks * (unsigned)E > 64ull * 1024 * gn;
+        // (one workgroup adds 720 slots of 64 experts in 20 us, four of 16 experts each in 4)
+        const bool few = gn <= 64 && (unsigned long long)blocks * (unsigned)E > 4096ull * gn && E > 16;
         const unsigned width = few ? 16u : cols, parts = few ? (unsigned)(E + 15) / 16 : 1u;
         if (!balance) {
             means = nullptr;
-            finish(router_finish_kernel<true, false>, parts, width);
+            finish(router_finish_kernel<true, false>, parts, width, FINISH_THREADS);
         } else if (few) {
-            finish(router_finish_kernel<true, false>, parts, width);
-            finish(router_finish_kernel<false, true>, 1u, cols);
+            finish(router_finish_kernel<true, false>, parts, width, FINISH_THREADS);
+            finish(router_finish_kernel<false, true>, 1u, cols, LOSS_THREADS);
         } else {
-            finish(router_finish_kernel<true, true>, 1u, cols);
+            finish(router_finish_kernel<true, true>, 1u, cols, FINISH_THREADS);
         }
         rc = dm::check_hip(hipGetLastError(), "router_finish_kernel launch");
         if (rc != DM_OK) return rc;
