@@ -146,6 +146,27 @@ __device__ __forceinline__ void place_row(float (&x)[4 * NQ], unsigned sub, unsi
     }
 }
 
+// The same for 16-bit elements before they are made float32, a quad at once; `pair`: two elements to fill with.
+template <int NQ, int L>
+__device__ __forceinline__ void place_raw(RawRow<NQ, false> &raw, unsigned sub, unsigned n, unsigned pair)
+{
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+        if (4 * (q + 1) * L <= n) continue;                    // (the same for all lanes)
+        const unsigned c = 4 * (q * L + sub);
+        // moved: places that the quad is to move down; n < 4: it was read in place, what is behind the end is made `fill`
+        const unsigned moved = n < 4 ? 0 : c - min(c, n - 4);
+        const unsigned long long v = (unsigned long long)raw.q[q][1] << 32 | raw.q[q][0];
+        const unsigned long long all = (unsigned long long)pair << 32 | pair;
+        const unsigned left = n < 4 ? min(n - min(c, n), 4u) : 4 - min(moved, 4u);      // elements of the row in the quad
+        const unsigned long long low = moved >= 4 ? 0ull : v >> (16 * (moved & 3));
+        const unsigned long long keep = left >= 4 ? ~0ull : (1ull << (16 * left)) - 1;
+        const unsigned long long r = (low & keep) | (all & ~keep);
+        raw.q[q][0] = (unsigned)r;
+        raw.q[q][1] = (unsigned)(r >> 32);
+    }
+}
+
 template <int NQ, int L, bool WIDE>
 __device__ __forceinline__ void row_values(const RawRow<NQ, WIDE> &raw, int dtype, unsigned sub, unsigned n, float fill, float (&x)[4 * NQ])
 {
@@ -237,6 +258,28 @@ __device__ __forceinline__ float largest(float v)
     return v;
 }
 #undef DM_MAX_DPP
+#define DM_MAX_DPP(v, control) asm("s_nop 1\n\tv_max_i32_dpp %0, %1, %1 " control " row_mask:0xf bank_mask:0xf" : "=v"(v) : "v"(v))
+template <int L>
+__device__ __forceinline__ int largest(int v)
+{
+    if (L >= 2) DM_MAX_DPP(v, "quad_perm:[1,0,3,2]");
+    if (L >= 4) DM_MAX_DPP(v, "quad_perm:[2,3,0,1]");
+    if (L >= 8) DM_MAX_DPP(v, "row_half_mirror");
+    if (L >= 16) DM_MAX_DPP(v, "row_mirror");
+    if (L >= 32) v = max(v, partner<16>(v));
+    if (L >= 64) v = max(v, partner<32>(v));
+    return v;
+}
+#undef DM_MAX_DPP
+
+// The middle one of three.
+__device__ __forceinline__ float median(float a, float b, float c) { return __builtin_amdgcn_fmed3f(a, b, c); }
+__device__ __forceinline__ int median(int a, int b, int c)
+{
+    int r;
+    asm("v_med3_i32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
 
 // The sum over the lanes of a row of 16 whose number is the same modulo L (L <= 16): every lane gets that of its own.
 template <int L, typename V>

@@ -11,6 +11,7 @@
 // lane that owns the expert, and leave once per workgroup, into a slot of the workspace.  A second kernel adds the slots in
 // index order in 64 bits: no float atomics, the same bits every run.
 #include <algorithm>
+#include <climits>
 
 #include "lanes.h"
 
@@ -84,23 +85,91 @@ __device__ __forceinline__ float sigmoid_weight(float x, float c, float exp_c, f
     return (x >= 0.0f ? 1.0f : t) * r;
 }
 
-// What the choice compares.  float32: the logits, with what is never chosen at -infinity.  16-bit logits are equal to one
-// another often, and equal ones are to go to the lowest index: as float32 their low 13 or 16 bits are zero, so the expert's
-// number goes into the low ten (1023 - e for positive logits, e for negative ones, where a longer mantissa means smaller).  No
-// two are equal then, and the order is that of (logit, lowest index).  +infinity becomes a number that is larger than any.
-constexpr unsigned ABOVE_ALL = 0x7F7F8000u;
-__device__ __forceinline__ float order_f32(float x) { return dm::max3(x, -__builtin_huge_valf(), -__builtin_huge_valf()); }
-__device__ __forceinline__ float order_16(float x, unsigned e)
+// What the choice compares: an order in which no two of a row are equal where that can be had, and its least.
+//   float32   the logits, with what is never chosen (-infinity, NaN) at -infinity.  Equal ones are seen to afterwards.
+//   16 bits   equal logits are frequent, and are to go to the lowest index: the logit as a 16-bit number of the same order
+//             (sign and magnitude to two's complement, which also makes the two zeros one), two at a time, in the upper half
+//             of an int, and 1023 - expert in the lower; -infinity lies below `least`, a NaN is put there
+template <bool WIDE>
+struct Order;
+template <>
+struct Order<true> {
+    typedef float Type;
+    static __device__ __forceinline__ Type never() { return -__builtin_huge_valf(); }
+    static __device__ __forceinline__ Type above_all() { return __builtin_huge_valf(); }
+    static __device__ __forceinline__ Type least(int) { return -__FLT_MAX__; }
+    static __device__ __forceinline__ float logit(Type y, int) { return y; }
+};
+template <>
+struct Order<false> {
+    typedef int Type;
+    typedef short Pair __attribute__((ext_vector_type(2)));
+    static __device__ __forceinline__ Type never() { return INT_MIN; }
+    static __device__ __forceinline__ Type above_all() { return INT_MAX; }
+    static __device__ __forceinline__ unsigned infinity(int dtype) { return dtype == DM_BF16 ? 0x7F80u : 0x7C00u; }
+    static __device__ __forceinline__ Type least(int dtype) { return (int)((1u - infinity(dtype)) << 16); }
+    static __device__ __forceinline__ float logit(Type y, int dtype)
+    {
+        const int v = y >> 16, sign = v >> 31;
+        const unsigned u = (unsigned)((v ^ sign) - sign) | ((unsigned)sign & 0x8000u);
+        return dtype == DM_BF16 ? __uint_as_float(u << 16) : (float)__builtin_bit_cast(dm::half_t, (uint16_t)u);
+    }
+    // two logits; low: 1023 - expert of each; over: not 0 for a NaN
+    static __device__ __forceinline__ void of(unsigned raw, unsigned low0, unsigned low1, unsigned inf2, Type *y0, Type *y1, unsigned *over)
+    {
+        const unsigned magnitude = raw & 0x7FFF7FFFu;
+        const Pair sign = __builtin_bit_cast(Pair, raw) >> 15;
+        const unsigned key = __builtin_bit_cast(unsigned, __builtin_bit_cast(Pair, magnitude ^ __builtin_bit_cast(unsigned, sign)) - sign);
+        unsigned beyond;
+        asm("v_pk_sub_u16 %0, %1, %2 clamp" : "=v"(beyond) : "v"(magnitude), "v"(inf2));
+        *over |= beyond;
+        *y0 = (int)(key << 16 | low0);
+        *y1 = (int)((key & 0xFFFF0000u) | low1);
+    }
+};
+
+// A lane's logits in their order.
+template <int NQ, int L>
+__device__ __forceinline__ void in_order(const dm::RawRow<NQ, true> &raw, int dtype, unsigned sub, unsigned E, bool counts,
+                                         float (&y)[4 * NQ], bool *nan)
 {
-    const float finite = __builtin_amdgcn_fmed3f(x + 0.0f, -__builtin_huge_valf(), __uint_as_float(ABOVE_ALL));      // (-0 is +0)
-    const unsigned u = __float_as_uint(finite);
-    const unsigned low = (1023u - e) ^ ((unsigned)((int)u >> 31) & 1023u);
-    return x > -__builtin_huge_valf() ? __uint_as_float(u | low) : -__builtin_huge_valf();
+    const float ninf = -__builtin_huge_valf();
+    dm::row_values<NQ, L, true>(raw, dtype, sub, E, ninf, y);
+    if (!counts) {
+#pragma unroll
+        for (int j = 0; j < 4 * NQ; ++j) y[j] = ninf;
+    }
+    *nan = false;
+#pragma unroll
+    for (int j = 0; j < 4 * NQ; ++j) {
+        *nan |= y[j] != y[j];
+        y[j] = dm::max3(y[j], ninf, ninf);
+    }
 }
-__device__ __forceinline__ float logit_of_order_16(float y)
+template <int NQ, int L>
+__device__ __forceinline__ void in_order(dm::RawRow<NQ, false> &raw, int dtype, unsigned sub, unsigned E, bool counts,
+                                         int (&y)[4 * NQ], bool *nan)
 {
-    const float x = __uint_as_float(__float_as_uint(y) & ~1023u);
-    return x == __uint_as_float(ABOVE_ALL) ? __builtin_huge_valf() : (y == -__builtin_huge_valf() ? y : x);
+    const unsigned inf = Order<false>::infinity(dtype), inf2 = inf << 16 | inf, pair = inf2 | 0x80008000u;
+    dm::place_raw<NQ, L>(raw, sub, E, pair);
+    if (!counts) {
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) raw.q[q][0] = raw.q[q][1] = pair;
+    }
+    unsigned over = 0;
+#pragma unroll
+    for (int q = 0; q < NQ; ++q)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const unsigned low = 1023u - (4 * (q * L + sub) + 2 * h);
+            Order<false>::of(raw.q[q][h], low, low - 1, inf2, &y[4 * q + 2 * h], &y[4 * q + 2 * h + 1], &over);
+        }
+    *nan = false;                                              // (the scores are made of the logits as they came)
+    if (__any(over)) {
+#pragma unroll
+        for (int j = 0; j < 4 * NQ; ++j)
+            if (((raw.q[j >> 2][(j >> 1) & 1] >> (16 * (j & 1))) & 0x7FFFu) > inf) y[j] = Order<false>::never();
+    }
 }
 
 // K: the longest list of largest logits that a lane keeps (k <= K), or 0: k of any size, in rounds over all logits.
@@ -154,39 +223,98 @@ __global__ __launch_bounds__(RT_THREADS) void router_forward_kernel(const Router
         const unsigned r = r0 + local;
         const bool there = r < at.rows;
         const size_t row = (size_t)at.row0 + (there ? r : 0);
-        const dm::RawRow<NQ, WIDE> raw = next;
+        dm::RawRow<NQ, WIDE> raw = next;
         const bool counts = there && next_counts != 0;
         if (r0 + ROWS < at.rows) fetch(r + ROWS);
-        float x[N];
-        dm::row_values<NQ, L, WIDE>(raw, dtype, sub, E, ninf, x);
-        if (!counts) {
+        typedef Order<WIDE> O;
+        typename O::Type y[N];
+        bool nan;
+        in_order<NQ, L>(raw, dtype, sub, E, counts, y, &nan);
+        constexpr int PLACES = K ? K : 1;
+        typename O::Type list[PLACES];
 #pragma unroll
-            for (int j = 0; j < N; ++j) x[j] = ninf;
-        }
-        // the order, its largest, and whether the row counts
-        float y[N];
-        if (WIDE) {
-#pragma unroll
-            for (int j = 0; j < N; ++j) y[j] = order_f32(x[j]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < N; ++j) y[j] = order_16(x[j], 4 * ((j >> 2) * L + sub) + (j & 3));
-        }
-        float list[K ? K : 1];
-#pragma unroll
-        for (int i = 0; i < (K ? K : 1); ++i) list[i] = ninf;
+        for (int i = 0; i < PLACES; ++i) list[i] = O::never();
 #pragma unroll
         for (int j = 0; j < N; ++j) {
 #pragma unroll
-            for (int i = (K ? K : 1) - 1; i >= 1; --i) list[i] = __builtin_amdgcn_fmed3f(list[i - 1], list[i], y[j]);
-            list[0] = __builtin_amdgcn_fmed3f(list[0], y[j], __builtin_huge_valf());
+            for (int i = PLACES - 1; i >= 1; --i) list[i] = dm::median(list[i - 1], list[i], y[j]);
+            list[0] = dm::median(list[0], y[j], O::above_all());
         }
-        const float top = dm::largest<L>(list[0]);
-        bool live;
-        if (!COUNT_ONLY) {
-            float mx = WIDE ? top : logit_of_order_16(top);
-            mx = top == ninf ? 0.0f : mx;
-            float sum = 0.0f;
+        const typename O::Type top = dm::largest<L>(list[0]);
+        if (COUNT_ONLY || !set.experts) {
+            bool again = K == 0;
+            if (K) {
+                typename O::Type last = O::never();
+                if (L == 1) {
+#pragma unroll
+                    for (int i = 0; i < PLACES; ++i) last = i + 1 == (int)k ? list[i] : last;
+                } else {
+                    last = top;
+#pragma unroll
+                    for (int i = 1; i < PLACES; ++i) {
+                        if (i < (int)k) {
+                            // (the median of a place, the next and the least is the next, of the largest the place itself; what
+                            // could come up after the k-th is not moved any more)
+                            const typename O::Type gone = list[0] == last ? O::never() : O::above_all();
+#pragma unroll
+                            for (int j = 0; j + i < PLACES; ++j) list[j] = dm::median(list[j], list[j + 1], gone);
+                            last = dm::largest<L>(list[0]);
+                        }
+                    }
+                }
+                last = max(last, O::least(dtype));             // (fewer than k: all that can be)
+                unsigned chosen = 0;
+#pragma unroll
+                for (int j = 0; j < N; ++j) {
+                    const unsigned one = y[j] >= last ? 1u : 0u;
+                    cnt[j] += one;
+                    if (WIDE) chosen += one;
+                }
+                if (WIDE) {
+                    chosen = dm::over_group<L>(chosen, dm::Add());
+                    again = __any(chosen > k);
+                    if (again) {
+#pragma unroll
+                        for (int j = 0; j < N; ++j) cnt[j] -= y[j] >= last ? 1u : 0u;
+                    }
+                }
+            }
+            if (again) {
+                // k times the largest that is left, of the lowest expert that has it
+                typename O::Type left[N];
+#pragma unroll
+                for (int j = 0; j < N; ++j) left[j] = y[j];
+                for (unsigned i = 0; i < k; ++i) {
+                    typename O::Type best = O::never();
+#pragma unroll
+                    for (int j = 0; j < N; ++j) best = dm::median(best, left[j], O::above_all());
+                    best = dm::largest<L>(best);
+                    unsigned first = 0xFFFFFFFFu;
+#pragma unroll
+                    for (int j = N - 1; j >= 0; --j)
+                        if (left[j] == best) first = (unsigned)(4 * ((j >> 2) * L + sub) + (j & 3));
+                    first = dm::over_group<L>(first, dm::Min());
+                    if (best < O::least(dtype)) first = 0xFFFFFFFFu;
+#pragma unroll
+                    for (int j = 0; j < N; ++j) {
+                        const bool hit = first == (unsigned)(4 * ((j >> 2) * L + sub) + (j & 3));
+                        cnt[j] += hit ? 1u : 0u;
+                        left[j] = hit ? O::never() : left[j];
+                    }
+                }
+            }
+        }
+        if constexpr (!COUNT_ONLY) {
+            // the scores, of the logits as they came
+            const float mx = top < O::least(dtype) ? 0.0f : O::logit(top, dtype);
+            float x[N];
+            if constexpr (WIDE) {
+#pragma unroll
+                for (int j = 0; j < N; ++j) x[j] = y[j];
+            } else {
+                dm::raw_values<NQ, WIDE>(raw, dtype, x);
+            }
+            float sum = nan ? __builtin_nanf("") : 0.0f;
             if (sigmoid) {
                 const float c = fminf(mx, 0.0f), exp_c = __builtin_amdgcn_exp2f(c * LOG2E);
 #pragma unroll
@@ -201,7 +329,7 @@ __global__ __launch_bounds__(RT_THREADS) void router_forward_kernel(const Router
                 for (int j = 0; j < N; ++j) sum += x[j];
             }
             sum = dm::over_group<L>(sum, dm::Add());
-            live = sum != 0.0f;                                // (a NaN makes it NaN)
+            const bool live = sum != 0.0f;                     // (a NaN makes it NaN)
             const float inv = live ? __builtin_amdgcn_rcpf(sum) : 0.0f;
 #pragma unroll
             for (int j = 0; j < N; ++j) psum[j] = __builtin_fmaf(x[j], inv, psum[j]);
@@ -210,74 +338,12 @@ __global__ __launch_bounds__(RT_THREADS) void router_forward_kernel(const Router
                 z += lse * lse;
                 ++n;
             }
-        } else {
-            live = true;                                       // (a row with nothing but -infinity and NaN chooses nothing)
-        }
-        if (!COUNT_ONLY && set.experts) {
-            if (live)
+            if (set.experts && live)
                 for (unsigned j = sub; j < k; j += L) {
                     const int64_t e = set.experts[(image_row + row) * k + j];
                     if (e >= 0 && e < (int64_t)E) atomicAdd(&hist[(unsigned)e], 1u);
                     else bad |= e != -1;
                 }
-            continue;
-        }
-        bool again = K == 0;
-        if (K) {
-            float last = ninf;
-            if (L == 1) {
-#pragma unroll
-                for (int i = 0; i < K; ++i) last = i + 1 == (int)k ? list[i] : last;
-            } else {
-                last = top;
-#pragma unroll
-                for (int i = 1; i < K; ++i) {
-                    if (i < (int)k) {
-                        // (the median of a place, the next and -infinity is the next, of +infinity the place itself)
-                        const float gone = list[0] == last ? ninf : __builtin_huge_valf();
-#pragma unroll
-                        for (int j = 0; j + 1 < K; ++j) list[j] = __builtin_amdgcn_fmed3f(list[j], list[j + 1], gone);
-                        list[K - 1] = __builtin_amdgcn_fmed3f(list[K - 1], ninf, gone);
-                        last = dm::largest<L>(list[0]);
-                    }
-                }
-            }
-            last = __builtin_amdgcn_fmed3f(last, -__FLT_MAX__, __builtin_huge_valf());       // (fewer than k: all that can be)
-            unsigned chosen = 0;
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                const unsigned one = y[j] >= last ? 1u : 0u;
-                cnt[j] += one;
-                if (WIDE) chosen += one;
-            }
-            if (WIDE) {
-                chosen = dm::over_group<L>(chosen, dm::Add());
-                again = __any(chosen > k);
-                if (again) {
-#pragma unroll
-                    for (int j = 0; j < N; ++j) cnt[j] -= y[j] >= last ? 1u : 0u;
-                }
-            }
-        }
-        if (again) {
-            // k times the largest that is left, of the lowest expert that has it
-            for (unsigned i = 0; i < k; ++i) {
-                float best = y[0];
-#pragma unroll
-                for (int j = 1; j < N; ++j) best = __builtin_amdgcn_fmed3f(best, y[j], __builtin_huge_valf());
-                best = dm::largest<L>(best);
-                unsigned first = 0xFFFFFFFFu;
-#pragma unroll
-                for (int j = N - 1; j >= 0; --j)
-                    if (y[j] == best) first = (unsigned)(4 * ((j >> 2) * L + sub) + (j & 3));
-                first = dm::over_group<L>(first, dm::Min());
-#pragma unroll
-                for (int j = 0; j < N; ++j) {
-                    const bool hit = best != ninf && first == (unsigned)(4 * ((j >> 2) * L + sub) + (j & 3));
-                    cnt[j] += hit ? 1u : 0u;
-                    y[j] = hit ? ninf : y[j];
-                }
-            }
         }
     }
     if (bad) dm::raise_status(status, DM_ST_LABEL_RANGE);
@@ -504,11 +570,16 @@ __global__ __launch_bounds__(RT_THREADS) void router_backward_kernel(const Route
         const unsigned r = r0 + local;
         const bool there = r < at.rows;
         const size_t row = (size_t)at.row0 + (there ? r : 0);
-        const dm::RawRow<NQ, WIDE> raw = next;
+        dm::RawRow<NQ, WIDE> raw = next;
         const bool counts = next_counts != 0;
         if (r0 + ROWS < at.rows) fetch(r + ROWS);
         float x[N];
-        dm::row_values<NQ, L, WIDE>(raw, dtype, sub, E, ninf, x);
+        if constexpr (WIDE) {
+            dm::row_values<NQ, L, WIDE>(raw, dtype, sub, E, ninf, x);
+        } else {
+            dm::place_raw<NQ, L>(raw, sub, E, dtype == DM_BF16 ? 0xFF80FF80u : 0xFC00FC00u);
+            dm::raw_values<NQ, WIDE>(raw, dtype, x);
+        }
         if (!counts) {
 #pragma unroll
             for (int j = 0; j < N; ++j) x[j] = ninf;
@@ -608,19 +679,19 @@ Form backward_form(unsigned E)
     return {4, E <= 512 ? 32 : 64};
 }
 
-// Chunks per image of a set, and their rows: over all sets of the call as many workgroups as the chip holds at once (three
-// per CU at the registers of the forward kernels: with 1020 workgroups a second round of a few of them doubled the time; eight
-// of the backward kernels), each with the same number of trips.
-constexpr long long FORWARD_RESIDENT = 3 * 256, BACKWARD_RESIDENT = 8 * 256;
+// Chunks per image of a set, and their rows: over all sets of the call as many workgroups as the chip holds at once (with
+// 1020 workgroups of the float32 kernel a second round of a few of them doubled the time), each with the same number of trips.
+// Per CU, at the kernels' registers: three of the forward kernel, eight of the backward kernel.  (Five of the forward kernel fit
+// for 16 bits: no faster, and two thirds more slots to add.)
+constexpr int FORWARD = 3 * 256, BACKWARD = 8 * 256;
 struct Chunks {
     unsigned count, rows;
 };
-Chunks chunks_of(const Shape &sh, int Q, bool backward = false)
+Chunks chunks_of(const Shape &sh, int Q, int resident)
 {
     const long long images = sh.merged ? 1 : sh.B;
     const long long rows = sh.merged ? (long long)sh.B * Q : Q;
-    const long long trip = RT_THREADS / (backward ? backward_form((unsigned)sh.E) : forward_form((unsigned)sh.E)).L;
-    const long long resident = backward ? BACKWARD_RESIDENT : FORWARD_RESIDENT;
+    const long long trip = RT_THREADS / (resident == BACKWARD ? backward_form((unsigned)sh.E) : forward_form((unsigned)sh.E)).L;
     const long long trips = std::max(1ll, (rows + trip - 1) / trip);
     const long long want = std::max(1ll, resident / std::max(1ll, std::min<long long>(sh.S, DM_MAX_SETS_PER_LAUNCH) * images));
     const long long each = (trips + want - 1) / want;
@@ -628,7 +699,7 @@ Chunks chunks_of(const Shape &sh, int Q, bool backward = false)
 }
 
 // The kernel arguments of sets first .. first + n - 1; returns the launch's workgroups.
-unsigned long long describe(const DmRouterSet *sets, int first, int n, const Shape &sh, int k, bool backward, RouterSets *a)
+unsigned long long describe(const DmRouterSet *sets, int first, int n, const Shape &sh, int k, int resident, RouterSets *a)
 {
     a->S = n;
     a->E = (unsigned)sh.E;
@@ -645,7 +716,7 @@ unsigned long long describe(const DmRouterSet *sets, int first, int n, const Sha
         s.image_stride = in.image_stride ? in.image_stride : (int64_t)in.Q * sh.E;
         s.images = sh.merged ? 1u : (unsigned)sh.B;
         s.Q = sh.merged ? (unsigned)sh.B * (unsigned)in.Q : (unsigned)in.Q;
-        const Chunks c = chunks_of(sh, in.Q, backward);
+        const Chunks c = chunks_of(sh, in.Q, resident);
         s.chunks = c.count;
         s.chunk_rows = c.rows;
         s.first_block = (unsigned)blocks;
@@ -656,13 +727,13 @@ unsigned long long describe(const DmRouterSet *sets, int first, int n, const Sha
 }
 
 // (the sets of a call go through launches of up to DM_MAX_SETS_PER_LAUNCH, one after the other, over the same workspace)
-unsigned long long most_blocks(const DmRouterSet *sets, const Shape &sh, bool backward = false)
+unsigned long long most_blocks(const DmRouterSet *sets, const Shape &sh, int resident)
 {
     unsigned long long most = 0;
     for (int first = 0; first < sh.S; first += DM_MAX_SETS_PER_LAUNCH) {
         unsigned long long blocks = 0;
         for (int s = first; s < std::min(sh.S, first + DM_MAX_SETS_PER_LAUNCH); ++s)
-            blocks += (unsigned long long)(sh.merged ? 1 : sh.B) * chunks_of(sh, sets[s].Q, backward).count;
+            blocks += (unsigned long long)(sh.merged ? 1 : sh.B) * chunks_of(sh, sets[s].Q, resident).count;
         most = std::max(most, blocks);
     }
     return most;
@@ -683,6 +754,7 @@ ForwardKernel forward_with(unsigned k, bool wide, bool count_only)
     if (k <= 2) return forward_of<NQ, L, 2>(wide, count_only);
     if (k <= 4) return forward_of<NQ, L, 4>(wide, count_only);
     if (k <= 8) return forward_of<NQ, L, 8>(wide, count_only);
+    if (k <= 16) return forward_of<NQ, L, 16>(wide, count_only);
     return forward_of<NQ, L, 0>(wide, count_only);
 }
 ForwardKernel forward_for(unsigned E, unsigned k, bool wide, bool count_only)
@@ -722,7 +794,7 @@ struct Workspace {
 };
 Workspace workspace_of(const DmRouterSet *sets, const Shape &sh)
 {
-    return Workspace{most_blocks(sets, sh), (unsigned long long)std::min(sh.S, DM_MAX_SETS_PER_LAUNCH) * (sh.per_image ? (unsigned long long)sh.B : 1ull)};
+    return Workspace{most_blocks(sets, sh, FORWARD), (unsigned long long)std::min(sh.S, DM_MAX_SETS_PER_LAUNCH) * (sh.per_image ? (unsigned long long)sh.B : 1ull)};
 }
 
 int forward(const DmRouterSet *sets, int S, int B, int E, int top_k, int dtype, int scores, int per_image,
@@ -754,7 +826,7 @@ int forward(const DmRouterSet *sets, int S, int B, int E, int top_k, int dtype, 
     for (int first = 0; first < S; first += DM_MAX_SETS_PER_LAUNCH) {
         RouterSets a;
         const int n = std::min(S - first, DM_MAX_SETS_PER_LAUNCH);
-        const unsigned blocks = (unsigned)describe(sets, first, n, sh, top_k, false, &a);
+        const unsigned blocks = (unsigned)describe(sets, first, n, sh, top_k, FORWARD, &a);
         if (blocks) {
             hipLaunchKernelGGL(forward_for((unsigned)E, given == 1 ? 1u : (unsigned)top_k, dtype == DM_F32, balance == nullptr), dim3(blocks), dim3(RT_THREADS), 0,
                                st, a, dtype, scores == DM_SCORES_SIGMOID ? 1 : 0, slots, status);
@@ -830,12 +902,12 @@ extern "C" int dm_balance_backward(const DmRouterSet *sets, int S, int B, int E,
     if (!slope || !inv_rows) return DM_E_INVALID_ARG;
     for (int s = 0; s < S; ++s)
         if (sets[s].Q > 0 && (!sets[s].logits || !sets[s].grad)) return DM_E_INVALID_ARG;
-    if (most_blocks(sets, sh, true) >= (1ull << 31)) return DM_E_UNSUPPORTED;
+    if (most_blocks(sets, sh, BACKWARD) >= (1ull << 31)) return DM_E_UNSUPPORTED;
     hipStream_t st = static_cast<hipStream_t>(stream);
     for (int first = 0; first < S; first += DM_MAX_SETS_PER_LAUNCH) {
         RouterSets a;
         const int n = std::min(S - first, DM_MAX_SETS_PER_LAUNCH);
-        const unsigned blocks = (unsigned)describe(sets, first, n, sh, 0, true, &a);
+        const unsigned blocks = (unsigned)describe(sets, first, n, sh, 0, BACKWARD, &a);
         const size_t g0 = (size_t)first * (per_image ? (size_t)B : 1);
         hipLaunchKernelGGL(dtype == DM_F32 ? backward_for<true>((unsigned)E) : backward_for<false>((unsigned)E), dim3(blocks), dim3(RT_THREADS), 0, st, a, dtype, scores == DM_SCORES_SIGMOID ? 1 : 0,
                            slope + g0 * E, inv_rows + g0, grad_balance ? grad_balance + g0 : nullptr,
