@@ -87,7 +87,7 @@ struct LossNode : torch::autograd::Node {
         TORCH_CHECK(!released, torch::autograd::ERR_BACKWARD_TWICE);
         variable_list out;
         {
-            at::AutoGradMode off(false);
+            const at::AutoDispatchBelowADInplaceOrView below;
             out = backward(grads);
         }
         if (!at::GradMode::is_enabled()) return out;

@@ -77,12 +77,28 @@ __device__ __forceinline__ void softmax_weights(float (&x)[N], float mx)
 #pragma unroll
     for (int j = 0; j < N; ++j) x[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[j], LOG2E, -base));
 }
-__device__ __forceinline__ float sigmoid_weight(float x, float c, float exp_c, float *rest)
+template <int N, bool REST>
+__device__ __forceinline__ void sigmoid_weights(float (&x)[N], float mx, float (&rest)[REST ? N : 1])
 {
-    const float t = __builtin_amdgcn_exp2f((-__builtin_fabsf(x) - c) * LOG2E);
-    const float r = __builtin_amdgcn_rcpf(1.0f + t * exp_c);
-    *rest = (x >= 0.0f ? t : 1.0f) * r;
-    return (x >= 0.0f ? 1.0f : t) * r;
+    auto weigh = [&](int j, float t, float r) {
+        const bool up = x[j] >= 0.0f;
+        if (REST) rest[REST ? j : 0] = (up ? t : 1.0f) * r;
+        x[j] = (up ? 1.0f : t) * r;
+    };
+    if (__any(mx < 0.0f)) {
+        const float c = fminf(mx, 0.0f), exp_c = __builtin_amdgcn_exp2f(c * LOG2E);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const float t = __builtin_amdgcn_exp2f((-__builtin_fabsf(x[j]) - c) * LOG2E);
+            weigh(j, t, __builtin_amdgcn_rcpf(__builtin_fmaf(t, exp_c, 1.0f)));
+        }
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const float t = __builtin_amdgcn_exp2f(-__builtin_fabsf(x[j]) * LOG2E);
+        weigh(j, t, __builtin_amdgcn_rcpf(1.0f + t));
+    }
 }
 
 // What the choice compares: an order in which no two of a row are equal where that can be had, and its least.
@@ -316,18 +332,13 @@ __global__ __launch_bounds__(RT_THREADS) void router_forward_kernel(const Router
             }
             float sum = nan ? __builtin_nanf("") : 0.0f;
             if (sigmoid) {
-                const float c = fminf(mx, 0.0f), exp_c = __builtin_amdgcn_exp2f(c * LOG2E);
-#pragma unroll
-                for (int j = 0; j < N; ++j) {
-                    float rest;
-                    x[j] = x[j] == ninf ? 0.0f : sigmoid_weight(x[j], c, exp_c, &rest);
-                    sum += x[j];
-                }
+                float none[1];
+                sigmoid_weights<N, false>(x, mx, none);
             } else {
                 softmax_weights(x, mx);
-#pragma unroll
-                for (int j = 0; j < N; ++j) sum += x[j];
             }
+#pragma unroll
+            for (int j = 0; j < N; ++j) sum += x[j];
             sum = dm::over_group<L>(sum, dm::Add());
             const bool live = sum != 0.0f;                     // (a NaN makes it NaN)
             const float inv = live ? __builtin_amdgcn_rcpf(sum) : 0.0f;
@@ -592,16 +603,9 @@ __global__ __launch_bounds__(RT_THREADS) void router_backward_kernel(const Route
         float sum = 0.0f, dot = 0.0f;
         float rest[N];
         if (sigmoid) {
-            const float c = fminf(mx, 0.0f), exp_c = __builtin_amdgcn_exp2f(c * LOG2E);
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                rest[j] = 1.0f;
-                x[j] = x[j] == ninf ? 0.0f : sigmoid_weight(x[j], c, exp_c, &rest[j]);
-            }
+            sigmoid_weights<N, true>(x, mx, rest);
         } else {
             softmax_weights(x, mx);
-#pragma unroll
-            for (int j = 0; j < N; ++j) rest[j] = 1.0f;
         }
 #pragma unroll
         for (int j = 0; j < N; ++j) {
@@ -613,13 +617,14 @@ __global__ __launch_bounds__(RT_THREADS) void router_backward_kernel(const Route
         const bool live = sum != 0.0f;
         const float inv = live ? __builtin_amdgcn_rcpf(sum) : 0.0f;
         dot *= inv;
-        // p (gb (f - dot) + gz lse)
-        const float lse = live ? mx + __builtin_amdgcn_logf(sum) * LN2 : 0.0f;
-        const float zpart = gz * lse;
+        // p (gb (f - dot) + gz lse); of a row that does not count 0 times 0, whatever comes from upstream
+        const float zpart = live ? gz * (mx + __builtin_amdgcn_logf(sum) * LN2) : 0.0f;
+        const float bpart = live ? gb : 0.0f;
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const float g = (x[j] * inv) * __builtin_fmaf(gb, f[j] - dot, zpart);
-            x[j] = live ? g * rest[j] : 0.0f;
+        for (int j = 0; j < N; ++j) x[j] = (x[j] * inv) * __builtin_fmaf(bpart, f[j] - dot, zpart);
+        if (sigmoid) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) x[j] *= rest[j];
         }
         if (there) dm::store_row<NQ, L, WIDE>(set.grad, dtype, (image_row + row) * E, sub, E, x);
     }
