@@ -792,6 +792,9 @@ BackwardKernel backward_for(unsigned E)
     }
 }
 
+// (a launch has fewer than 2^32 threads)
+constexpr unsigned long long MOST_BLOCKS = (1ull << 32) / RT_THREADS - 1, MOST_GROUPS = (1ull << 32) / FINISH_THREADS - 1;
+
 // Workspace: the slots of a launch's workgroups, then the sums of p of its groups.
 struct Workspace {
     unsigned long long blocks, groups;
@@ -824,7 +827,7 @@ int forward(const DmRouterSet *sets, int S, int B, int E, int top_k, int dtype, 
     }
     if (given == 1 && !balance) return DM_E_INVALID_ARG;       // (the counts of given indices need no logits)
     const Workspace need = workspace_of(sets, sh);
-    if (need.blocks >= (1ull << 31)) return DM_E_UNSUPPORTED;
+    if (need.blocks > MOST_BLOCKS || need.groups > MOST_GROUPS) return DM_E_UNSUPPORTED;
     if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0 || workspace_bytes < need.bytes(E)) return DM_E_INVALID_ARG;
     unsigned *slots = static_cast<unsigned *>(workspace);
     double *means = reinterpret_cast<double *>(slots + (size_t)std::max(1ull, need.blocks) * slot_words((unsigned)E));
@@ -907,7 +910,7 @@ extern "C" int dm_balance_backward(const DmRouterSet *sets, int S, int B, int E,
     if (!slope || !inv_rows) return DM_E_INVALID_ARG;
     for (int s = 0; s < S; ++s)
         if (sets[s].Q > 0 && (!sets[s].logits || !sets[s].grad)) return DM_E_INVALID_ARG;
-    if (most_blocks(sets, sh, BACKWARD) >= (1ull << 31)) return DM_E_UNSUPPORTED;
+    if (most_blocks(sets, sh, BACKWARD) > MOST_BLOCKS) return DM_E_UNSUPPORTED;
     hipStream_t st = static_cast<hipStream_t>(stream);
     for (int first = 0; first < S; first += DM_MAX_SETS_PER_LAUNCH) {
         RouterSets a;

@@ -254,7 +254,10 @@ def _status_word(device):
     index = device.index if device.index is not None else torch.cuda.current_device()
     status = _cls_status.get(index)
     if status is None:
-        status = _cls_status[index] = torch.zeros(1, dtype=torch.int32, device=device)
+        status = torch.zeros(1, dtype=torch.int32, device=device)
+        if not torch.cuda.is_current_stream_capturing():
+            torch.cuda.current_stream(device).synchronize()          # once: other streams' kernels write it too
+        _cls_status[index] = status
     return status
 
 

@@ -394,8 +394,8 @@ int dm_cross_entropy_from_saved(const uint8_t *codes, const int8_t *steps, int d
  *   workspace             device memory, 16-byte aligned, dm_balance_workspace bytes, overwritten
  * grad = grad_balance / n * p_e (f_e - sum_j f_j p_j) [* (1 - sigmoid(x_e))] + grad_z / n * 2 logsumexp(x) p_e;
  * grad_balance, grad_z: device float[groups], either may be NULL (no gradient from that side).
- * Sums of a fixed order: bitwise reproducible.  1 <= E <= 1024, 1 <= top_k <= E (with experts: top_k >= 1), Q of a set and
- * the total number of groups < 2^31 (DM_E_UNSUPPORTED beyond).  dm_balance_workspace returns a negative code for
+ * Sums of a fixed order: bitwise reproducible.  1 <= E <= 1024, 1 <= top_k <= E (with experts: top_k >= 1), B * Q of a set
+ * < 2^31, images of sixteen sets < 2^22 with per_image, else < 2^24 (DM_E_UNSUPPORTED beyond).  dm_balance_workspace returns a negative code for
  * arguments that the calls refuse.
  */
 #define DM_SCORES_SOFTMAX 0

@@ -51,6 +51,8 @@ def test_arguments_are_refused():
     both = sets_of(5, 5)
     both[1].experts = WORD                                                    # given for one set, not for the other
     assert loss(both, 2) == bad
+    # more workgroups than a launch has threads for: images by themselves, and images that are not dense
+    assert loss(sets_of(2), 1, B=1 << 22, per_image=1) == big and loss(sets_of(2, stride=99), 1, B=1 << 24) == big
     one[0].logits = None
     assert loss(one, 1) == bad
     assert lib.dm_balance_workspace(one, 1, 2, 0, 0) == bad and lib.dm_balance_workspace(one, 1, 2, 4096, 0) == big
@@ -73,8 +75,12 @@ def test_backward_arguments_are_refused():
     assert back(S=-1) == bad and back(E=0) == bad and back(dtype=-1) == bad and back(scores=5) == bad
     assert back(slope=None) == bad and back(inv=None) == bad
     assert back(scores=1) == bad                                              # sigmoid scores have no z
+    assert lib.dm_balance_backward(sets_of(2, stride=99), 1, 1 << 24, 8, 0, 0, 0, WORD, WORD, WORD, WORD, None) == _lib.E_UNSUPPORTED
     one[0].grad = None
     assert back() == bad
+    # the counts alone are those of logits
+    given = sets_of(5, experts=WORD)
+    assert lib.dm_expert_counts(given, 1, 2, 8, 2, 0, 0, WORD, 0x10000, 1 << 40, WORD, None) == bad
 
 
 def test_cpu_tensors_are_refused():

@@ -334,6 +334,51 @@ def test_only_one_of_the_losses_is_differentiated():
         grad.sum().backward()
 
 
+def test_the_graph_is_kept_or_not():
+    from detr_amd import losses
+
+    a = make((2, 30, 9), "f32", 4).cuda().requires_grad_(True)
+    out = losses.balance_losses(a, 2)
+    (first,) = torch.autograd.grad(out.balance.sum(), a, retain_graph=True)
+    (second,) = torch.autograd.grad(out.balance.sum(), a)
+    assert torch.equal(first, second)
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(out.z.sum(), a)
+    # logits that were changed in place since are noticed
+    b = a.detach().clone().requires_grad_(True)
+    out = losses.balance_losses(b, 2)
+    with torch.no_grad():
+        b.add_(1.0)
+    with pytest.raises(RuntimeError, match="inplace|in-place"):
+        out.balance.sum().backward()
+
+
+def test_one_tensor_for_two_sets_and_broadcast_logits():
+    from detr_amd import losses
+
+    x = make((2, 30, 9), "f32", 4)
+    dev = x.cuda().requires_grad_(True)
+    out = losses.balance_losses([dev, dev], 2)
+    weight = torch.tensor([1.0, 3.0]).cuda()
+    (twice,) = torch.autograd.grad(out.balance, dev, weight)
+    (once,) = torch.autograd.grad(losses.balance_losses(dev, 2).balance, dev, weight[:1])
+    torch.testing.assert_close(twice, 4 * once, rtol=8 * U, atol=2.0 ** -126)
+    # a row of logits for all queries, images that share their logits
+    row = make((1, 1, 9), "f32", 5).cuda().requires_grad_(True)
+    wide = row.expand(2, 30, 9)
+    out = losses.balance_losses(wide, 2)
+    want = oracle.balance_losses(row.detach().cpu().double().numpy(), 2, grad_balance=[1.0])
+    (grad,) = torch.autograd.grad(out.balance.sum(), row)
+    assert out.counts.tolist()[0] == (60 * want["counts"][0]).tolist()
+    # (60 gradients of 1 / 60 of the row's, added up in float32)
+    scale = np.abs(want["p"]) * (np.abs(want["f"]).max() * 2)
+    assert (np.abs(grad.cpu().numpy() - want["grad"]) <= (5 * 10 + 40 + 64) * U * (scale + np.abs(want["grad"])) + 2.0 ** -126).all()
+    shared = make((1, 30, 9), "f32", 6).cuda().requires_grad_(True)
+    (grad,) = torch.autograd.grad(losses.balance_losses(shared.expand(3, 30, 9), 2).balance.sum(), shared)
+    (want,) = torch.autograd.grad(losses.balance_losses(shared, 2).balance.sum(), shared)
+    torch.testing.assert_close(grad, want, rtol=0, atol=float(300 * U * want.abs().max()))
+
+
 def test_total():
     from detr_amd import losses
 

@@ -388,6 +388,24 @@ def test_views_streams_and_repeats():
         grad.sum().backward()
 
 
+def test_the_graph_is_kept_or_not():
+    from detr_amd import losses
+
+    x, cls = inputs((3, 40, 9), "f32", 9)
+    for fn in (lambda d: losses.focal_loss(d, cls.cuda(), 1.0, saved_bits=8),
+               lambda d: losses.cross_entropy(d, cls.clamp(max=8).cuda(), saved_bits=8)):
+        dev = x.cuda().requires_grad_(True)
+        loss = fn(dev)
+        (first,) = torch.autograd.grad(loss, dev, retain_graph=True)
+        # (the bytes are kept, not the logits: they may change)
+        with torch.no_grad():
+            dev.zero_()
+        (second,) = torch.autograd.grad(loss, dev)
+        assert torch.equal(first, second)
+        with pytest.raises(RuntimeError, match="second time"):
+            torch.autograd.grad(loss, dev)
+
+
 def test_two_captured_steps_side_by_side():
     from detr_amd import losses
 
