@@ -9,6 +9,8 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 ROOT = os.path.dirname(os.path.abspath(__file__))
 PKG = os.path.join(ROOT, "detr_amd")
@@ -22,7 +24,7 @@ HEADERS = [os.path.join(CSRC, h) for h in ("dm_common.h", "lanes.h", "cls_common
 # reference's elementwise torch ops (hipcc would otherwise fuse a*b+c into an fma).
 # -packed-fp32-ops: no v_pk_*_f32, which -O3 makes of ordinary float code by itself; some of their forms have given wrong
 # results now and then, with no error.
-FLAGS = ["--offload-arch=gfx950", "-O3", "-ffp-contract=off", "-fPIC", "-shared", "-std=c++17", "-Wno-pass-failed",
+FLAGS = ["--offload-arch=gfx950", "-O3", "-ffp-contract=off", "-fPIC", "-std=c++17", "-Wno-pass-failed",
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
@@ -112,11 +114,23 @@ def _build_kernels(force=False, verbose=False):
     hipcc = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
     # DETR_AMD_EXTRA_FLAGS: extra hipcc flags for instrumented one-off builds (e.g. -DDM_LAP_STAMPS)
     extra = os.environ.get("DETR_AMD_EXTRA_FLAGS", "").split()
-    cmd = [hipcc] + FLAGS + extra + ["-I", os.path.join(ROOT, "include"), "-I", CSRC, "-o", LIB] + \
-          [os.path.join(CSRC, s) for s in SOURCES]
-    if verbose:
-        print(" ".join(cmd))
-    subprocess.check_call(cmd)
+
+    def run(cmd):
+        if verbose:
+            print(" ".join(cmd))
+        subprocess.check_call(cmd)
+
+    # (the sources side by side: one after the other they take three minutes)
+    with tempfile.TemporaryDirectory() as objects:
+        def compile_one(source):
+            out = os.path.join(objects, source + ".o")
+            run([hipcc] + FLAGS + extra + ["-I", os.path.join(ROOT, "include"), "-I", CSRC, "-c", "-o", out,
+                                           os.path.join(CSRC, source)])
+            return out
+
+        with ThreadPoolExecutor(max_workers=min(len(SOURCES), os.cpu_count() or 1)) as pool:
+            compiled = list(pool.map(compile_one, SOURCES))
+        run([hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB] + compiled)
     return LIB
 
 
