@@ -654,33 +654,36 @@ int check_shape(const DmRouterSet *sets, int S, int B, int E, int per_image, Sha
     return DM_OK;
 }
 
-// Lanes per row and logits per lane.  Forward: ... 
+// Quads of four logits per lane, and lanes per row.
+//   Forward: as few lanes as can hold the row with sixteen logits each.  Every reduction over lanes is paid per row, every
+//   lane behind the row's end as well: 354 MB of float32 logits of 16, 48, 64 and 96 experts (top 2, 4, 4, 4) take 79, 79, 79 and
+//   80 us, with half as many logits per lane 105, 101, 89 and 117 us.
+//   Backward, float32: four logits per lane and up to sixteen lanes, whose store is a run of memory; in the forward pass's
+//   forms 12, 24 and 48 experts take 171, 169 and 157 us for 354 MB read and written instead of 152, 149 and 149.
+//   Backward, 16 bits: bound by instructions, not memory, where lanes lie behind the row's end: 12, 20, 33 and 96 experts take
+//   91, 95, 101 and 86 us for 177 MB read and written with twelve logits per lane, 103, 114, 145 and 96 us with four or eight.
 struct Form {
     int NQ, L;
 };
 Form forward_form(unsigned E)
 {
-    if (E <= 4) return {1, 1};
-    if (E <= 8) return {2, 1};
-    if (E <= 16) return {2, 2};
-    if (E <= 32) return {2, 4};
-    if (E <= 64) return {4, 4};
-    if (E <= 96) return {3, 8};
-    if (E <= 128) return {4, 8};
-    if (E <= 192) return {3, 16};
-    if (E <= 256) return {4, 16};
+    if (E <= 8) return {E <= 4 ? 1 : 2, 1};
+    if (E <= 16) return {E <= 12 ? 3 : 4, 1};
+    if (E <= 32) return {E <= 24 ? 3 : 4, 2};
+    if (E <= 64) return {E <= 48 ? 3 : 4, 4};
+    if (E <= 128) return {E <= 96 ? 3 : 4, 8};
+    if (E <= 256) return {E <= 192 ? 3 : 4, 16};
     return {4, E <= 512 ? 32 : 64};
 }
-Form backward_form(unsigned E)
+Form backward_form(unsigned E, bool wide)
 {
     if (E <= 4) return {1, 1};
     if (E <= 8) return {1, 2};
-    if (E <= 16) return {1, 4};
-    if (E <= 32) return {1, 8};
-    if (E <= 64) return {1, 16};
-    if (E <= 128) return {2, 16};
-    if (E <= 192) return {3, 16};
-    if (E <= 256) return {4, 16};
+    if (E <= 16) return !wide && E <= 12 ? Form{3, 1} : Form{1, 4};
+    if (E <= 32) return !wide && E <= 24 ? Form{3, 2} : Form{1, 8};
+    if (E <= 64) return !wide && E <= 48 ? Form{3, 4} : Form{1, 16};
+    if (E <= 128) return E <= 96 ? Form{3, 8} : Form{2, 16};
+    if (E <= 256) return {E <= 192 ? 3 : 4, 16};
     return {4, E <= 512 ? 32 : 64};
 }
 
@@ -688,23 +691,27 @@ Form backward_form(unsigned E)
 // 1020 workgroups of the float32 kernel a second round of a few of them doubled the time), each with the same number of trips.
 // Per CU, at the kernels' registers: three of the forward kernel, eight of the backward kernel.  (Five of the forward kernel fit
 // for 16 bits: no faster, and two thirds more slots to add.)
-constexpr int FORWARD = 3 * 256, BACKWARD = 8 * 256;
+struct Pass {
+    int resident, lanes;         // workgroups, lanes per row
+};
+Pass forward_pass(const Shape &sh) { return {3 * 256, forward_form((unsigned)sh.E).L}; }
+Pass backward_pass(const Shape &sh, bool wide) { return {8 * 256, backward_form((unsigned)sh.E, wide).L}; }
 struct Chunks {
     unsigned count, rows;
 };
-Chunks chunks_of(const Shape &sh, int Q, int resident)
+Chunks chunks_of(const Shape &sh, int Q, const Pass &pass)
 {
     const long long images = sh.merged ? 1 : sh.B;
     const long long rows = sh.merged ? (long long)sh.B * Q : Q;
-    const long long trip = RT_THREADS / (resident == BACKWARD ? backward_form((unsigned)sh.E) : forward_form((unsigned)sh.E)).L;
+    const long long trip = RT_THREADS / pass.lanes;
     const long long trips = std::max(1ll, (rows + trip - 1) / trip);
-    const long long want = std::max(1ll, resident / std::max(1ll, std::min<long long>(sh.S, DM_MAX_SETS_PER_LAUNCH) * images));
+    const long long want = std::max(1ll, pass.resident / std::max(1ll, std::min<long long>(sh.S, DM_MAX_SETS_PER_LAUNCH) * images));
     const long long each = (trips + want - 1) / want;
     return Chunks{(unsigned)((trips + each - 1) / each), (unsigned)(each * trip)};
 }
 
 // The kernel arguments of sets first .. first + n - 1; returns the launch's workgroups.
-unsigned long long describe(const DmRouterSet *sets, int first, int n, const Shape &sh, int k, int resident, RouterSets *a)
+unsigned long long describe(const DmRouterSet *sets, int first, int n, const Shape &sh, int k, const Pass &pass, RouterSets *a)
 {
     a->S = n;
     a->E = (unsigned)sh.E;
@@ -721,7 +728,7 @@ unsigned long long describe(const DmRouterSet *sets, int first, int n, const Sha
         s.image_stride = in.image_stride ? in.image_stride : (int64_t)in.Q * sh.E;
         s.images = sh.merged ? 1u : (unsigned)sh.B;
         s.Q = sh.merged ? (unsigned)sh.B * (unsigned)in.Q : (unsigned)in.Q;
-        const Chunks c = chunks_of(sh, in.Q, resident);
+        const Chunks c = chunks_of(sh, in.Q, pass);
         s.chunks = c.count;
         s.chunk_rows = c.rows;
         s.first_block = (unsigned)blocks;
@@ -732,13 +739,13 @@ unsigned long long describe(const DmRouterSet *sets, int first, int n, const Sha
 }
 
 // (the sets of a call go through launches of up to DM_MAX_SETS_PER_LAUNCH, one after the other, over the same workspace)
-unsigned long long most_blocks(const DmRouterSet *sets, const Shape &sh, int resident)
+unsigned long long most_blocks(const DmRouterSet *sets, const Shape &sh, const Pass &pass)
 {
     unsigned long long most = 0;
     for (int first = 0; first < sh.S; first += DM_MAX_SETS_PER_LAUNCH) {
         unsigned long long blocks = 0;
         for (int s = first; s < std::min(sh.S, first + DM_MAX_SETS_PER_LAUNCH); ++s)
-            blocks += (unsigned long long)(sh.merged ? 1 : sh.B) * chunks_of(sh, sets[s].Q, resident).count;
+            blocks += (unsigned long long)(sh.merged ? 1 : sh.B) * chunks_of(sh, sets[s].Q, pass).count;
         most = std::max(most, blocks);
     }
     return most;
@@ -766,9 +773,11 @@ ForwardKernel forward_for(unsigned E, unsigned k, bool wide, bool count_only)
 {
     const Form f = forward_form(E);
     switch (f.L) {
-    case 1: return f.NQ == 1 ? forward_with<1, 1>(k, wide, count_only) : forward_with<2, 1>(k, wide, count_only);
-    case 2: return forward_with<2, 2>(k, wide, count_only);
-    case 4: return f.NQ == 2 ? forward_with<2, 4>(k, wide, count_only) : forward_with<4, 4>(k, wide, count_only);
+    case 1:
+        return f.NQ == 1 ? forward_with<1, 1>(k, wide, count_only) : f.NQ == 2 ? forward_with<2, 1>(k, wide, count_only)
+               : f.NQ == 3 ? forward_with<3, 1>(k, wide, count_only) : forward_with<4, 1>(k, wide, count_only);
+    case 2: return f.NQ == 3 ? forward_with<3, 2>(k, wide, count_only) : forward_with<4, 2>(k, wide, count_only);
+    case 4: return f.NQ == 3 ? forward_with<3, 4>(k, wide, count_only) : forward_with<4, 4>(k, wide, count_only);
     case 8: return f.NQ == 3 ? forward_with<3, 8>(k, wide, count_only) : forward_with<4, 8>(k, wide, count_only);
     case 16: return f.NQ == 3 ? forward_with<3, 16>(k, wide, count_only) : forward_with<4, 16>(k, wide, count_only);
     case 32: return forward_with<4, 32>(k, wide, count_only);
@@ -778,12 +787,12 @@ ForwardKernel forward_for(unsigned E, unsigned k, bool wide, bool count_only)
 template <bool WIDE>
 BackwardKernel backward_for(unsigned E)
 {
-    const Form f = backward_form(E);
+    const Form f = backward_form(E, WIDE);
     switch (f.L) {
-    case 1: return router_backward_kernel<1, 1, WIDE>;
-    case 2: return router_backward_kernel<1, 2, WIDE>;
-    case 4: return router_backward_kernel<1, 4, WIDE>;
-    case 8: return router_backward_kernel<1, 8, WIDE>;
+    case 1: if constexpr (!WIDE) { if (f.NQ == 3) return router_backward_kernel<3, 1, WIDE>; } return router_backward_kernel<1, 1, WIDE>;
+    case 2: if constexpr (!WIDE) { if (f.NQ == 3) return router_backward_kernel<3, 2, WIDE>; } return router_backward_kernel<1, 2, WIDE>;
+    case 4: if constexpr (!WIDE) { if (f.NQ == 3) return router_backward_kernel<3, 4, WIDE>; } return router_backward_kernel<1, 4, WIDE>;
+    case 8: return f.NQ == 3 ? router_backward_kernel<3, 8, WIDE> : router_backward_kernel<1, 8, WIDE>;
     case 16:
         return f.NQ == 1 ? router_backward_kernel<1, 16, WIDE> : f.NQ == 2 ? router_backward_kernel<2, 16, WIDE>
                : f.NQ == 3 ? router_backward_kernel<3, 16, WIDE> : router_backward_kernel<4, 16, WIDE>;
@@ -802,7 +811,7 @@ struct Workspace {
 };
 Workspace workspace_of(const DmRouterSet *sets, const Shape &sh)
 {
-    return Workspace{most_blocks(sets, sh, FORWARD), (unsigned long long)std::min(sh.S, DM_MAX_SETS_PER_LAUNCH) * (sh.per_image ? (unsigned long long)sh.B : 1ull)};
+    return Workspace{most_blocks(sets, sh, forward_pass(sh)), (unsigned long long)std::min(sh.S, DM_MAX_SETS_PER_LAUNCH) * (sh.per_image ? (unsigned long long)sh.B : 1ull)};
 }
 
 int forward(const DmRouterSet *sets, int S, int B, int E, int top_k, int dtype, int scores, int per_image,
@@ -834,7 +843,7 @@ int forward(const DmRouterSet *sets, int S, int B, int E, int top_k, int dtype, 
     for (int first = 0; first < S; first += DM_MAX_SETS_PER_LAUNCH) {
         RouterSets a;
         const int n = std::min(S - first, DM_MAX_SETS_PER_LAUNCH);
-        const unsigned blocks = (unsigned)describe(sets, first, n, sh, top_k, FORWARD, &a);
+        const unsigned blocks = (unsigned)describe(sets, first, n, sh, top_k, forward_pass(sh), &a);
         if (blocks) {
             hipLaunchKernelGGL(forward_for((unsigned)E, given == 1 ? 1u : (unsigned)top_k, dtype == DM_F32, balance == nullptr), dim3(blocks), dim3(RT_THREADS), 0,
                                st, a, dtype, scores == DM_SCORES_SIGMOID ? 1 : 0, slots, status);
@@ -910,12 +919,12 @@ extern "C" int dm_balance_backward(const DmRouterSet *sets, int S, int B, int E,
     if (!slope || !inv_rows) return DM_E_INVALID_ARG;
     for (int s = 0; s < S; ++s)
         if (sets[s].Q > 0 && (!sets[s].logits || !sets[s].grad)) return DM_E_INVALID_ARG;
-    if (most_blocks(sets, sh, BACKWARD) > MOST_BLOCKS) return DM_E_UNSUPPORTED;
+    if (most_blocks(sets, sh, backward_pass(sh, dtype == DM_F32)) > MOST_BLOCKS) return DM_E_UNSUPPORTED;
     hipStream_t st = static_cast<hipStream_t>(stream);
     for (int first = 0; first < S; first += DM_MAX_SETS_PER_LAUNCH) {
         RouterSets a;
         const int n = std::min(S - first, DM_MAX_SETS_PER_LAUNCH);
-        const unsigned blocks = (unsigned)describe(sets, first, n, sh, 0, BACKWARD, &a);
+        const unsigned blocks = (unsigned)describe(sets, first, n, sh, 0, backward_pass(sh, dtype == DM_F32), &a);
         const size_t g0 = (size_t)first * (per_image ? (size_t)B : 1);
         hipLaunchKernelGGL(dtype == DM_F32 ? backward_for<true>((unsigned)E) : backward_for<false>((unsigned)E), dim3(blocks), dim3(RT_THREADS), 0, st, a, dtype, scores == DM_SCORES_SIGMOID ? 1 : 0,
                            slope + g0 * E, inv_rows + g0, grad_balance ? grad_balance + g0 : nullptr,
