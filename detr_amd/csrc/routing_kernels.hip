@@ -158,8 +158,9 @@ __device__ __forceinline__ void in_order(const dm::RawRow<NQ, true> &raw, int dt
     *nan = false;
 #pragma unroll
     for (int j = 0; j < 4 * NQ; ++j) {
-        *nan |= y[j] != y[j];
-        y[j] = dm::max3(y[j], ninf, ninf);
+        const bool is = y[j] != y[j];
+        *nan |= is;
+        y[j] = is ? ninf : y[j];
     }
 }
 template <int NQ, int L>
