@@ -189,12 +189,19 @@ __device__ __forceinline__ void store_row(void *base, int dtype, size_t first, u
     else store(static_cast<half_t *>(base) + first);
 }
 
-// Largest of three, in one instruction.  (fmaxf would first quiet each argument, as IEEE asks of a signalling NaN.)  A quiet
+// Largest and smallest of three, in one instruction.  (fmaxf would first quiet each argument, as IEEE asks of a signalling NaN.)  A quiet
 // NaN is passed over, a signalling one may come out.
 __device__ __forceinline__ float max3(float a, float b, float c)
 {
     float r;
     asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+
+__device__ __forceinline__ float min3(float a, float b, float c)
+{
+    float r;
+    asm("v_min3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
     return r;
 }
 
@@ -226,7 +233,6 @@ __device__ __forceinline__ double partner(double v)
     return __builtin_bit_cast(double, partner<STEP>(__builtin_bit_cast(unsigned long long, v)));
 }
 
-struct Max { template <typename V> __device__ __forceinline__ V operator()(V a, V b) const { return a > b ? a : b; } };
 struct Min { template <typename V> __device__ __forceinline__ V operator()(V a, V b) const { return a < b ? a : b; } };
 struct Add { template <typename V> __device__ __forceinline__ V operator()(V a, V b) const { return a + b; } };
 

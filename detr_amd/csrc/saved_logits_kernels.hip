@@ -10,6 +10,7 @@
 //   focal           blocks of 128 consecutive logits of the flat array, clamped to +-20 first: sigmoid(-20) = 2e-9 is below
 //                   the rounding of a float32 gradient of order one, and one masked logit does not take the block's
 //                   resolution away.  The span is 40 at most, so 2^-2 always suffices and no byte is cut off at 255.
+//                   Logits of rows that do not count take no part: a padded row may hold anything.
 //                   A head per block, 32 bits: largest whole number << 8 | e.
 //   cross entropy   a block is a row: the softmax does not change when a row's largest logit is taken off, so e is all that
 //                   is kept beside the bytes.  2^-3 at most: logits further below the largest than 31.9 are cut off there,
@@ -123,7 +124,7 @@ struct BlockRows {
     int64_t label[QUADS][ROWS];
     unsigned col[QUADS];
     int hot[QUADS][ROWS];       // place of the row's positive logit in the quad, if it is there
-    bool skipped;               // some row may not count: `counts` has to be asked
+    bool skipped;               // some row may not count: `dropped` has to be asked
 
     // (first: of the lane's logits in the flat array)
     __device__ __forceinline__ void ask(const int64_t *cls, const Walk &at, unsigned first, unsigned rows)
@@ -154,11 +155,19 @@ struct BlockRows {
         if (ONE_CLASS) return hot[q][k] == (int)k;
         return hot[q][0] == (int)k || hot[q][1] == (int)k;
     }
-    __device__ __forceinline__ bool counts(unsigned q, unsigned k, unsigned C, const FocalParams &fp, bool *bad) const
+    // Which of a quad's logits (a bit each) are of rows that do not count.
+    __device__ __forceinline__ unsigned dropped(unsigned q, unsigned C, const FocalParams &fp, bool *bad) const
     {
-        const int code = row_code(ONE_CLASS ? label[q][k] : col[q] + k >= C ? label[q][1] : label[q][0], C, fp);
-        *bad |= code == ROW_BAD;
-        return code >= 0;
+        unsigned of_row[ROWS];
+#pragma unroll
+        for (unsigned k = 0; k < ROWS; ++k) {
+            const int code = row_code(label[q][k], C, fp);
+            *bad |= code == ROW_BAD;
+            of_row[k] = code < 0 ? 15u : 0u;
+        }
+        if (ONE_CLASS) return (of_row[0] & 1u) | (of_row[1] & 2u) | (of_row[ROWS - 2] & 4u) | (of_row[ROWS - 1] & 8u);
+        const unsigned first = (1u << min(C - col[q], 4u)) - 1;      // of the first row
+        return (of_row[0] & first) | (of_row[1] & ~first);
     }
 };
 
@@ -178,11 +187,24 @@ __global__ __launch_bounds__(CLS_THREADS) void focal_saved_kernel(const T *__res
     float acc = 0.0f;
     bool bad = false;
 
-    // a block with its logits and rows; `end`: logits of the flat array (whole blocks lie before it)
-    auto work = [&](unsigned block, const float (&v)[4 * QUADS], BlockRows<ONE_CLASS> &rows_of, bool whole) {
+    // a block with its logits and rows; whole: all 128 are there
+    auto work = [&](unsigned block, float (&v)[4 * QUADS], BlockRows<ONE_CLASS> &rows_of, bool whole) {
         const unsigned first = block * BLOCK + 4 * sub;
-        auto inside = [&](unsigned q, unsigned k) { return whole || first + 4 * LANES * q + k < n; };
         rows_of.settle(C, fp);
+        // logits of rows that do not count, or behind the last one, take no part, whatever they hold: at an infinity on their
+        // class's side their loss is 0
+        unsigned dropped = 0;
+        if (rows_of.skipped || !whole) {
+#pragma unroll
+            for (unsigned q = 0; q < QUADS; ++q) {
+                const unsigned at = first + 4 * LANES * q, there = whole ? 4u : at < n ? min(n - at, 4u) : 0u;
+                const unsigned out = (rows_of.dropped(q, C, fp, &bad) | (15u << there)) & 15u;
+#pragma unroll
+                for (unsigned k = 0; k < 4; ++k)
+                    if (out >> k & 1) v[4 * q + k] = rows_of.positive(q, k) ? __builtin_huge_valf() : -__builtin_huge_valf();
+                dropped |= out << (4 * q);
+            }
+        }
         float c[4 * QUADS], high = -FOCAL_CLAMP, low = FOCAL_CLAMP, sum = 0.0f;
         bool nan = false;
 #pragma unroll
@@ -195,32 +217,39 @@ __global__ __launch_bounds__(CLS_THREADS) void focal_saved_kernel(const T *__res
                 const FocalParts f = focal_parts<GAMMA2>(positive ? -x : x, fp.gamma);
                 term[k] = (positive ? alpha1 : alpha0) * (f.softplus * f.power);
                 c[4 * q + k] = __builtin_amdgcn_fmed3f(x, -FOCAL_CLAMP, FOCAL_CLAMP);
-                if (inside(q, k)) {
-                    nan |= x != x;
-                    low = __builtin_amdgcn_fmed3f(low, c[4 * q + k], -FOCAL_CLAMP);
-                    high = __builtin_amdgcn_fmed3f(high, c[4 * q + k], FOCAL_CLAMP);
-                }
+                nan |= x != x;
             }
-            if (rows_of.skipped || !whole) {
-#pragma unroll
-                for (unsigned k = 0; k < 4; ++k) term[k] = inside(q, k) && rows_of.counts(q, k, C, fp, &bad) ? term[k] : 0.0f;
-            }
+            low = dm::min3(dm::min3(low, c[4 * q], c[4 * q + 1]), c[4 * q + 2], c[4 * q + 3]);
+            high = dm::max3(dm::max3(high, c[4 * q], c[4 * q + 1]), c[4 * q + 2], c[4 * q + 3]);
             sum += (term[0] + term[1]) + (term[2] + term[3]);
         }
         acc += sum;
         if (!codes) return;
+        if (dropped) {
+            low = FOCAL_CLAMP;
+            high = -FOCAL_CLAMP;
+#pragma unroll
+            for (unsigned j = 0; j < 4 * QUADS; ++j) {
+                low = dropped >> j & 1 ? low : dm::min3(low, c[j], c[j]);
+                high = dropped >> j & 1 ? high : dm::max3(high, c[j], c[j]);
+            }
+        }
         high = dm::largest<LANES>(high);
         low = -dm::largest<LANES>(-low);
         const bool block_nan = ((__ballot(nan) >> (lane & ~(LANES - 1))) & ((1u << LANES) - 1)) != 0;
         const int e = step_exponent(high, low, FOCAL_COARSEST);
         const float inverse = power_of_two(-e);
         const float top = __builtin_rintf(high * inverse);
+        if (dropped) {
+#pragma unroll
+            for (unsigned j = 0; j < 4 * QUADS; ++j)
+                if (dropped >> j & 1) c[j] = high;             // (the byte 0)
+        }
 #pragma unroll
         for (unsigned q = 0; q < QUADS; ++q) {
             unsigned packed = 0;
 #pragma unroll
-            for (unsigned k = 0; k < 4; ++k)
-                packed = pack_code(packed, k, inside(q, k) ? top - __builtin_rintf(c[4 * q + k] * inverse) : 0.0f);
+            for (unsigned k = 0; k < 4; ++k) packed = pack_code(packed, k, top - __builtin_rintf(c[4 * q + k] * inverse));
             codes[block * (BLOCK / 4) + LANES * q + sub] = packed;
         }
         if (sub == 0) heads[block] = block_nan ? (NOT_A_NUMBER & 255) : (int)top * 256 | (e & 255);
@@ -306,9 +335,10 @@ __global__ __launch_bounds__(CLS_THREADS) void focal_from_saved_kernel(const uns
                 g[k] = (positive ? alpha1 : alpha0) * slope;
             }
             if (rows_of.skipped) {
-                bool bad;
+                bool bad = false;
+                const unsigned out = rows_of.dropped(q, C, fp, &bad);
 #pragma unroll
-                for (unsigned k = 0; k < 4; ++k) g[k] = rows_of.counts(q, k, C, fp, &bad) ? g[k] : 0.0f;
+                for (unsigned k = 0; k < 4; ++k) g[k] = out >> k & 1 ? 0.0f : g[k];
             }
             if (block < whole) {
                 Four t;
@@ -647,12 +677,12 @@ void launch_focal_from_saved(const uint8_t *codes, const int32_t *heads, const i
                        rows, fp, grad_loss, static_cast<T *>(grad));
 }
 
-// Workgroups for a number of trips: as many as the chip holds at once (seven per CU at these kernels' registers), each with
-// the same number of trips.  (256 x 900 x 91 logits are 5119 trips of the focal kernels: with 2048 workgroups half of them
-// make three and the others wait for them.)
+// Workgroups for a number of trips: as many as the chip holds at once (six per CU at these kernels' registers), each with the
+// same number of trips.  (256 x 900 x 91 logits are 5119 trips of the focal kernels: with 1707 workgroups, the most of which
+// each makes three, 171 of them wait for the others' end, 27.9 us; 1280 that make four take 26.8.)
 unsigned even_blocks(unsigned trips)
 {
-    constexpr unsigned RESIDENT = 7 * 256;
+    constexpr unsigned RESIDENT = 6 * 256;
     static_assert(RESIDENT <= (unsigned)CLS_MAX_BLOCKS, "a partial sum for each");
     const unsigned each = std::max(1u, (trips + RESIDENT - 1) / RESIDENT);
     return std::max(1u, (trips + each - 1) / each);

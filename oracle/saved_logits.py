@@ -16,21 +16,29 @@ def step_exponent(block, coarsest):
     return coarsest
 
 
-def focal_codes(x):
-    """(bytes [n], heads [blocks], decoded logits like x) of the flat array; the heads as signed 32-bit words."""
+def focal_codes(x, keep=True):
+    """(bytes [n], heads [blocks], decoded logits like x) of the flat array; the heads as signed 32-bit words.  keep: whether a
+    logit's row counts; the others take no part (they decode to 0 here, a block of them alone has the head 0).
+    """
     flat = np.asarray(x, dtype=np.float64).reshape(-1)
+    keep = np.broadcast_to(keep, np.shape(x)).reshape(-1)
     codes, heads, decoded = np.zeros(flat.size, np.uint8), [], np.empty(flat.size)
     for i in range(0, flat.size, 128):
-        block = np.clip(flat[i:i + 128], -FOCAL_CLAMP, FOCAL_CLAMP)
+        kept = np.flatnonzero(keep[i:i + 128]) + i
+        decoded[i:i + 128] = 0.0
+        if not kept.size:
+            heads.append(0)
+            continue
+        block = np.clip(flat[kept], -FOCAL_CLAMP, FOCAL_CLAMP)
         if np.isnan(block).any():
             heads.append(NOT_A_NUMBER & 255)
-            decoded[i:i + 128] = np.nan
+            decoded[kept] = np.nan
             continue
         e = step_exponent(block, FOCAL_COARSEST)
         q = np.rint(block * 2.0 ** -e)
-        codes[i:i + 128] = q.max() - q
+        codes[kept] = q.max() - q
         heads.append(int(q.max()) * 256 + (e & 255))
-        decoded[i:i + 128] = q * 2.0 ** e
+        decoded[kept] = q * 2.0 ** e
     return codes, np.array(heads, dtype=np.int64).astype(np.int32), decoded.reshape(np.shape(x))
 
 
@@ -68,7 +76,7 @@ def focal(x, cls, num_boxes, alpha=0.25, gamma=2.0, ignore_index=None):
     with np.errstate(all="ignore"):
         softplus, s, _ = parts(sign * x)
         loss = np.where(keep, factor * softplus * s ** gamma, 0.0).sum()
-        decoded = focal_codes(x)[2]
+        decoded = focal_codes(x, keep)[2]
         softplus, s, rest = parts(sign * decoded)
         grad = np.where(keep, sign * factor * s ** gamma * (s + gamma * softplus * rest), 0.0)
     return loss, grad, decoded

@@ -209,13 +209,33 @@ def test_gamma_and_alpha(gamma, alpha):
     check_focal(x, cls, alpha=alpha, gamma=gamma)
 
 
+@pytest.mark.parametrize("C", [1, 2, 3, 11, 91, 128, 300])
+@pytest.mark.parametrize("filled", [float("nan"), float("inf"), -float("inf"), 3e4])
+def test_what_rows_that_do_not_count_hold_changes_nothing(C, filled):
+    """A block of the focal code spans several rows: the others keep their gradients, to the bit."""
+    from detr_amd import losses
+
+    x, cls = inputs((5, 37, C), "f32", 6 * C)
+    ignored = torch.rand(5, 37, generator=torch.Generator().manual_seed(C)) < 0.4
+    ignored[2] = True
+    cls[ignored] = -1
+    grads, sums = [], []
+    for value in (0.0, filled):
+        x[ignored] = value
+        dev = x.cuda().requires_grad_(True)
+        sums.append(losses.focal_loss(dev, cls.cuda(), 3.0, ignore_index=-1, saved_bits=8))
+        grads.append(torch.autograd.grad(sums[-1], dev)[0])
+    assert torch.equal(sums[0], sums[1]) and torch.equal(grads[0], grads[1])
+    assert bool((grads[1][ignored.cuda()] == 0).all()) and bool(grads[1][~ignored.cuda()].ne(0).all())
+    x[ignored] = 0.0
+    check_focal(x, cls, ignore_index=-1)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 def test_ignored_rows(dtype):
     x, cls = inputs((4, 33, 11), dtype, 1)
     cls[torch.rand(4, 33, generator=torch.Generator().manual_seed(1)) < 0.4] = -1
     x[cls == -1] = float("nan")
-    # (an ignored row's NaN stays out of the loss; the focal code marks a block of 128 logits, so there the others of the block
-    # have no gradient either and only the loss is compared)
     from detr_amd import losses
 
     want, _, _ = oracle.focal(torch.nan_to_num(x).double().numpy(), cls.numpy(), 3.0, ignore_index=-1)
