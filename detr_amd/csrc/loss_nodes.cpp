@@ -201,7 +201,7 @@ Tensor cls_losses(const std::vector<Tensor> &logits, const std::vector<Tensor> &
         TORCH_CHECK_VALUE(x.dim() >= 1 && x.sizes().slice(0, x.dim() - 1) == cls.sizes(), "logits ", x.sizes(), " must be target_cls ",
                           cls.sizes(), " + [C]");
         TORCH_CHECK_VALUE(x.size(-1) >= 1, "logits of no class");
-        TORCH_CHECK_NOT_IMPLEMENTED(x.size(-1) < (1ll << 31), "rows * C must be below 2^31");
+        TORCH_CHECK_NOT_IMPLEMENTED(x.size(-1) < (1ll << 31) && x.numel() < (1ll << 31), "rows * C must be below 2^31");
     }
     const bool grad = wants_grad(logits);
     std::shared_ptr<ClsNode> node;

@@ -264,6 +264,38 @@ def test_large_and_infinite_logits(scores, E):
     assert int(out.counts[0, 2, 1]) >= 1
 
 
+@pytest.mark.parametrize("E", [4, 8, 40, 200, 700])
+def test_a_signalling_nan_is_not_chosen(E):
+    from detr_amd import losses
+
+    x = make((2, 67, E), "f32", E)
+    quiet, signalling = x.clone(), x.clone()
+    quiet[:, ::3, 1::2] = float("nan")
+    signalling.view(torch.int32)[:, ::3, 1::2] = 0x7F800001
+    for k in (1, 2):
+        assert torch.equal(losses.expert_counts(signalling.cuda(), k), losses.expert_counts(quiet.cuda(), k))
+        assert losses.balance_losses(signalling.cuda(), k).balance.isnan().all()
+
+
+def test_offsets_beyond_32_bits():
+    """More than 2^32 logits: the rows of a short pattern over and over.  A lane adds Q / (768 x 256) = 2731 rows."""
+    from detr_amd import losses
+
+    pattern = make((1, 4096, 8), "bf16", 5)
+    times = 131073
+    x = pattern[0].cuda().expand(times, 4096, 8).reshape(1, -1, 8).requires_grad_(True)
+    assert x.numel() > 1 << 32
+    out = losses.balance_losses(x, 2)
+    want = losses.balance_losses(pattern.cuda().requires_grad_(True), 2)
+    assert torch.equal(out.counts, want.counts * times)
+    assert torch.equal(losses.expert_counts(x, 2), out.counts)
+    assert abs(out.balance.item() - want.balance.item()) <= (2731 + 700) * U * want.balance.item()
+    assert abs(out.z.item() - want.z.item()) <= (2731 + 700) * U * want.z.item()
+    (grad,) = torch.autograd.grad(out.balance.sum() + out.z.sum(), x, retain_graph=False, grad_outputs=torch.tensor(1e6).cuda())
+    tiles = grad.view(times, 4096, 8)
+    assert bool(tiles[0].ne(0).any()) and bool((tiles == tiles[:1]).all())
+
+
 def test_gradient_against_differences():
     """Central differences of the loss itself, in the kernel's own arithmetic.  The loss is a smooth function of the logits
     while no choice changes (steps of 2^-6 between logits that lie at least 2^-4 apart): the difference quotient is off by

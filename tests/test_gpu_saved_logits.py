@@ -335,6 +335,35 @@ def test_the_loss_is_the_references(name):
     assert abs(loss.item() - case.loss) <= 1e-5 * abs(case.loss) + 1e-7
 
 
+@pytest.mark.parametrize("kind", ["focal", "ce"])
+def test_the_largest_sizes(kind):
+    """Just below 2^31 logits, the rows of a short pattern (of whole blocks) over and over: the same gradients everywhere."""
+    from detr_amd import losses
+
+    C, times = 91, 184365
+    x, cls = inputs((128, C), "bf16", 7, none=C - 1)
+    big = x.cuda().expand(times, 128, C).reshape(-1, C).requires_grad_(True)
+    assert (1 << 31) - 128 * C < big.numel() < 1 << 31
+    maps = cls.cuda().expand(times, 128).reshape(-1)
+    small = x.cuda().requires_grad_(True)
+
+    def loss(x, cls, n):
+        return losses.focal_loss(x, cls, n, saved_bits=8) if kind == "focal" else losses.cross_entropy(x, cls, saved_bits=8)
+
+    # (a lane adds up to 2^31 / (1280 x 256) logits in float32, or the rows' terms: 6600 additions)
+    got, want = loss(big, maps, float(times)), loss(small, cls.cuda(), 1.0)
+    assert abs(got.item() - want.item()) <= (6600 + 200) * U * want.item()
+    (grad,) = torch.autograd.grad(got, big, torch.tensor(float(times)).cuda())
+    tiles = grad.view(times, 128, C)
+    assert bool((tiles == tiles[:1]).all())
+    (few,) = torch.autograd.grad(want, small)
+    if kind == "focal":                      # (the same scale, exactly or but for the rounding of 1 / times, and of its product)
+        off = (tiles[0].float() - few.float()).abs()
+        assert bool((off <= (2 * 2.0 ** -8 + 4 * U) * few.float().abs()).all())
+    with pytest.raises(NotImplementedError):
+        loss(torch.empty(1, 1, dtype=torch.bfloat16, device="cuda").expand(1 << 31, 1), maps[:1].expand(1 << 31), 1.0)
+
+
 def test_gradient_against_differences():
     """Central differences of the loss (the 32-bit call's) at logits that the bytes hold exactly (multiples of 1/16 over a
     range below 15.9).  h = 2^-5: off by h^2 / 6 times a third derivative (of a focal term or a row's loss: below 4, over the
