@@ -10,6 +10,15 @@
 // Forward: workgroups walk chunks of an image's rows, a group of lanes per row; sums over rows stay in registers of the
 // lane that owns the expert, and leave once per workgroup, into a slot of the workspace.  A second kernel adds the slots in
 // index order in 64 bits: no float atomics, the same bits every run.
+//
+// What bounds it, as measured (a copy of a GiB runs at 5.1 TB/s, a kernel of a few workgroups takes 4 us among others):
+//   memory          6 x 256 x 900 x 64 float32, top 4 (354 MB): forward 107 us, sums and loss 5 each, backward 123 (708 MB at
+//                   5.8 TB/s).  Forward, sums and loss by themselves, over and over, take 75 (4.7 TB/s); in a step they wait for the
+//                   gradients of the one before, of which the caches hold up to 256 MB, to be written.
+//   instructions    16-bit logits with many choices: 2 x 64 x 1050 x 160 bfloat16, sigmoid scores, top 8 (43 MB): forward 36 us,
+//                   sums and loss 7, backward 27; counts alone of 256 x 900 x 256, top 8 (118 MB): 45 us, the vector units
+//                   busy 81 % of it, 22 instructions per logit of which 8 keep the list and 3 make the order.
+//   the launches    6 x 64 x 600 x 16 float32 (15 MB): 10.5, 5.5 and 8.6 us; 1 x 300 x 8: 4.5, 4.0 and 2.8.
 #include <algorithm>
 #include <climits>
 
@@ -196,7 +205,11 @@ __device__ __forceinline__ void in_order(dm::RawRow<NQ, false> &raw, int dtype, 
 // list, and the last one taken, T, is the row's k-th largest: the experts with a logit of at least T are the chosen ones.
 // Where equal logits lie across the border, or T came out too low because equal heads went together, more than k are: those
 // rows are chosen again, one by one (float32 only, 16-bit logits are made unequal).  k rounds over all logits, each a
-// comparison, a selection and a maximum, take 2.5 k instructions per logit instead of k.
+// comparison, a selection and a maximum, take 2.5 k instructions per logit instead of k: with the finish 6 x 256 x 900 x 64
+// float32 take 123 us for the top 16 from lists and 320 for the top 17 in rounds (top 2, 4, 8: 72, 78, 92).
+//
+// The next row is asked for before this one is worked on, and no branch lies between its loads: one row in flight is what a
+// lane has registers for (two were slower), and with three workgroups per CU that keeps the memory busy.
 template <int NQ, int L, int K, bool WIDE, bool COUNT_ONLY>
 __global__ __launch_bounds__(RT_THREADS) void router_forward_kernel(const RouterSets a, const int dtype, const int sigmoid,
                                                                     unsigned *__restrict__ slots, int32_t *__restrict__ status)
@@ -410,6 +423,7 @@ __global__ __launch_bounds__(RT_THREADS) void router_forward_kernel(const Router
 
 // The slots of a group's workgroups added in index order: `cols` experts at a time (a power of two, 64 at most), a thread per
 // expert and every FINISH_THREADS / cols-th slot, their sums joined in order.  Then the loss of the sums.
+// Bound by the latency of its loads: 5 us for 125 slots of 64 experts in each of six groups, 7 to 9 for 768 slots of one.
 //   SUMS and LOSS   a workgroup per group does both
 //   SUMS alone      gridDim.y workgroups per group, each its share of the experts; the sums go to counts and means
 //   LOSS alone      a workgroup per group, from counts and means
@@ -547,6 +561,9 @@ __global__ __launch_bounds__(FINISH_THREADS) void router_finish_kernel(const Rou
     }
 }
 
+// The logits once more, their scores and their share in the gradient, a row per group of lanes as above: the row's dot product
+// with f needs all of its scores, and reading 4 bytes again costs less than 4 bytes kept in between and read.  Memory bound
+// from float32 logits (5.8 TB/s read and written in a step of 354 MB of logits, 4.8 when it is repeated by itself over 708 MB).
 template <int NQ, int L, bool WIDE>
 __global__ __launch_bounds__(RT_THREADS) void router_backward_kernel(const RouterSets a, const int dtype, const int sigmoid,
                                                                      const float *__restrict__ slope,

@@ -18,6 +18,15 @@
 // e = -128 marks a block with a NaN (cross entropy: a row whose softmax is NaN); its gradient is NaN.
 //
 // The gradient is that of the loss at the decoded logits; the loss itself is of the logits as they came.
+//
+// Measured (a copy of a GiB runs at 5.1 TB/s, a kernel of a few workgroups takes 4 us among others), forward and backward:
+//   focal           256 x 900 x 91 float32 (84 MB of logits, 21 of bytes): 26.8 and 26.4 us, 4 TB/s, bound by the instructions
+//                   of an exponential, a logarithm and a reciprocal per logit; 4 x 300 x 1203 bfloat16: 7.6 and 6.1;
+//                   64 x 600 x 2 float32: 4.6 and 4.3
+//   cross entropy   256 x 900 x 92 float32 (85 MB, 21 MB): 22.4 and 18.7 us, 4.7 and 5.7 TB/s, at the rate of a copy;
+//                   16 x 301 x 1205 float16 (12 MB, 6 MB): 10.9 and 8.4
+// The sums of the workgroups' partial sums take 2 to 4 us more.  The host's part of a call and its backward pass, about 45 us,
+// most of it the autograd engine's, covers all of these.
 #include <algorithm>
 #include <climits>
 
@@ -171,7 +180,8 @@ struct BlockRows {
     }
 };
 
-// Loss, bytes and heads.  codes NULL: the loss alone.
+// Loss, bytes and heads.  codes NULL: the loss alone.  One exponential per logit serves the softplus, the sigmoid and its
+// power; the block's step is found from its extremes (8 lanes, three exchanges) while the logits are still in registers.
 template <typename T, bool GAMMA2, bool ONE_CLASS>
 __global__ __launch_bounds__(CLS_THREADS) void focal_saved_kernel(const T *__restrict__ x, const int64_t *__restrict__ cls,
                                                                   const unsigned n, const unsigned C, const unsigned rows,
@@ -294,6 +304,7 @@ __global__ __launch_bounds__(CLS_THREADS) void focal_saved_kernel(const T *__res
     if (threadIdx.x == 0) partials[blockIdx.x] = total;
 }
 
+// The gradient of the logits that the bytes stand for, with the same exponential, logarithm and reciprocal per logit.
 template <typename T, bool GAMMA2, bool ONE_CLASS>
 __global__ __launch_bounds__(CLS_THREADS) void focal_from_saved_kernel(const unsigned *__restrict__ codes,
                                                                        const int32_t *__restrict__ heads,
@@ -458,6 +469,8 @@ __global__ __launch_bounds__(CLS_THREADS) void ce_saved_kernel(const void *__res
     }
 }
 
+// softmax of the decoded row less its own class, times weight and scale: the row's largest decodes to 0, so there is no maximum
+// to find, and a byte's exponential is one product and one instruction.
 template <int NQ, int L, bool WIDE>
 __global__ __launch_bounds__(CLS_THREADS) void ce_from_saved_kernel(const uint8_t *__restrict__ codes, const int8_t *__restrict__ steps,
                                                                     const int64_t *__restrict__ cls, const float *__restrict__ weight,
@@ -524,7 +537,8 @@ __global__ __launch_bounds__(CLS_THREADS) void ce_from_saved_kernel(const uint8_
 }
 
 // Rows too long for a wavefront's registers: a workgroup per row, which it walks twice (forward: largest, smallest and sum
-// of exponentials in one pass, the bytes in the second, out of the cache; backward: the sum, then the gradient).
+// of exponentials in one pass, the bytes in the second, out of the cache; backward: the sum, then the gradient).  354 MB of float32
+// logits of 4096 classes take 136 and 161 us, of 2048 classes in registers 95 and 89.
 constexpr int WIDE_WAVES = CLS_THREADS / 64;
 
 struct RowStats {
