@@ -267,8 +267,9 @@ __global__ __launch_bounds__(RT_THREADS) void router_forward_kernel(const Router
 #pragma unroll
         for (int j = 0; j < N; ++j) {
 #pragma unroll
-            for (int i = PLACES - 1; i >= 1; --i) list[i] = dm::median(list[i - 1], list[i], y[j]);
-            list[0] = dm::median(list[0], y[j], O::above_all());
+            for (int i = PLACES - 1; i >= 1; --i)
+                if (i <= j) list[i] = dm::median(list[i - 1], list[i], y[j]);      // (place j is empty before the j-th)
+            list[0] = j ? dm::median(list[0], y[j], O::above_all()) : y[0];
         }
         const typename O::Type top = dm::largest<L>(list[0]);
         if (COUNT_ONLY || !set.experts) {
