@@ -198,15 +198,15 @@ __device__ __forceinline__ void in_order(dm::RawRow<NQ, false> &raw, int dtype, 
     }
 }
 
-// K: the longest list of largest logits that a lane keeps (k <= K), or 0: k of any size, in rounds over all logits.
+// K: the longest list of largest logits that a lane keeps, k at most; 16: any k (a lane has no more logits than that).
 //
 // The choice.  A lane inserts its logits into a sorted list of its K largest, one instruction per place (the new place i is
 // the median of the old i - 1, the old i and the logit); then k times the largest head of the row's lanes is taken off its
 // list, and the last one taken, T, is the row's k-th largest: the experts with a logit of at least T are the chosen ones.
 // Where equal logits lie across the border, or T came out too low because equal heads went together, more than k are: those
-// rows are chosen again, one by one (float32 only, 16-bit logits are made unequal).  k rounds over all logits, each a
-// comparison, a selection and a maximum, take 2.5 k instructions per logit instead of k: with the finish 6 x 256 x 900 x 64
-// float32 take 123 us for the top 16 from lists and 320 for the top 17 in rounds (top 2, 4, 8: 72, 78, 92).
+// rows are chosen again, one by one (float32 only, 16-bit logits are made unequal): k rounds over all logits, each a maximum, a
+// search for its lowest place and a selection.  With lists 6 x 256 x 900 x 64 float32 take, sums and loss among them, 73, 78, 90 and
+// 125 us for the top 2, 4, 8 and 16 and 148 for the top 17; with such rounds for every row the top 17 took 320.
 //
 // The next row is asked for before this one is worked on, and no branch lies between its loads: one row in flight is what a
 // lane has registers for (two were slower), and with three workgroups per CU that keeps the memory busy.
@@ -260,7 +260,7 @@ __global__ __launch_bounds__(RT_THREADS) void router_forward_kernel(const Router
         typename O::Type y[N];
         bool nan;
         in_order<NQ, L>(raw, dtype, sub, E, counts, y, &nan);
-        constexpr int PLACES = K ? K : 1;
+        constexpr int PLACES = K < N ? K : N;
         typename O::Type list[PLACES];
 #pragma unroll
         for (int i = 0; i < PLACES; ++i) list[i] = O::never();
@@ -273,44 +273,41 @@ __global__ __launch_bounds__(RT_THREADS) void router_forward_kernel(const Router
         }
         const typename O::Type top = dm::largest<L>(list[0]);
         if (COUNT_ONLY || !set.experts) {
-            bool again = K == 0;
-            if (K) {
-                typename O::Type last = O::never();
-                if (L == 1) {
+            typename O::Type last = O::never();
+            if (L == 1) {
 #pragma unroll
-                    for (int i = 0; i < PLACES; ++i) last = i + 1 == (int)k ? list[i] : last;
+                for (int i = 0; i < PLACES; ++i) last = i + 1 == (int)k ? list[i] : last;
+            } else {
+                last = top;
+                // the heads that equal `last` off their lists, as far as `places`, and the largest head that is left (the median of a
+                // place, the next and the least is the next, of the largest the place itself)
+                auto next_largest = [&](int places) {
+                    const typename O::Type gone = list[0] == last ? O::never() : O::above_all();
+#pragma unroll
+                    for (int j = 0; j < PLACES; ++j)
+                        if (j < places) list[j] = dm::median(list[j], j + 1 < PLACES ? list[j + 1] : O::never(), gone);
+                    last = dm::largest<L>(list[0]);
+                };
+                if (K == 16 && k > 16) {
+                    for (unsigned i = 1; i < k; ++i) next_largest(PLACES);
                 } else {
-                    last = top;
 #pragma unroll
-                    for (int i = 1; i < PLACES; ++i) {
-                        if (i < (int)k) {
-                            // (the median of a place, the next and the least is the next, of the largest the place itself; what
-                            // could come up after the k-th is not moved any more)
-                            const typename O::Type gone = list[0] == last ? O::never() : O::above_all();
-#pragma unroll
-                            for (int j = 0; j + i < PLACES; ++j) list[j] = dm::median(list[j], list[j + 1], gone);
-                            last = dm::largest<L>(list[0]);
-                        }
-                    }
-                }
-                last = max(last, O::least(dtype));             // (fewer than k: all that can be)
-                unsigned chosen = 0;
-#pragma unroll
-                for (int j = 0; j < N; ++j) {
-                    const unsigned one = y[j] >= last ? 1u : 0u;
-                    cnt[j] += one;
-                    if (WIDE) chosen += one;
-                }
-                if (WIDE) {
-                    chosen = dm::over_group<L>(chosen, dm::Add());
-                    again = __any(chosen > k);
-                    if (again) {
-#pragma unroll
-                        for (int j = 0; j < N; ++j) cnt[j] -= y[j] >= last ? 1u : 0u;
-                    }
+                    for (int i = 1; i < K; ++i)
+                        if (i < (int)k) next_largest(K - i);       // (what could come up after the k-th is not moved any more)
                 }
             }
-            if (again) {
+            last = max(last, O::least(dtype));                 // (fewer than k: all that can be)
+            unsigned chosen = 0;
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const unsigned one = y[j] >= last ? 1u : 0u;
+                cnt[j] += one;
+                if (WIDE) chosen += one;
+            }
+            if (WIDE) chosen = dm::over_group<L>(chosen, dm::Add());
+            if (WIDE && __any(chosen > k)) {
+#pragma unroll
+                for (int j = 0; j < N; ++j) cnt[j] -= y[j] >= last ? 1u : 0u;
                 // k times the largest that is left, of the lowest expert that has it
                 typename O::Type left[N];
 #pragma unroll
@@ -785,8 +782,7 @@ ForwardKernel forward_with(unsigned k, bool wide, bool count_only)
     if (k <= 2) return forward_of<NQ, L, 2>(wide, count_only);
     if (k <= 4) return forward_of<NQ, L, 4>(wide, count_only);
     if (k <= 8) return forward_of<NQ, L, 8>(wide, count_only);
-    if (k <= 16) return forward_of<NQ, L, 16>(wide, count_only);
-    return forward_of<NQ, L, 0>(wide, count_only);
+    return forward_of<NQ, L, 16>(wide, count_only);
 }
 ForwardKernel forward_for(unsigned E, unsigned k, bool wide, bool count_only)
 {

@@ -106,6 +106,17 @@ def test_every_number_of_choices(k, dtype):
     run_and_check([make((3, 11, 40), dtype, k)], k)
 
 
+@pytest.mark.parametrize("E,k", [(20, 17), (24, 24), (33, 9), (90, 15), (96, 96), (100, 17), (256, 16), (256, 20), (300, 64), (1000, 31), (1024, 1024)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_many_choices(E, k, dtype):
+    x = make((2, 23, E), dtype, E + k)
+    run_and_check([x], k)
+    x[:, ::2] = (x[:, ::2].float() * 4).round().div(4).to(x.dtype)          # (equal ones, across lanes and in one lane's share)
+    x[:, 5, ::2] = -float("inf")
+    x[0, 7] = x[0, 7, 0]
+    run_and_check([x], k)
+
+
 @pytest.mark.parametrize("S,B,Q,E,k", [(1, 1, 1, 8, 2), (1, 1, 2000, 8, 1), (6, 4, 150, 16, 2), (2, 7, 301, 24, 3), (18, 2, 9, 6, 2),
                                        (1, 300, 3, 10, 2), (3, 33, 65, 64, 4)])
 @pytest.mark.parametrize("per_image", [False, True])
