@@ -373,6 +373,19 @@ __device__ __forceinline__ float row_weight(int64_t y, unsigned C, int64_t ignor
     return weight ? weight[y] : 1.0f;
 }
 
+// The bytes of the classes c .. c + 3 of a row of C, at any alignment.
+__device__ __forceinline__ void store_codes(uint8_t *row, unsigned c, unsigned C, unsigned packed)
+{
+    typedef unsigned Word __attribute__((aligned(1)));
+    if (c + 4 <= C) {
+        *reinterpret_cast<Word *>(row + c) = packed;
+    } else {
+#pragma unroll
+        for (unsigned k = 0; k < 3; ++k)
+            if (c + k < C) row[c + k] = (uint8_t)(packed >> (8 * k));
+    }
+}
+
 // L lanes share a row and keep it in registers, NQ quads of four logits each; the next row is asked for before this one is
 // worked on.
 template <int NQ, int L, bool WIDE>
@@ -449,14 +462,7 @@ __global__ __launch_bounds__(CLS_THREADS) void ce_saved_kernel(const void *__res
             for (int k = 0; k < 4; ++k)
                 packed = pack_code(packed, k, __builtin_amdgcn_fmed3f(top - __builtin_rintf(v[4 * q + k] * inverse), 0.0f, 255.0f));
             const unsigned c = 4 * (q * L + sub);
-            if (live && c + 4 <= C) {
-                typedef unsigned Word __attribute__((aligned(1)));
-                *reinterpret_cast<Word *>(out + c) = packed;
-            } else if (live) {
-#pragma unroll
-                for (unsigned k = 0; k < 3; ++k)
-                    if (c + k < C) out[c + k] = (uint8_t)(packed >> (8 * k));
-            }
+            if (live) store_codes(out, c, C, packed);
         }
         if (sub == 0 && live) steps[row] = (int8_t)(sum == sum ? e : NOT_A_NUMBER);
     }
@@ -613,10 +619,13 @@ __global__ __launch_bounds__(CLS_THREADS) void ce_saved_wide_kernel(const T *__r
         for (unsigned c = 4 * threadIdx.x; c < C; c += 4 * CLS_THREADS) {
             float t[4];
             dm::load_quad(lg, c, C, -inf, t);
+            unsigned packed = 0;
+#pragma unroll
             for (unsigned k = 0; k < 4; ++k) {
-                const float z = fminf(fmaxf(t[k], -CE_CLAMP), CE_CLAMP);
-                if (c + k < C) out[c + k] = (uint8_t)(unsigned)fminf(top - __builtin_rintf(z * inverse), 255.0f);
+                const float z = __builtin_amdgcn_fmed3f(t[k], -CE_CLAMP, CE_CLAMP);
+                packed = pack_code(packed, k, __builtin_amdgcn_fmed3f(top - __builtin_rintf(z * inverse), 0.0f, 255.0f));
             }
+            store_codes(out, c, C, packed);
         }
         if (threadIdx.x == 0) steps[row] = (int8_t)(sum == sum ? e : NOT_A_NUMBER);
     }
