@@ -86,16 +86,6 @@ __device__ __forceinline__ FocalParts focal_parts(float z, float gamma)
     return f;
 }
 
-// A row's class as the focal loss needs it, 64 bits looked at once: the place of its positive logit counted from the row's
-// first, or none; and whether the row may not count (ignored, or a class that is none), which `row_code` then settles.
-__device__ __forceinline__ bool class_place(int64_t label, unsigned C, const FocalParams &fp, int *place)
-{
-    const unsigned low = (unsigned)label;
-    const bool small = (unsigned)((uint64_t)label >> 32) == 0;
-    *place = small && low < C ? (int)low : INT_MIN / 2;
-    return !(small && low <= C) || (fp.use_ignore && label == fp.ignore_index);
-}
-
 // The focal kernels' share of the flat array: 8 lanes take a block of 128 logits, each four quads of four consecutive ones,
 // 32 logits apart (a load of the 8 lanes is 128 bytes of float32).  With four logits per lane, and 32 lanes to agree on a
 // block's step, the agreement cost as much as half of the loss itself.
@@ -149,15 +139,24 @@ struct BlockRows {
     }
     __device__ __forceinline__ void settle(unsigned C, const FocalParams &fp)
     {
-        skipped = false;
+        unsigned largest = 0, high = 0;
 #pragma unroll
         for (unsigned q = 0; q < QUADS; ++q)
 #pragma unroll
             for (unsigned k = 0; k < ROWS; ++k) {
-                int place;
-                skipped |= class_place(label[q][k], C, fp, &place);
-                hot[q][k] = place + (ONE_CLASS ? (int)k : k ? (int)(C - col[q]) : -(int)col[q]);
+                const unsigned low = (unsigned)label[q][k];
+                high |= (unsigned)((uint64_t)label[q][k] >> 32);
+                largest = max(largest, low);
+                // (a class that is none is nowhere: its row's neighbours in the quad are others')
+                hot[q][k] = (low < C ? (int)low : INT_MIN / 2) + (ONE_CLASS ? (int)k : k ? (int)(C - col[q]) : -(int)col[q]);
             }
+        skipped = high != 0 || largest > C;
+        if (fp.use_ignore && (uint64_t)fp.ignore_index <= C) {
+#pragma unroll
+            for (unsigned q = 0; q < QUADS; ++q)
+#pragma unroll
+                for (unsigned k = 0; k < ROWS; ++k) skipped |= (unsigned)label[q][k] == (unsigned)fp.ignore_index;
+        }
     }
     __device__ __forceinline__ bool positive(unsigned q, unsigned k) const
     {
