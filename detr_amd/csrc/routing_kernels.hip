@@ -15,9 +15,9 @@
 //   memory          6 x 256 x 900 x 64 float32, top 4 (354 MB): forward 107 us, sums and loss 5 each, backward 123 (708 MB at
 //                   5.8 TB/s).  Forward, sums and loss by themselves, over and over, take 75 (4.7 TB/s); in a step they wait for the
 //                   gradients of the one before, of which the caches hold up to 256 MB, to be written.
-//   instructions    16-bit logits with many choices: 2 x 64 x 1050 x 160 bfloat16, sigmoid scores, top 8 (43 MB): forward 36 us,
-//                   sums and loss 7, backward 27; counts alone of 256 x 900 x 256, top 8 (118 MB): 45 us, the vector units
-//                   busy 81 % of it, 22 instructions per logit of which 8 keep the list and 3 make the order.
+//   instructions    16-bit logits with many choices: 2 x 64 x 1050 x 160 bfloat16, sigmoid scores, top 8 (43 MB): forward 35 us,
+//                   sums and loss 7, backward 27; counts alone of 256 x 900 x 256, top 8 (118 MB): 44 us, the vector units
+//                   busy four fifths of it, 20 instructions per logit of which 6 keep the list and 3 make the order.
 //   the launches    6 x 64 x 600 x 16 float32 (15 MB): 10.5, 5.5 and 8.6 us; 1 x 300 x 8: 4.5, 4.0 and 2.8.
 #include <algorithm>
 #include <climits>

@@ -20,8 +20,8 @@
 // The gradient is that of the loss at the decoded logits; the loss itself is of the logits as they came.
 //
 // Measured (a copy of a GiB runs at 5.1 TB/s, a kernel of a few workgroups takes 4 us among others), forward and backward:
-//   focal           256 x 900 x 91 float32 (84 MB of logits, 21 of bytes): 26.8 and 26.4 us, 4 TB/s, bound by the instructions
-//                   of an exponential, a logarithm and a reciprocal per logit; 4 x 300 x 1203 bfloat16: 7.6 and 6.1;
+//   focal           256 x 900 x 91 float32 (84 MB of logits, 21 of bytes): 27 and 25 us, 4 TB/s, bound by the 50 to 60
+//                   instructions per logit, an exponential, a logarithm and a reciprocal among them; 4 x 300 x 1203 bfloat16: 7.6 and 6.1;
 //                   64 x 600 x 2 float32: 4.6 and 4.3
 //   cross entropy   256 x 900 x 92 float32 (85 MB, 21 MB): 22.4 and 18.7 us, 4.7 and 5.7 TB/s, at the rate of a copy;
 //                   16 x 301 x 1205 float16 (12 MB, 6 MB): 10.9 and 8.4
@@ -543,7 +543,7 @@ __global__ __launch_bounds__(CLS_THREADS) void ce_from_saved_kernel(const uint8_
 
 // Rows too long for a wavefront's registers: a workgroup per row, which it walks twice (forward: largest, smallest and sum
 // of exponentials in one pass, the bytes in the second, out of the cache; backward: the sum, then the gradient).  354 MB of float32
-// logits of 4096 classes take 136 and 161 us, of 2048 classes in registers 95 and 89.
+// logits of 4096 classes take 127 and 161 us, of 2048 classes in registers 95 and 89.
 constexpr int WIDE_WAVES = CLS_THREADS / 64;
 
 struct RowStats {
