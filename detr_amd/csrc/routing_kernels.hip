@@ -9,7 +9,7 @@
 //
 // Forward: workgroups walk chunks of an image's rows, a group of lanes per row; sums over rows stay in registers of the
 // lane that owns the expert, and leave once per workgroup, into a slot of the workspace.  A second kernel adds the slots in
-// index order in 64 bits: no float atomics, the same bits every run.
+// index order in 64 bits: no float atomics, the same bits every run.  A group that one workgroup walks needs no second kernel.
 //
 // What bounds it, as measured (a copy of a GiB runs at 5.1 TB/s, a kernel of a few workgroups takes 4 us among others):
 //   memory          6 x 256 x 900 x 64 float32, top 4 (354 MB): forward 107 us, sums and loss 5 each, backward 123 (708 MB at
@@ -18,7 +18,8 @@
 //   instructions    16-bit logits with many choices: 2 x 64 x 1050 x 160 bfloat16, sigmoid scores, top 8 (43 MB): forward 35 us,
 //                   sums and loss 7, backward 27; counts alone of 256 x 900 x 256, top 8 (118 MB): 44 us, the vector units
 //                   busy four fifths of it, 20 instructions per logit of which 6 keep the list and 3 make the order.
-//   the launches    6 x 64 x 600 x 16 float32 (15 MB): 10.5, 5.5 and 8.6 us; 1 x 300 x 8: 4.5, 4.0 and 2.8.
+//   the launches    6 x 64 x 600 x 16 float32 (15 MB): 10.5, 5.5 and 8.6 us; 1 x 300 x 8, where one workgroup makes the loss as well:
+//                   6.0 and 2.8.
 #include <algorithm>
 #include <climits>
 
@@ -198,6 +199,70 @@ __device__ __forceinline__ void in_order(dm::RawRow<NQ, false> &raw, int dtype, 
     }
 }
 
+// What a group's loss is made of, and where it goes.
+struct Results {
+    const int64_t *given_counts;
+    float *balance, *z;
+    int64_t *counts;
+    float *slope, *inv_rows;
+};
+constexpr int LOSS_THREADS = 256, LOSS_WAVES = LOSS_THREADS / 64, LOSS_EACH = RT_MAX_EXPERTS / LOSS_THREADS;
+struct LossSums {
+    unsigned long long rows[LOSS_WAVES], total[LOSS_WAVES];
+    double z[LOSS_WAVES], dot[LOSS_WAVES];
+};
+
+// The loss of a group, and what its gradient needs, by LOSS_THREADS threads.  A thread brings the counts and the sums of p of its
+// experts tid, tid + LOSS_THREADS, ..., and its share of the rows that count and of the sum of lse^2.
+__device__ __forceinline__ void group_loss(const Results &out, const unsigned E, const size_t group, const long long (&counts)[LOSS_EACH],
+                                           const double (&sums)[LOSS_EACH], unsigned long long rows, double zs, LossSums &lds)
+{
+    const unsigned tid = threadIdx.x;
+    double dot = 0.0;
+    unsigned long long total = 0;
+#pragma unroll
+    for (int j = 0; j < LOSS_EACH; ++j) {                      // (0 behind the last expert)
+        dot += (double)counts[j] * sums[j];
+        total += (unsigned long long)counts[j];
+    }
+    // over the wave, then over the waves, in every thread
+    rows = dm::over_group<64>(rows, dm::Add());
+    total = dm::over_group<64>(total, dm::Add());
+    zs = dm::over_group<64>(zs, dm::Add());
+    dot = dm::over_group<64>(dot, dm::Add());
+    if ((tid & 63) == 0) {
+        lds.rows[tid >> 6] = rows;
+        lds.total[tid >> 6] = total;
+        lds.z[tid >> 6] = zs;
+        lds.dot[tid >> 6] = dot;
+    }
+    __syncthreads();
+    rows = lds.rows[0];
+    total = lds.total[0];
+    zs = lds.z[0];
+    dot = lds.dot[0];
+#pragma unroll
+    for (int w = 1; w < LOSS_WAVES; ++w) {
+        rows += lds.rows[w];
+        total += lds.total[w];
+        zs += lds.z[w];
+        dot += lds.dot[w];
+    }
+    const long long all = (long long)total;
+    const double inv_n = rows ? 1.0 / (double)rows : 0.0;
+    const double per_count = all > 0 ? (double)E / (double)all : 0.0;
+    if (tid == 0) {
+        out.balance[group] = (float)(dot * per_count * inv_n);
+        if (out.z) out.z[group] = (float)(zs * inv_n);
+        out.inv_rows[group] = (float)inv_n;
+    }
+#pragma unroll
+    for (int j = 0; j < LOSS_EACH; ++j) {
+        const unsigned e = tid + j * LOSS_THREADS;
+        if (e < E) out.slope[group * E + e] = all > 0 ? (float)((double)counts[j] * per_count - 1.0) : 0.0f;
+    }
+}
+
 // K: the longest list of largest logits that a lane keeps, k at most; 16: any k (a lane has no more logits than that).
 //
 // The choice.  A lane inserts its logits into a sorted list of its K largest, one instruction per place (the new place i is
@@ -210,9 +275,12 @@ __device__ __forceinline__ void in_order(dm::RawRow<NQ, false> &raw, int dtype, 
 //
 // The next row is asked for before this one is worked on, and no branch lies between its loads: one row in flight is what a
 // lane has registers for (two were slower), and with three workgroups per CU that keeps the memory busy.
+//
+// whole: every group has one workgroup, which makes the group's loss itself instead of leaving its sums.
 template <int NQ, int L, int K, bool WIDE, bool COUNT_ONLY>
 __global__ __launch_bounds__(RT_THREADS) void router_forward_kernel(const RouterSets a, const int dtype, const int sigmoid,
-                                                                    unsigned *__restrict__ slots, int32_t *__restrict__ status)
+                                                                    const int whole, unsigned *__restrict__ slots,
+                                                                    const Results out, int32_t *__restrict__ status)
 {
     constexpr int N = 4 * NQ;                                  // logits of a row per lane
     constexpr int PARTS = L <= 16 ? 4 : 64 / L;                // partial sums of p that a wave leaves
@@ -221,6 +289,7 @@ __global__ __launch_bounds__(RT_THREADS) void router_forward_kernel(const Router
     __shared__ float psum_lds[COUNT_ONLY ? 1 : RT_WAVES * PARTS][COUNT_ONLY ? 1 : WIDTH];
     __shared__ double z_lds[RT_WAVES];
     __shared__ unsigned n_lds[RT_WAVES];
+    __shared__ LossSums loss_lds;
     const unsigned E = a.E, k = a.k;
     const float ninf = -__builtin_huge_valf();
     for (unsigned e = threadIdx.x; e < WIDTH; e += RT_THREADS) hist[e] = 0;
@@ -397,6 +466,34 @@ __global__ __launch_bounds__(RT_THREADS) void router_forward_kernel(const Router
         }
     }
     __syncthreads();
+    if (whole) {
+        static_assert(RT_THREADS == LOSS_THREADS, "");
+        const size_t group = a.first_group[at.set] + (a.per_image ? at.image : 0);
+        long long counts[LOSS_EACH];
+        double sums[LOSS_EACH];
+#pragma unroll
+        for (int j = 0; j < LOSS_EACH; ++j) {
+            const unsigned e = threadIdx.x + j * RT_THREADS;
+            counts[j] = 0;
+            sums[j] = 0.0;
+            if (e < E) {
+                counts[j] = (long long)hist[e];
+                out.counts[group * E + e] = counts[j];
+                if (!COUNT_ONLY) {
+                    float s = psum_lds[0][e];
+#pragma unroll
+                    for (int w = 1; w < RT_WAVES * PARTS; ++w) s += psum_lds[w][e];
+                    sums[j] = (double)s;
+                    if (out.given_counts) counts[j] = out.given_counts[group * E + e];
+                }
+            }
+        }
+        if (!COUNT_ONLY) {
+            const bool brings = threadIdx.x < RT_WAVES;
+            group_loss(out, E, group, counts, sums, brings ? n_lds[threadIdx.x] : 0, brings ? z_lds[threadIdx.x] : 0.0, loss_lds);
+        }
+        return;
+    }
     unsigned *slot = slots + (size_t)blockIdx.x * slot_words(E);
     for (unsigned e = threadIdx.x; e < E; e += RT_THREADS) {
         if (!COUNT_ONLY) {
@@ -427,19 +524,17 @@ __global__ __launch_bounds__(RT_THREADS) void router_forward_kernel(const Router
 //   LOSS alone      a workgroup per group, from counts and means
 // Two launches are taken for few groups of many experts, where one workgroup would read a megabyte of slots by itself.  (One
 // launch in which the last of a group's workgroups makes the loss is slower: the fences it needs write the caches back.)
-constexpr int FINISH_THREADS = 1024, FINISH_WAVES = FINISH_THREADS / 64, LOSS_THREADS = 256;
+constexpr int FINISH_THREADS = 1024, FINISH_WAVES = FINISH_THREADS / 64;
 
 template <bool SUMS, bool LOSS>
 __global__ __launch_bounds__(FINISH_THREADS) void router_finish_kernel(const RouterSets a, const unsigned *__restrict__ slots,
-                                                                       const unsigned cols, const int64_t *__restrict__ given_counts,
-                                                                       double *__restrict__ means, float *__restrict__ balance,
-                                                                       float *__restrict__ z, int64_t *__restrict__ counts,
-                                                                       float *__restrict__ slope, float *__restrict__ inv_rows)
+                                                                       const unsigned cols, double *__restrict__ means, const Results out)
 {
     __shared__ double p_lds[FINISH_WAVES][64];
     __shared__ unsigned long long c_lds[FINISH_WAVES][64];
     __shared__ double P[RT_MAX_EXPERTS];
     __shared__ long long C[RT_MAX_EXPERTS];
+    __shared__ LossSums loss_lds;
     const unsigned E = a.E, words = slot_words(E), tid = threadIdx.x, group = blockIdx.x;
     int set = 0;
     while (set + 1 < a.S && group >= a.first_group[set + 1]) ++set;
@@ -487,7 +582,7 @@ __global__ __launch_bounds__(FINISH_THREADS) void router_finish_kernel(const Rou
                     p += p_lds[i][col];
                     c += c_lds[i][col];
                 }
-                counts[(size_t)group * E + e] = (int64_t)c;
+                out.counts[(size_t)group * E + e] = (int64_t)c;
                 if (LOSS) {
                     P[e] = p;
                     C[e] = (long long)c;
@@ -499,64 +594,28 @@ __global__ __launch_bounds__(FINISH_THREADS) void router_finish_kernel(const Rou
         }
     }
     if (!LOSS || tid >= LOSS_THREADS) return;
-    // the rows that count and the sum of lse^2; the counts and sum_e c_e P_e
-    constexpr int EACH = RT_MAX_EXPERTS / LOSS_THREADS;
-    const int64_t *shares = given_counts ? given_counts : SUMS ? nullptr : counts;
-    long long mine[EACH];
-    double zs = 0.0, dot = 0.0;
-    unsigned long long rows = 0, total = 0;
+    const int64_t *given = out.given_counts ? out.given_counts : SUMS ? nullptr : out.counts;
+    long long counts[LOSS_EACH];
+    double sums[LOSS_EACH];
 #pragma unroll
-    for (int j = 0; j < EACH; ++j) {
+    for (int j = 0; j < LOSS_EACH; ++j) {
         const unsigned e = tid + j * LOSS_THREADS;
-        mine[j] = 0;
+        counts[j] = 0;
+        sums[j] = 0.0;
         if (e < E) {
-            mine[j] = shares ? shares[(size_t)group * E + e] : C[e];
-            dot += (double)mine[j] * (SUMS ? P[e] : means[(size_t)group * E + e]);
-            total += (unsigned long long)mine[j];
+            counts[j] = given ? given[(size_t)group * E + e] : C[e];
+            sums[j] = SUMS ? P[e] : means[(size_t)group * E + e];
         }
     }
+    double zs = 0.0;
+    unsigned long long rows = 0;
 #pragma unroll 4
     for (unsigned i = tid; i < slots_of_group; i += LOSS_THREADS) {
         const unsigned *slot = first + (size_t)i * words;
         zs += *reinterpret_cast<const double *>(slot + 2 * E);
         rows += slot[2 * E + 2];
     }
-    // over the wave, then over the waves, in every thread
-    rows = dm::over_group<64>(rows, dm::Add());
-    total = dm::over_group<64>(total, dm::Add());
-    zs = dm::over_group<64>(zs, dm::Add());
-    dot = dm::over_group<64>(dot, dm::Add());
-    if ((tid & 63) == 0) {
-        c_lds[tid >> 6][0] = rows;
-        c_lds[tid >> 6][1] = total;
-        p_lds[tid >> 6][0] = zs;
-        p_lds[tid >> 6][1] = dot;
-    }
-    __syncthreads();
-    rows = c_lds[0][0];
-    total = c_lds[0][1];
-    zs = p_lds[0][0];
-    dot = p_lds[0][1];
-#pragma unroll
-    for (int w = 1; w < LOSS_THREADS / 64; ++w) {
-        rows += c_lds[w][0];
-        total += c_lds[w][1];
-        zs += p_lds[w][0];
-        dot += p_lds[w][1];
-    }
-    const long long all = (long long)total;
-    const double inv_n = rows ? 1.0 / (double)rows : 0.0;
-    const double per_count = all > 0 ? (double)E / (double)all : 0.0;
-    if (tid == 0) {
-        balance[group] = (float)(dot * per_count * inv_n);
-        if (z) z[group] = (float)(zs * inv_n);
-        inv_rows[group] = (float)inv_n;
-    }
-#pragma unroll
-    for (int j = 0; j < EACH; ++j) {
-        const unsigned e = tid + j * LOSS_THREADS;
-        if (e < E) slope[(size_t)group * E + e] = all > 0 ? (float)((double)mine[j] * per_count - 1.0) : 0.0f;
-    }
+    group_loss(out, E, group, counts, sums, rows, zs, loss_lds);
 }
 
 // The logits once more, their scores and their share in the gradient, a row per group of lanes as above: the row's dot product
@@ -709,9 +768,22 @@ Form backward_form(unsigned E, bool wide)
 // for 16 bits: no faster, and two thirds more slots to add.)
 struct Pass {
     int resident, lanes;         // workgroups, lanes per row
+    bool whole;                  // one workgroup per group
 };
-Pass forward_pass(const Shape &sh) { return {3 * 256, forward_form((unsigned)sh.E).L}; }
-Pass backward_pass(const Shape &sh, bool wide) { return {8 * 256, backward_form((unsigned)sh.E, wide).L}; }
+Pass forward_pass(const DmRouterSet *sets, const Shape &sh)
+{
+    // Groups of up to WHOLE_TRIPS trips by one workgroup each: no second launch, whose time a few trips one after the other cost
+    // less than.  Six sets of four trips: counts and forward pass of 8 experts 6.7 and 9.5 us among others instead of 8.8 and 11.6,
+    // of 64 6.7 and 10.1 instead of 9.9 and 12.6, of 256 (bfloat16, top 8) 7.9 and 10.8 instead of 11.6 and 15.1; of eight trips
+    // 7.6 and 11.3 instead of 8.8 and 11.6, but 9.7 and 14.9 instead of 9.8 and 12.6, and 12.1 and 16.9 instead of 11.9 and 15.5.
+    constexpr long long WHOLE_TRIPS = 4;
+    const int lanes = forward_form((unsigned)sh.E).L;
+    bool whole = sh.merged || sh.per_image;
+    for (int s = 0; s < sh.S && whole; ++s)
+        whole = (sh.merged ? (long long)sh.B * sets[s].Q : (long long)sets[s].Q) <= WHOLE_TRIPS * (RT_THREADS / lanes);
+    return {3 * 256, lanes, whole};
+}
+Pass backward_pass(const Shape &sh, bool wide) { return {8 * 256, backward_form((unsigned)sh.E, wide).L, false}; }
 struct Chunks {
     unsigned count, rows;
 };
@@ -722,7 +794,7 @@ Chunks chunks_of(const Shape &sh, int Q, const Pass &pass)
     const long long trip = RT_THREADS / pass.lanes;
     const long long trips = std::max(1ll, (rows + trip - 1) / trip);
     const long long want = std::max(1ll, pass.resident / std::max(1ll, std::min<long long>(sh.S, DM_MAX_SETS_PER_LAUNCH) * images));
-    const long long each = (trips + want - 1) / want;
+    const long long each = pass.whole ? trips : (trips + want - 1) / want;
     return Chunks{(unsigned)((trips + each - 1) / each), (unsigned)(each * trip)};
 }
 
@@ -767,7 +839,7 @@ unsigned long long most_blocks(const DmRouterSet *sets, const Shape &sh, const P
     return most;
 }
 
-typedef void (*ForwardKernel)(RouterSets, int, int, unsigned *, int32_t *);
+typedef void (*ForwardKernel)(RouterSets, int, int, int, unsigned *, Results, int32_t *);
 typedef void (*BackwardKernel)(RouterSets, int, int, const float *, const float *, const float *, const float *);
 
 template <int NQ, int L, int K>
@@ -826,7 +898,7 @@ struct Workspace {
 };
 Workspace workspace_of(const DmRouterSet *sets, const Shape &sh)
 {
-    return Workspace{most_blocks(sets, sh, forward_pass(sh)), (unsigned long long)std::min(sh.S, DM_MAX_SETS_PER_LAUNCH) * (sh.per_image ? (unsigned long long)sh.B : 1ull)};
+    return Workspace{most_blocks(sets, sh, forward_pass(sets, sh)), (unsigned long long)std::min(sh.S, DM_MAX_SETS_PER_LAUNCH) * (sh.per_image ? (unsigned long long)sh.B : 1ull)};
 }
 
 int forward(const DmRouterSet *sets, int S, int B, int E, int top_k, int dtype, int scores, int per_image,
@@ -853,27 +925,26 @@ int forward(const DmRouterSet *sets, int S, int B, int E, int top_k, int dtype, 
     const Workspace need = workspace_of(sets, sh);
     if (need.blocks > MOST_BLOCKS || need.groups > MOST_GROUPS) return DM_E_UNSUPPORTED;
     if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0 || workspace_bytes < need.bytes(E)) return DM_E_INVALID_ARG;
+    const Pass pass = forward_pass(sets, sh);
     unsigned *slots = static_cast<unsigned *>(workspace);
     double *means = reinterpret_cast<double *>(slots + (size_t)std::max(1ull, need.blocks) * slot_words((unsigned)E));
     for (int first = 0; first < S; first += DM_MAX_SETS_PER_LAUNCH) {
         RouterSets a;
         const int n = std::min(S - first, DM_MAX_SETS_PER_LAUNCH);
-        const unsigned blocks = (unsigned)describe(sets, first, n, sh, top_k, forward_pass(sh), &a);
-        if (blocks) {
-            hipLaunchKernelGGL(forward_for((unsigned)E, given == 1 ? 1u : (unsigned)top_k, dtype == DM_F32, balance == nullptr), dim3(blocks), dim3(RT_THREADS), 0,
-                               st, a, dtype, scores == DM_SCORES_SIGMOID ? 1 : 0, slots, status);
-            rc = dm::check_hip(hipGetLastError(), "router_forward_kernel launch");
-            if (rc != DM_OK) return rc;
-        }
+        const unsigned blocks = (unsigned)describe(sets, first, n, sh, top_k, pass, &a);
         const size_t g0 = (size_t)first * (per_image ? (size_t)B : 1);
         const unsigned gn = (unsigned)n * (per_image ? (unsigned)B : 1u);
+        const Results out{given_counts ? given_counts + g0 * E : nullptr, balance ? balance + g0 : nullptr, z ? z + g0 : nullptr,
+                          counts + g0 * E, slope ? slope + g0 * E : nullptr, inv_rows ? inv_rows + g0 : nullptr};
+        hipLaunchKernelGGL(forward_for((unsigned)E, given == 1 ? 1u : (unsigned)top_k, dtype == DM_F32, balance == nullptr), dim3(blocks),
+                           dim3(RT_THREADS), 0, st, a, dtype, scores == DM_SCORES_SIGMOID ? 1 : 0, pass.whole ? 1 : 0, slots, out, status);
+        rc = dm::check_hip(hipGetLastError(), "router_forward_kernel launch");
+        if (rc != DM_OK) return rc;
+        if (pass.whole) continue;
         unsigned cols = 1;
         while (cols < 64 && cols < (unsigned)E) cols <<= 1;
         auto finish = [&](auto kernel, unsigned parts, unsigned width, int threads) {
-            hipLaunchKernelGGL(kernel, dim3(gn, parts), dim3(threads), 0, st, a, slots, width,
-                               given_counts ? given_counts + g0 * E : nullptr, means, balance ? balance + g0 : nullptr,
-                               z ? z + g0 : nullptr, counts + g0 * E, slope ? slope + g0 * E : nullptr,
-                               inv_rows ? inv_rows + g0 : nullptr);
+            hipLaunchKernelGGL(kernel, dim3(gn, parts), dim3(threads), 0, st, a, slots, width, means, out);
         };
         // (one workgroup adds 720 slots of 64 experts in 20 us, four of 16 experts each in 4)
         const bool few = gn <= 64 && (unsigned long long)blocks * (unsigned)E > 4096ull * gn && E > 16;

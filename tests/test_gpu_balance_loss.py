@@ -100,6 +100,17 @@ def test_every_number_of_experts(E, dtype):
     run_and_check(xs, 1, scores="sigmoid", per_image=True)
 
 
+# (the same with rows for several workgroups per set, and per image)
+@pytest.mark.parametrize("E", [1, 2, 3, 4, 5, 7, 8, 9, 12, 13, 16, 17, 24, 31, 32, 33, 48, 49, 64, 65, 96, 97, 100, 128, 129, 160, 192, 193,
+                               255, 256, 257, 384, 385, 512, 513, 768, 769, 1000, 1023, 1024])
+@pytest.mark.parametrize("per_image", [False, True])
+def test_more_rows_than_one_workgroup_takes(E, per_image):
+    Q = 1300 * 16 // max(E, 16) + 3
+    xs = [make((2, q, E), "f32", 100 * E + q) for q in (Q, 7)]
+    run_and_check(xs, min(E, 2), per_image=per_image)
+    run_and_check([make((1, Q, E), "bf16", E)], min(E, 5), scores="sigmoid", per_image=per_image)
+
+
 @pytest.mark.parametrize("k", [1, 2, 4, 7, 8, 16, 33, 40])
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_every_number_of_choices(k, dtype):
