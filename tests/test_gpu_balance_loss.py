@@ -223,6 +223,30 @@ def test_given_experts(per_image):
     assert torch.equal(a.counts, b.counts) and torch.equal(a.balance, b.balance)
 
 
+@pytest.mark.parametrize("E", [10, 40, 300])
+@pytest.mark.parametrize("per_image", [False, True])
+def test_many_rows_with_masks_indices_and_counts(E, per_image):
+    B, Q, k = 6, 700, 3
+    gen = torch.Generator().manual_seed(E)
+    xs = [make((B, Q, E), "f16", 70 + s) for s in range(2)]
+    masks = [torch.rand(B, Q, generator=gen) < 0.7, torch.rand(B, Q, generator=gen) < 0.5]
+    masks[1][2] = False
+    experts = [torch.randint(-1, E, (B, Q, k), generator=gen) for _ in xs]
+    counts = torch.randint(0, 400, (2, B, E) if per_image else (2, E), generator=gen)
+    run_and_check(xs, k, masks=masks, per_image=per_image)
+    run_and_check(xs, k, masks=masks, experts=experts, per_image=per_image)
+    run_and_check(xs, k, masks=masks, counts=counts, per_image=per_image)
+    run_and_check(xs, k, masks=masks, experts=experts, counts=counts, scores="sigmoid", per_image=per_image)
+    # images apart in memory, the rows of each dense
+    whole = torch.zeros(B, Q + 5, E, dtype=torch.float16, device="cuda")
+    views = []
+    for x in xs:
+        whole[:, 3:Q + 3].copy_(x)
+        views.append(whole[:, 3:Q + 3].detach().requires_grad_(True))
+        whole = torch.zeros_like(whole)
+    run_and_check(xs, k, masks=masks, per_image=per_image, device_xs=views)
+
+
 @pytest.mark.parametrize("per_image", [False, True])
 def test_counts_of_all_ranks(per_image):
     """Two halves of a batch with the counts of both: the mean of their losses is the loss of the whole batch."""
