@@ -25,7 +25,7 @@
 //                   64 x 600 x 2 float32: 4.6 and 4.3
 //   cross entropy   256 x 900 x 92 float32 (85 MB, 21 MB): 22.4 and 18.7 us, 4.7 and 5.7 TB/s, at the rate of a copy;
 //                   16 x 301 x 1205 float16 (12 MB, 6 MB): 10.9 and 8.4
-// The sums of the workgroups' partial sums take 2 to 4 us more.  The host's part of a call and its backward pass, about 45 us,
+// The sums of the workgroups' partial sums take 2 to 4 us more; one workgroup by itself makes the loss as well.  The host's part of a call and its backward pass, about 45 us,
 // most of it the autograd engine's, covers all of these.
 #include <algorithm>
 #include <climits>
@@ -186,7 +186,7 @@ __global__ __launch_bounds__(CLS_THREADS) void focal_saved_kernel(const T *__res
                                                                   const unsigned n, const unsigned C, const unsigned rows,
                                                                   const FocalParams fp, unsigned *__restrict__ codes,
                                                                   int32_t *__restrict__ heads, double *__restrict__ partials,
-                                                                  int32_t *__restrict__ status)
+                                                                  float *__restrict__ loss_out, int32_t *__restrict__ status)
 {
     typedef typename dm::Quad<T>::type Four;
     __shared__ double lds[CLS_THREADS / 64];
@@ -300,7 +300,10 @@ __global__ __launch_bounds__(CLS_THREADS) void focal_saved_kernel(const T *__res
     }
     if (bad) dm::raise_status(status, DM_ST_LABEL_RANGE);
     const double total = block_sum((double)acc, lds);
-    if (threadIdx.x == 0) partials[blockIdx.x] = total;
+    if (threadIdx.x == 0) {
+        if (gridDim.x == 1) loss_out[0] = (float)(total * (double)fp.scale);
+        else partials[blockIdx.x] = total;
+    }
 }
 
 // The gradient of the logits that the bytes stand for, with the same exponential, logarithm and reciprocal per logit.
@@ -372,6 +375,18 @@ __device__ __forceinline__ float row_weight(int64_t y, unsigned C, int64_t ignor
     return weight ? weight[y] : 1.0f;
 }
 
+// A workgroup's sums: of the only one they are the loss (as cls_loss_finish_kernel makes it).
+__device__ __forceinline__ void ce_sums(double num, double den, double *partials, float *loss_out)
+{
+    if (gridDim.x == 1) {
+        loss_out[0] = (float)(num / den);
+        loss_out[1] = (float)(1.0 / den);
+    } else {
+        partials[2 * blockIdx.x] = num;
+        partials[2 * blockIdx.x + 1] = den;
+    }
+}
+
 // The bytes of the classes c .. c + 3 of a row of C, at any alignment.
 __device__ __forceinline__ void store_codes(uint8_t *row, unsigned c, unsigned C, unsigned packed)
 {
@@ -392,7 +407,8 @@ __global__ __launch_bounds__(CLS_THREADS) void ce_saved_kernel(const void *__res
                                                                const float *__restrict__ weight, const unsigned rows,
                                                                const unsigned C, const int64_t ignore_index,
                                                                uint8_t *__restrict__ codes, int8_t *__restrict__ steps,
-                                                               double *__restrict__ partials, int32_t *__restrict__ status)
+                                                               double *__restrict__ partials, float *__restrict__ loss_out,
+                                                               int32_t *__restrict__ status)
 {
     __shared__ double lds[CLS_THREADS / 64];
     constexpr int N = 4 * NQ;
@@ -468,10 +484,7 @@ __global__ __launch_bounds__(CLS_THREADS) void ce_saved_kernel(const void *__res
     if (bad) dm::raise_status(status, DM_ST_LABEL_RANGE);
     const double a = block_sum((double)num, lds);
     const double b = block_sum((double)den, lds);
-    if (threadIdx.x == 0) {
-        partials[2 * blockIdx.x] = a;
-        partials[2 * blockIdx.x + 1] = b;
-    }
+    if (threadIdx.x == 0) ce_sums(a, b, partials, loss_out);
 }
 
 // softmax of the decoded row less its own class, times weight and scale: the row's largest decodes to 0, so there is no maximum
@@ -566,7 +579,8 @@ __global__ __launch_bounds__(CLS_THREADS) void ce_saved_wide_kernel(const T *__r
                                                                     const float *__restrict__ weight, const unsigned rows,
                                                                     const unsigned C, const int64_t ignore_index,
                                                                     uint8_t *__restrict__ codes, int8_t *__restrict__ steps,
-                                                                    double *__restrict__ partials, int32_t *__restrict__ status)
+                                                                    double *__restrict__ partials, float *__restrict__ loss_out,
+                                                                    int32_t *__restrict__ status)
 {
     __shared__ RowStats lds[WIDE_WAVES];
     const float inf = __builtin_huge_valf();
@@ -629,10 +643,7 @@ __global__ __launch_bounds__(CLS_THREADS) void ce_saved_wide_kernel(const T *__r
         if (threadIdx.x == 0) steps[row] = (int8_t)(sum == sum ? e : NOT_A_NUMBER);
     }
     if (bad) dm::raise_status(status, DM_ST_LABEL_RANGE);
-    if (threadIdx.x == 0) {
-        partials[2 * blockIdx.x] = num;
-        partials[2 * blockIdx.x + 1] = den;
-    }
+    if (threadIdx.x == 0) ce_sums(num, den, partials, loss_out);
 }
 
 template <typename T>
@@ -682,12 +693,12 @@ __global__ __launch_bounds__(CLS_THREADS) void ce_from_saved_wide_kernel(const u
 
 template <typename T>
 void launch_focal_saved(const void *logits, const int64_t *cls, unsigned n, unsigned C, unsigned rows, const FocalParams &fp,
-                        uint8_t *codes, int32_t *heads, double *partials, int32_t *status, int blocks, hipStream_t st)
+                        uint8_t *codes, int32_t *heads, double *partials, float *loss_out, int32_t *status, int blocks, hipStream_t st)
 {
     auto kernel = fp.gamma == 2.0f ? (C == 1 ? focal_saved_kernel<T, true, true> : focal_saved_kernel<T, true, false>)
                                    : (C == 1 ? focal_saved_kernel<T, false, true> : focal_saved_kernel<T, false, false>);
     hipLaunchKernelGGL(kernel, dim3(blocks), dim3(CLS_THREADS), 0, st, static_cast<const T *>(logits), cls, n, C, rows, fp,
-                       reinterpret_cast<unsigned *>(codes), heads, partials, status);
+                       reinterpret_cast<unsigned *>(codes), heads, partials, loss_out, status);
 }
 template <typename T>
 void launch_focal_from_saved(const uint8_t *codes, const int32_t *heads, const int64_t *cls, unsigned n, unsigned C, unsigned rows,
@@ -702,18 +713,25 @@ void launch_focal_from_saved(const uint8_t *codes, const int32_t *heads, const i
 // Workgroups for a number of trips: as many as the chip holds at once (six per CU at these kernels' registers), each with the
 // same number of trips.  (256 x 900 x 91 logits are 5119 trips of the focal kernels: with 1707 workgroups, the most of which
 // each makes three, 171 of them wait for the others' end, 27.9 us; 1280 that make four take 26.8.)
-unsigned even_blocks(unsigned trips)
+// One for up to `alone` trips, which then makes the loss itself.
+unsigned even_blocks(unsigned trips, unsigned alone)
 {
+    if (trips <= alone) return 1;
     constexpr unsigned RESIDENT = 6 * 256;
     static_assert(RESIDENT <= (unsigned)CLS_MAX_BLOCKS, "a partial sum for each");
     const unsigned each = std::max(1u, (trips + RESIDENT - 1) / RESIDENT);
     return std::max(1u, (trips + each - 1) / each);
 }
 
-int focal_blocks(unsigned n)
+// Trips of a forward pass that one workgroup makes by itself: calls of one, two and three trips of the focal kernel (4096 logits each)
+// take 8.2, 8.2 and 9.7 us among others instead of 8.3, 11.0 and 11.1, of four 11.3 instead of 11.2; four trips of the cross
+// entropy 8.0 to 9.9 instead of 11.1, eight 9.3 to 17.3.
+constexpr unsigned FOCAL_ALONE = 3, CE_ALONE = 4;
+
+int focal_blocks(unsigned n, unsigned alone)
 {
     const unsigned per_block = BLOCK * BLOCKS_AT_A_TIME;
-    return (int)even_blocks(n / per_block + (n % per_block != 0));
+    return (int)even_blocks(n / per_block + (n % per_block != 0), alone);
 }
 
 constexpr unsigned WIDEST = 2048;      // logits of a row that a wavefront keeps in registers
@@ -764,23 +782,23 @@ void with_ce_form(unsigned C, F &&f)
     }
 #undef DM_FORM
 }
-unsigned ce_blocks(unsigned rows, unsigned C, bool filled)
+unsigned ce_blocks(unsigned rows, unsigned C, bool filled, unsigned alone)
 {
     const unsigned rows_per_block = C <= WIDEST ? (unsigned)(CLS_THREADS / ce_form(C, filled).L) : 1u;
-    return even_blocks(rows / rows_per_block + (rows % rows_per_block != 0));
+    return even_blocks(rows / rows_per_block + (rows % rows_per_block != 0), C <= WIDEST ? alone : 0);
 }
 template <typename T>
 void launch_ce_saved(const void *logits, int dtype, const int64_t *cls, const float *weight, unsigned rows, unsigned C, int64_t ignore_index,
-                     uint8_t *codes, int8_t *steps, double *partials, int32_t *status, unsigned blocks, hipStream_t st)
+                     uint8_t *codes, int8_t *steps, double *partials, float *loss_out, int32_t *status, unsigned blocks, hipStream_t st)
 {
     if (C > WIDEST) {
         hipLaunchKernelGGL(ce_saved_wide_kernel<T>, dim3(blocks), dim3(CLS_THREADS), 0, st, static_cast<const T *>(logits), cls, weight,
-                           rows, C, ignore_index, codes, steps, partials, status);
+                           rows, C, ignore_index, codes, steps, partials, loss_out, status);
         return;
     }
     with_ce_form<sizeof(T) == 2>(C, [&](auto nq, auto l) {
         hipLaunchKernelGGL((ce_saved_kernel<decltype(nq)::value, decltype(l)::value, sizeof(T) == 4>), dim3(blocks), dim3(CLS_THREADS), 0,
-                           st, logits, dtype, cls, weight, rows, C, ignore_index, codes, steps, partials, status);
+                           st, logits, dtype, cls, weight, rows, C, ignore_index, codes, steps, partials, loss_out, status);
     });
 }
 template <typename T>
@@ -822,12 +840,12 @@ extern "C" int dm_focal_loss_saved(const void *logits, int dtype, const int64_t 
     if (((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(heads)) & 3) != 0) return DM_E_INVALID_ARG;
     hipStream_t st = static_cast<hipStream_t>(stream);
     const unsigned n = (unsigned)(rows * C);
-    const int blocks = focal_blocks(n);
+    const int blocks = focal_blocks(n, FOCAL_ALONE);
     const FocalParams fp{alpha, gamma, scale, ignore_index, use_ignore};
     auto launch = dtype == DM_F32 ? launch_focal_saved<float> : dtype == DM_BF16 ? launch_focal_saved<dm::bf16_t> : launch_focal_saved<dm::half_t>;
-    launch(logits, target_cls, n, (unsigned)C, (unsigned)rows, fp, codes, heads, partials, status, blocks, st);
+    launch(logits, target_cls, n, (unsigned)C, (unsigned)rows, fp, codes, heads, partials, loss_out, status, blocks, st);
     rc = dm::check_hip(hipGetLastError(), "focal_saved_kernel launch");
-    if (rc != DM_OK) return rc;
+    if (rc != DM_OK || blocks == 1) return rc;
     hipLaunchKernelGGL(cls_loss_finish_kernel<true>, dim3(1), dim3(CLS_THREADS), 0, st, partials, blocks, scale, loss_out);
     return dm::check_hip(hipGetLastError(), "cls_loss_finish_kernel launch");
 }
@@ -842,7 +860,7 @@ extern "C" int dm_focal_loss_from_saved(const uint8_t *codes, const int32_t *hea
     if (rows == 0) return DM_OK;
     hipStream_t st = static_cast<hipStream_t>(stream);
     const unsigned n = (unsigned)(rows * C);
-    const int blocks = focal_blocks(n);
+    const int blocks = focal_blocks(n, 0);
     const FocalParams fp{alpha, gamma, scale, ignore_index, use_ignore};
     auto launch = dtype == DM_F32 ? launch_focal_from_saved<float>
                   : dtype == DM_BF16 ? launch_focal_from_saved<dm::bf16_t> : launch_focal_from_saved<dm::half_t>;
@@ -858,11 +876,11 @@ extern "C" int dm_cross_entropy_saved(const void *logits, int dtype, const int64
     if (rc != DM_OK) return rc;
     if (!known(dtype) || (codes != nullptr) != (steps != nullptr)) return DM_E_INVALID_ARG;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    const unsigned blocks = ce_blocks((unsigned)rows, (unsigned)C, dtype != DM_F32);
+    const unsigned blocks = ce_blocks((unsigned)rows, (unsigned)C, dtype != DM_F32, CE_ALONE);
     auto launch = dtype == DM_F32 ? launch_ce_saved<float> : dtype == DM_BF16 ? launch_ce_saved<dm::bf16_t> : launch_ce_saved<dm::half_t>;
-    launch(logits, dtype, target_cls, weight, (unsigned)rows, (unsigned)C, ignore_index, codes, steps, partials, status, blocks, st);
+    launch(logits, dtype, target_cls, weight, (unsigned)rows, (unsigned)C, ignore_index, codes, steps, partials, loss_out, status, blocks, st);
     rc = dm::check_hip(hipGetLastError(), "ce_saved_kernel launch");
-    if (rc != DM_OK) return rc;
+    if (rc != DM_OK || blocks == 1) return rc;
     hipLaunchKernelGGL(cls_loss_finish_kernel<false>, dim3(1), dim3(CLS_THREADS), 0, st, partials, (int)blocks, 1.0f, loss_out);
     return dm::check_hip(hipGetLastError(), "cls_loss_finish_kernel launch");
 }
@@ -878,6 +896,6 @@ extern "C" int dm_cross_entropy_from_saved(const uint8_t *codes, const int8_t *s
     auto launch = dtype == DM_F32 ? launch_ce_from_saved<float>
                   : dtype == DM_BF16 ? launch_ce_from_saved<dm::bf16_t> : launch_ce_from_saved<dm::half_t>;
     launch(codes, steps, dtype, target_cls, weight, (unsigned)rows, (unsigned)C, ignore_index, inv_weight, grad_loss, grad_out,
-           ce_blocks((unsigned)rows, (unsigned)C, false), static_cast<hipStream_t>(stream));
+           ce_blocks((unsigned)rows, (unsigned)C, false, 0), static_cast<hipStream_t>(stream));
     return dm::check_hip(hipGetLastError(), "ce_from_saved_kernel launch");
 }

@@ -192,6 +192,18 @@ def test_every_number_of_classes(C, dtype):
     check_ce(x, cls)
 
 
+@pytest.mark.parametrize("C", CLASSES)
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_more_rows_than_one_workgroup_takes(C, dtype):
+    rows = 1100 if C <= 16 else 600 if C <= 32 else 300 if C <= 128 else 70 if C <= 512 else 20
+    x, cls = inputs((1, rows, C), dtype, 3 * C, shift=-1.0)
+    cls[0, ::7] = -1
+    check_focal(x, cls, ignore_index=-1)
+    x, cls = inputs((1, rows, C), dtype, 3 * C + 1, none=C - 1)
+    cls[0, ::5] = -1
+    check_ce(x, cls, torch.rand(C, generator=torch.Generator().manual_seed(C)) + 0.1, ignore_index=-1)
+
+
 @pytest.mark.parametrize("rows", [(1, 1), (1, 43), (7, 300), (64, 600)])
 @pytest.mark.parametrize("C", [1, 2, 3, 9])
 def test_few_classes_many_rows(rows, C):
