@@ -20,7 +20,7 @@
 // The gradient is that of the loss at the decoded logits; the loss itself is of the logits as they came.
 //
 // Measured (a copy of a GiB runs at 5.1 TB/s, a kernel of a few workgroups takes 4 us among others), forward and backward:
-//   focal           256 x 900 x 91 float32 (84 MB of logits, 21 of bytes): 27 and 25 us, 4 TB/s, bound by the 50 to 60
+//   focal           256 x 900 x 91 float32 (84 MB of logits, 21 of bytes): 27 and 25 us, 4 TB/s, bound by 50 and 35 vector
 //                   instructions per logit, an exponential, a logarithm and a reciprocal among them; 4 x 300 x 1203 bfloat16: 7.6 and 6.1;
 //                   64 x 600 x 2 float32: 4.6 and 4.3
 //   cross entropy   256 x 900 x 92 float32 (85 MB, 21 MB): 22.4 and 18.7 us, 4.7 and 5.7 TB/s, at the rate of a copy;
