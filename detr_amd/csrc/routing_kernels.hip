@@ -692,8 +692,9 @@ __global__ __launch_bounds__(RT_THREADS) void router_backward_kernel(const Route
         const bool live = sum != 0.0f;
         const float inv = live ? __builtin_amdgcn_rcpf(sum) : 0.0f;
         dot *= inv;
-        // p (gb (f - dot) + gz lse); of a row that does not count 0 times 0, whatever comes from upstream
-        const float zpart = live ? gz * (mx + __builtin_amdgcn_logf(sum) * LN2) : 0.0f;
+        // p (gb (f - dot) + gz lse); of a row that does not count 0 times 0, whatever comes from upstream; with no gradient of z no
+        // product with lse at all: a sigmoid row may hold an infinite logit (its score is 1), and 0 times that is NaN
+        const float zpart = live && grad_z ? gz * (mx + __builtin_amdgcn_logf(sum) * LN2) : 0.0f;
         const float bpart = live ? gb : 0.0f;
 #pragma unroll
         for (int j = 0; j < N; ++j) x[j] = (x[j] * inv) * __builtin_fmaf(bpart, f[j] - dot, zpart);

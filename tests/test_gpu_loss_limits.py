@@ -1,0 +1,46 @@
+"""The 8-bit classification losses and the balance loss at the ends of what they take: infinite logits of sigmoid routers, sums of
+very many equal terms, a row of more than 2^30 classes, gammas below zero."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from detr_amd import _lib, losses
+from detr_amd._lib import lib
+from oracle import balance_loss as oracle
+from test_gpu_balance_loss import check_set
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+DTYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+
+
+@pytest.mark.parametrize("E", [3, 8, 13, 40, 160, 700])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("per_image", [False, True])
+def test_gradient_of_infinite_logits_with_sigmoid_scores(E, dtype, per_image):
+    """sigmoid(+inf) = 1: the loss is finite, and so is its gradient (0 at the infinite logit, whose score no longer moves).
+    The bound of tests/test_gpu_balance_loss.py: scores off by (5 D + 40) u with D the largest finite |x|, below 8 here."""
+    gen = torch.Generator().manual_seed(E)
+    x = torch.randn(3, 21, E, generator=gen).clamp(-7, 7).to(DTYPES[dtype])
+    x[0, 3, 1] = x[1, 4, E - 1] = x[1, 20, 0] = math.inf
+    x[2, 7, :2] = math.inf
+    x[2, 8] = math.inf                                     # even scores
+    x[0, 5, 0], x[0, 5, 2] = -math.inf, math.inf
+    leaf = x.cuda().requires_grad_(True)
+    out = losses.balance_losses(leaf, 2, scores="sigmoid", per_image=per_image)
+    (grad,) = torch.autograd.grad(out.balance.sum(), leaf)
+    want = oracle.balance_losses(x.double().numpy(), 2, scores="sigmoid", per_image=per_image,
+                                 grad_balance=np.ones(3 if per_image else 1))
+    assert np.isfinite(want["grad"]).all() and bool(grad.isfinite().all())
+    assert bool((grad[leaf.isinf()] == 0).all())
+    t = (5 * 8 + 40) * U
+    np.testing.assert_allclose(out.balance.detach().double().cpu().numpy().reshape(-1), want["balance"], rtol=t + 314 * U, atol=0)
+    fi = torch.finfo(grad.dtype)
+    p, f = want["p"], np.abs(want["f"])[:, None]
+    scale = np.abs(want["gb"])[:, None, None] * (f + (p * f).sum(-1, keepdims=True))
+    bound = t * p * scale + (fi.eps / 2 + 4 * U) * np.abs(want["grad"]) + fi.smallest_normal * fi.eps + 2.0 ** -126 * (1 + scale)
+    off = np.abs(grad.double().cpu().numpy() - want["grad"])
+    assert (off <= bound).all(), float((off / bound).max())
