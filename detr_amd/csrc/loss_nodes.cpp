@@ -9,11 +9,13 @@
 //
 // No GPU code: the kernels are reached through the addresses of libdetr_match.so's entry points, handed over once by `bind`.
 // Built against one torch version, which the module names (`built_for_torch`); the Python code refuses it under any other.
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include "detr_match.h"
@@ -77,6 +79,20 @@ int dtype_code(const Tensor &t, const char *what)
     default: TORCH_CHECK_TYPE(false, what, " must be float32, bfloat16 or float16, got ", t.scalar_type());
     }
     return -1;
+}
+
+// What works below autograd does not show: a tangent would be dropped without a word, and a trace would hold the allocations
+// without the kernels between them.
+void refuse_tracing()
+{
+    const bool proxies = c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value();
+    TORCH_CHECK_NOT_IMPLEMENTED(!torch::jit::tracer::isTracing() && !proxies,
+                                "detr_amd.losses: this call cannot be traced (torch.jit.trace, torch.fx of tensors)");
+}
+void refuse_tangent(const Tensor &t)
+{
+    TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(/*level=*/0).defined(),
+                                "detr_amd.losses: this loss has no derivative for forward-mode differentiation");
 }
 
 // A node that is used once unless the graph is retained, and whose gradients have no gradients of their own.
@@ -191,6 +207,9 @@ Tensor cls_losses(const std::vector<Tensor> &logits, const std::vector<Tensor> &
 {
     const size_t S = logits.size();
     TORCH_CHECK_VALUE(S > 0 && maps.size() == S, "one class map for every set of logits");
+    refuse_tracing();
+    for (const auto &x : logits) refuse_tangent(x);
+    if (weight_in) refuse_tangent(*weight_in);
     const at::Device device = logits[0].device();
     for (size_t i = 0; i < S; ++i) {
         const Tensor &x = logits[i], &cls = maps[i];
@@ -433,6 +452,8 @@ std::tuple<Tensor, std::optional<Tensor>, Tensor> balance_losses(const std::vect
     c.top_k = top_k;
     c.sigmoid = sigmoid;
     c.per_image = per_image;
+    refuse_tracing();
+    for (const auto &x : in) refuse_tangent(x);
     const bool grad = wants_grad(in);
     std::shared_ptr<BalanceNode> node;
     if (grad) {
@@ -487,6 +508,7 @@ Tensor expert_counts(const std::vector<Tensor> &in, int64_t top_k, const Optiona
     RouterCall c{};
     c.top_k = top_k;
     c.per_image = per_image;
+    refuse_tracing();
     const at::AutoDispatchBelowADInplaceOrView below;
     const Routers r(in, mask, OptionalTensors(in.size()), c);
     const at::Device device = r.logits[0].device();
