@@ -101,10 +101,12 @@ struct LossNode : torch::autograd::Node {
     {
         std::lock_guard<std::mutex> lock(mutex_);
         TORCH_CHECK(!released, torch::autograd::ERR_BACKWARD_TWICE);
+        // (the hooks of saved tensors may run anything, a whole forward pass among it: not below autograd)
+        const variable_list saved = unpack(grads);
         variable_list out;
         {
             const at::AutoDispatchBelowADInplaceOrView below;
-            out = backward(grads);
+            out = backward(grads, saved);
         }
         if (!at::GradMode::is_enabled()) return out;
         // create_graph=True: what would differentiate these gradients again is refused when it is tried
@@ -120,9 +122,29 @@ struct LossNode : torch::autograd::Node {
         released = true;
         drop();
     }
-    virtual variable_list backward(variable_list &grads) = 0;
+    // What the backward pass needs of the saved tensors, in an order of the node's own.
+    virtual variable_list unpack(const variable_list &grads) = 0;
+    virtual variable_list backward(const variable_list &grads, const variable_list &saved) = 0;
     virtual void drop() = 0;
     bool released = false;
+};
+
+// A saved tensor, and what the kernels take it for: a hook (torch.autograd.graph.saved_tensors_hooks) may hand back another.
+struct Saved {
+    SavedVariable variable;
+    at::Device device = at::kCPU;
+    at::ScalarType type = at::kByte;
+    at::DimVector sizes;
+
+    Saved() = default;
+    explicit Saved(const Tensor &t) : variable(t, false), device(t.device()), type(t.scalar_type()), sizes(t.sizes()) {}
+    Tensor unpack() const
+    {
+        const Tensor t = variable.unpack();
+        TORCH_CHECK(t.defined() && t.device() == device && t.scalar_type() == type && t.sizes() == at::IntArrayRef(sizes),
+                    "detr_amd.losses: a hook has handed back another saved tensor than ", type, " ", at::IntArrayRef(sizes), " on ", device);
+        return t;
+    }
 };
 
 bool wants_grad(const std::vector<Tensor> &inputs)
@@ -150,45 +172,60 @@ struct ClsNode : LossNode {
         at::DimVector shape;
         int dtype;
         int64_t rows, C, n, data;      // bytes of `codes` before the heads or steps
-        Tensor codes;
-        SavedVariable cls;
+        Saved codes, cls;              // (of the sets that need a gradient)
     };
     std::vector<Set> sets;
-    SavedVariable weight;
+    Saved weight;
     bool weighted = false;
-    Tensor out;                        // [S, 2]; cross entropy: 1 / sum of the weights in the second column
+    Saved out;                         // cross entropy: [S, 2], 1 / sum of the weights in the second column
 
     std::string name() const override { return call.ce ? "CrossEntropy8Backward" : "FocalLoss8Backward"; }
     void drop() override
     {
         for (auto &s : sets) {
-            s.codes.reset();
-            s.cls.reset_data();
+            s.codes.variable.reset_data();
+            s.cls.variable.reset_data();
         }
-        weight.reset_data();
-        out.reset();
+        weight.variable.reset_data();
+        out.variable.reset_data();
     }
-    variable_list backward(variable_list &grads) override
+    variable_list unpack(const variable_list &grads) override
+    {
+        variable_list saved(2 * sets.size() + 2);
+        if (!grads[0].defined()) return saved;
+        bool any = false;
+        for (size_t i = 0; i < sets.size(); ++i) {
+            if (!task_should_compute_output(i) || sets[i].n == 0) continue;
+            saved[2 * i] = sets[i].codes.unpack();
+            saved[2 * i + 1] = sets[i].cls.unpack();
+            any = true;
+        }
+        if (any && weighted) saved[2 * sets.size()] = weight.unpack();
+        if (any && call.ce) saved[2 * sets.size() + 1] = out.unpack();
+        return saved;
+    }
+    variable_list backward(const variable_list &grads, const variable_list &saved) override
     {
         variable_list result(sets.size());
         if (!grads[0].defined()) return result;
         const Tensor upstream = grads[0].contiguous();
         const c10::DeviceGuard guard(upstream.device());
         void *stream = current_stream(upstream.device());
-        const Tensor w = weighted ? weight.unpack() : Tensor();
+        auto dense = [](const Tensor &t) { return t.defined() ? t.contiguous() : t; };
+        const Tensor w = dense(saved[2 * sets.size()]), sums = dense(saved[2 * sets.size() + 1]);
         for (size_t i = 0; i < sets.size(); ++i) {
             if (!task_should_compute_output(i)) continue;
             Set &s = sets[i];
             Tensor grad = at::empty(s.shape, s.options);
             result[i] = grad;
             if (s.n == 0) continue;
-            const Tensor cls = s.cls.unpack();
-            const auto *codes = static_cast<const uint8_t *>(s.codes.const_data_ptr());
+            const Tensor bytes = dense(saved[2 * i]), cls = dense(saved[2 * i + 1]);
+            const auto *codes = bytes.const_data_ptr<uint8_t>();
             const auto *g_loss = static_cast<const float *>(upstream.const_data_ptr()) + i;
             if (call.ce)
                 check(g.ce_from_saved(codes, reinterpret_cast<const int8_t *>(codes + s.data), s.dtype, cls.const_data_ptr<int64_t>(),
-                                      weighted ? w.const_data_ptr<float>() : nullptr, s.rows, static_cast<int>(s.C), call.ignore_index,
-                                      out.const_data_ptr<float>() + 2 * i + 1, g_loss, grad.mutable_data_ptr(), stream),
+                                      w.defined() ? w.const_data_ptr<float>() : nullptr, s.rows, static_cast<int>(s.C), call.ignore_index,
+                                      sums.const_data_ptr<float>() + 2 * i + 1, g_loss, grad.mutable_data_ptr(), stream),
                       "dm_cross_entropy_from_saved");
             else
                 check(g.focal_from_saved(codes, reinterpret_cast<const int32_t *>(codes + s.data), s.dtype, cls.const_data_ptr<int64_t>(),
@@ -230,7 +267,7 @@ Tensor cls_losses(const std::vector<Tensor> &logits, const std::vector<Tensor> &
         node->call = call;
         node->sets.resize(S);
     }
-    const at::AutoDispatchBelowADInplaceOrView below;
+    std::optional<at::AutoDispatchBelowADInplaceOrView> below(std::in_place);
     const c10::DeviceGuard guard(device);
     Tensor weight;
     if (weight_in) {
@@ -246,6 +283,7 @@ Tensor cls_losses(const std::vector<Tensor> &logits, const std::vector<Tensor> &
     const Tensor partials = at::empty({DM_CLS_LOSS_PARTIALS}, bytes.dtype(at::kDouble));
     Tensor out = at::empty({static_cast<int64_t>(S), 2}, floats);
     void *stream = current_stream(device);
+    std::vector<Tensor> kept(2 * S);                   // codes and classes
     for (size_t i = 0; i < S; ++i) {
         const Tensor x = logits[i].contiguous(), cls = maps[i].contiguous();
         const int dtype = dtype_code(x, "logits");
@@ -281,17 +319,26 @@ Tensor cls_losses(const std::vector<Tensor> &logits, const std::vector<Tensor> &
             s.C = C;
             s.n = n;
             s.data = data;
-            s.codes = codes;
-            s.cls = SavedVariable(cls, false);
+            if (codes.defined()) {
+                kept[2 * i] = codes;
+                kept[2 * i + 1] = cls;
+            }
         }
     }
     Tensor losses = scalar ? out.select(1, 0).select(0, 0) : out.select(1, 0);
     if (grad) {
+        below.reset();                                 // (saving may run hooks)
+        for (size_t i = 0; i < S; ++i) {
+            if (!kept[2 * i].defined()) continue;
+            node->sets[i].codes = Saved(kept[2 * i]);
+            node->sets[i].cls = Saved(kept[2 * i + 1]);
+        }
         if (weight.defined()) {
-            node->weight = SavedVariable(weight, false);
+            node->weight = Saved(weight);
             node->weighted = true;
         }
-        node->out = out;
+        // (a version of its own: the losses, which may be changed in place, are the other column)
+        if (call.ce) node->out = Saved(out.variable_data());
         torch::autograd::set_history(losses, node);
     }
     return losses;
@@ -404,39 +451,53 @@ Tensor workspace_for(const std::vector<DmRouterSet> &sets, const RouterCall &c, 
 
 struct BalanceNode : LossNode {
     RouterCall call;
-    std::vector<SavedVariable> logits, masks;
+    std::vector<Saved> logits, masks;
     std::vector<char> masked;
-    Tensor kept;      // slope [groups, E], then 1 / n [groups]
+    Saved kept;       // slope [groups, E], then 1 / n [groups]
 
     std::string name() const override { return "BalanceLossesBackward"; }
     void drop() override
     {
-        for (auto &v : logits) v.reset_data();
-        for (auto &v : masks) v.reset_data();
-        kept.reset();
+        for (auto &v : logits) v.variable.reset_data();
+        for (auto &v : masks) v.variable.reset_data();
+        kept.variable.reset_data();
     }
-    variable_list backward(variable_list &grads) override
+    static bool any(const variable_list &grads) { return grads[0].defined() || (grads.size() > 1 && grads[1].defined()); }
+    variable_list unpack(const variable_list &grads) override
+    {
+        const size_t S = logits.size();
+        variable_list saved(2 * S + 1);
+        if (!any(grads)) return saved;
+        for (size_t i = 0; i < S; ++i) {
+            saved[2 * i] = logits[i].unpack();
+            if (masked[i]) saved[2 * i + 1] = masks[i].unpack();
+        }
+        saved[2 * S] = kept.unpack();
+        return saved;
+    }
+    variable_list backward(const variable_list &grads, const variable_list &saved) override
     {
         const size_t S = logits.size();
         variable_list result(S);
-        const bool any = grads[0].defined() || (grads.size() > 1 && grads[1].defined());
-        if (!any) return result;
+        if (!any(grads)) return result;
         const Tensor gb = grads[0].defined() ? grads[0].contiguous() : Tensor();
         const Tensor gz = grads.size() > 1 && grads[1].defined() ? grads[1].contiguous() : Tensor();
-        const c10::DeviceGuard guard(kept.device());
+        const Tensor shares = saved[2 * S].contiguous();
+        const c10::DeviceGuard guard(shares.device());
         std::vector<DmRouterSet> sets(S);
         std::vector<Tensor> held(2 * S);
         for (size_t i = 0; i < S; ++i) {
-            held[2 * i] = logits[i].unpack();
-            if (masked[i]) held[2 * i + 1] = masks[i].unpack();
-            result[i] = at::empty(held[2 * i].sizes(), held[2 * i].options().memory_format(at::MemoryFormat::Contiguous));
+            const Tensor &x = saved[2 * i];
+            held[2 * i] = image_stride(x) >= 0 ? x : x.contiguous();
+            if (masked[i]) held[2 * i + 1] = saved[2 * i + 1].contiguous();
+            result[i] = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
             describe(sets, i, held[2 * i], held[2 * i + 1], Tensor(), &result[i]);
         }
-        const float *slope = kept.const_data_ptr<float>();
+        const float *slope = shares.const_data_ptr<float>();
         check(g.balance_backward(sets.data(), static_cast<int>(S), static_cast<int>(call.B), static_cast<int>(call.E), call.dtype,
                                  call.sigmoid, call.per_image, slope, slope + call.groups() * call.E,
                                  gb.defined() ? gb.const_data_ptr<float>() : nullptr, gz.defined() ? gz.const_data_ptr<float>() : nullptr,
-                                 current_stream(kept.device())),
+                                 current_stream(shares.device())),
               "dm_balance_backward");
         for (size_t i = 0; i < S; ++i)
             if (!task_should_compute_output(i)) result[i].reset();
@@ -460,7 +521,7 @@ std::tuple<Tensor, std::optional<Tensor>, Tensor> balance_losses(const std::vect
         node = std::shared_ptr<BalanceNode>(new BalanceNode(), torch::autograd::deleteNode);
         node->set_next_edges(torch::autograd::collect_next_edges(in));
     }
-    const at::AutoDispatchBelowADInplaceOrView below;
+    std::optional<at::AutoDispatchBelowADInplaceOrView> below(std::in_place);
     const Routers r(in, mask, given, c);
     const at::Device device = r.logits[0].device();
     const c10::DeviceGuard guard(device);
@@ -488,14 +549,15 @@ std::tuple<Tensor, std::optional<Tensor>, Tensor> balance_losses(const std::vect
                          workspace.numel(), status.mutable_data_ptr<int32_t>(), current_stream(device)),
           "dm_balance_loss");
     if (grad) {
+        below.reset();                                 // (saving may run hooks)
         node->call = c;
-        node->kept = kept;
+        node->kept = Saved(kept);
         node->masked.resize(in.size());
         node->masks.resize(in.size());
         for (size_t i = 0; i < in.size(); ++i) {
-            node->logits.emplace_back(r.logits[i], false);
+            node->logits.emplace_back(r.logits[i]);
             node->masked[i] = r.masks[i].defined();
-            if (node->masked[i]) node->masks[i] = SavedVariable(r.masks[i], false);
+            if (node->masked[i]) node->masks[i] = Saved(r.masks[i]);
         }
         torch::autograd::set_history(balance, node);
         if (!sigmoid) torch::autograd::set_history(z, node);

@@ -33,6 +33,111 @@ NAMES = ["focal", "ce", "balance", "sigmoid"]
 
 
 @pytest.mark.parametrize("name", NAMES)
+def test_hooks_see_all_that_is_saved(name):
+    x, cls = data()
+    mask = torch.rand(cls.shape, generator=torch.Generator().manual_seed(1)).cuda() < 0.8
+    loss, least = calls(cls, mask)[name]
+    x.requires_grad_(True)
+    (want,) = torch.autograd.grad(loss(x), x)
+    packed, unpacked = [], []
+
+    def pack(t):
+        packed.append(t.numel() * t.element_size())
+        return t.cpu(), t.device
+
+    def unpack(p):
+        unpacked.append(p[0].numel() * p[0].element_size())
+        return p[0].to(p[1])
+
+    with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+        value = loss(x)
+    # (what is kept, the classes or logits, the mask; beside what torch's own nodes around it save)
+    inputs = 8 * cls.numel() if name in ("focal", "ce") else 2 * 4 * x.numel() + 2 * mask.numel()
+    assert sum(packed) >= least + inputs and not unpacked
+    (got,) = torch.autograd.grad(value, x)
+    assert torch.equal(got, want) and sum(unpacked) >= least + inputs
+
+
+@pytest.mark.parametrize("name", ["focal", "ce"])
+def test_saved_bytes_leave_the_gpu(name):
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    cls = torch.zeros(64, 3000, dtype=torch.int64, device="cuda")
+    x = torch.randn(64, 3000, 21, device="cuda", generator=gen, requires_grad=True)
+    loss, n = calls(cls)[name]
+    (want,) = torch.autograd.grad(loss(x), x)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    with torch.autograd.graph.save_on_cpu():
+        value = loss(x)
+    torch.cuda.synchronize()
+    assert torch.cuda.memory_allocated() - before < n // 8
+    (got,) = torch.autograd.grad(value, x)
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("name", NAMES)
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_checkpoints(name, reentrant):
+    """Without reentrance what is saved is dropped, and computed again when the backward pass asks for it."""
+    from torch.utils.checkpoint import checkpoint
+
+    x, cls = data()
+    loss, _ = calls(cls)[name]
+    results = []
+    for how in (lambda f, *a: f(*a), lambda f, *a: checkpoint(f, *a, use_reentrant=reentrant)):
+        a, b = x.clone().requires_grad_(True), torch.linspace(0.5, 1.5, 21, device="cuda").requires_grad_(True)
+        value = how(lambda a, b: loss(a * b), a, b)
+        value.backward()
+        results.append((value.detach(), a.grad, b.grad))
+    for plain, again in zip(*results):
+        assert torch.equal(plain, again)
+
+
+@pytest.mark.parametrize("name", NAMES)
+@pytest.mark.parametrize("wrong", ["device", "type", "shape"])
+def test_a_hook_that_hands_back_another_tensor_is_refused(name, wrong):
+    x, cls = data()
+    loss, _ = calls(cls)[name]
+    x.requires_grad_(True)
+    other = {"device": lambda t: t.cpu(), "type": lambda t: t.double(), "shape": lambda t: t.flatten()[1:]}[wrong]
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, other):
+        value = loss(x).view(1)          # (no node of torch's own below saves a tensor)
+    with pytest.raises(RuntimeError, match="saved tensor"):
+        torch.autograd.grad(value.sum(), x)
+
+
+def test_a_hook_may_hand_back_other_strides():
+    x, cls = data()
+    for name in NAMES:
+        loss, _ = calls(cls)[name]
+        leaf = x.clone().requires_grad_(True)
+        (want,) = torch.autograd.grad(loss(leaf), leaf)
+
+        def apart(t):
+            wide = torch.zeros(*t.shape, 3, dtype=t.dtype, device=t.device)
+            wide[..., 1] = t
+            return wide[..., 1]
+
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, apart):
+            value = loss(leaf)
+        (got,) = torch.autograd.grad(value, leaf)
+        assert torch.equal(got, want)
+
+
+def test_the_loss_may_be_changed_in_place():
+    """The loss shares its memory with what is kept for the backward pass, not its version."""
+    x, cls = data()
+    for name in NAMES:
+        loss, _ = calls(cls)[name]
+        leaf = x.clone().requires_grad_(True)
+        (want,) = torch.autograd.grad(loss(leaf), leaf)
+        value = loss(leaf)
+        value *= 2.0
+        (got,) = torch.autograd.grad(value, leaf)
+        torch.testing.assert_close(got, 2 * want, rtol=2.0 ** -22, atol=2.0 ** -126)
+
+
+@pytest.mark.parametrize("name", NAMES)
 def test_forward_mode_and_tracing_are_refused(name):
     import torch.autograd.forward_ad as fw
 
