@@ -86,7 +86,7 @@ def fuse_cls_criterion(own, seen_devices=None, saved_bits: int = 32) -> bool:
     if name == "FocalLoss" and all(hasattr(own, a) for a in ("alpha", "gamma", "n_cls")):
         def forward(inputs, targets, num_boxes):
             x = losses._class_last(inputs, targets, own.n_cls, None)
-            if x is None or x.shape[-1] != own.n_cls or not losses._takes(x, targets, saved_bits):
+            if x is None or x.shape[-1] != own.n_cls or not losses._takes(x, targets, saved_bits, own.gamma):
                 return own_forward(inputs, targets, num_boxes)
             if seen_devices is not None:
                 seen_devices.add(x.device)

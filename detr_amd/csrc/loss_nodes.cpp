@@ -348,6 +348,7 @@ Tensor focal_losses(const std::vector<Tensor> &logits, const std::vector<Tensor>
                     const std::vector<double> &scales, std::optional<int64_t> ignore_index, bool scalar, const Tensor &status)
 {
     TORCH_CHECK_VALUE(scales.size() == logits.size(), "one scale for every set of logits");
+    TORCH_CHECK_VALUE(!(gamma < 0.0), "gamma must not be below zero with saved_bits=8, got ", gamma);
     return cls_losses(logits, maps, std::nullopt, ClsCall{false, alpha, gamma, scales, ignore_index.value_or(0), ignore_index.has_value()},
                       scalar, status);
 }

@@ -11,7 +11,8 @@
 //                   the rounding of a float32 gradient of order one, and one masked logit does not take the block's
 //                   resolution away.  The span is 40 at most, so 2^-2 always suffices and no byte is cut off at 255.
 //                   Logits of rows that do not count take no part: a padded row may hold anything.
-//                   A head per block, 32 bits: largest whole number << 8 | e.
+//                   A head per block, 32 bits: largest whole number << 8 | e.  With a gamma below zero none of this would hold
+//                   (a slope falls off like exp((1 + gamma) z) only): refused.
 //   cross entropy   a block is a row: the softmax does not change when a row's largest logit is taken off, so e is all that
 //                   is kept beside the bytes.  2^-3 at most: logits further below the largest than 31.9 are cut off there,
 //                   at a probability of e^-31.9 = 1e-14.  (Logits beyond +-2^20 count as +-2^20.)
@@ -836,7 +837,7 @@ extern "C" int dm_focal_loss_saved(const void *logits, int dtype, const int64_t 
 {
     int rc = check_common(logits, target_cls, rows, C, loss_out, partials, status);
     if (rc != DM_OK) return rc;
-    if (!known(dtype) || (codes != nullptr) != (heads != nullptr)) return DM_E_INVALID_ARG;
+    if (!known(dtype) || (codes != nullptr) != (heads != nullptr) || gamma < 0.0f) return DM_E_INVALID_ARG;
     if (((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(heads)) & 3) != 0) return DM_E_INVALID_ARG;
     hipStream_t st = static_cast<hipStream_t>(stream);
     const unsigned n = (unsigned)(rows * C);
@@ -856,6 +857,7 @@ extern "C" int dm_focal_loss_from_saved(const uint8_t *codes, const int32_t *hea
 {
     const int rc = check_from_saved(codes, heads, dtype, target_cls, rows, C, grad_loss, grad_out);
     if (rc != DM_OK) return rc;
+    if (gamma < 0.0f) return DM_E_INVALID_ARG;
     if (((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(heads)) & 3) != 0) return DM_E_INVALID_ARG;
     if (rows == 0) return DM_OK;
     hipStream_t st = static_cast<hipStream_t>(stream);

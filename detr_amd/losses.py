@@ -374,7 +374,8 @@ def focal_loss(logits: torch.Tensor, target_cls: torch.Tensor, num_boxes, alpha:
     byte that stands for the logit itself -- 128 consecutive logits share a power-of-two step, 2^-16 to 2^-2 as their range
     asks, 1/16 for a range of 8 to 15.9; logits beyond +-20 count as +-20 -- from which the backward pass computes the
     gradient: a quarter of the memory between the passes, the same loss, and the gradient at logits that are off by at most
-    half a step.  With 8 bits the logits may also be bfloat16 or float16; their gradient is of their type."""
+    half a step.  With 8 bits the logits may also be bfloat16 or float16; their gradient is of their type.  A `gamma` below
+    zero needs 32 bits."""
     if _check_saved_bits(saved_bits):
         return _loss_nodes().focal_losses([logits], [target_cls], float(alpha), float(gamma), [1.0 / float(num_boxes)], ignore_index,
                                           True, _status_word(logits.device))
@@ -393,8 +394,10 @@ def cross_entropy(logits: torch.Tensor, target_cls: torch.Tensor, weight: Option
     return _CrossEntropy.apply(logits, target_cls, weight, ignore_index)
 
 
-def _takes(x, targets, saved_bits: int = 32) -> bool:
+def _takes(x, targets, saved_bits: int = 32, gamma: float = 0.0) -> bool:
     """Whether the kernels take these tensors as they are (anything else goes to the caller's own implementation)."""
+    if saved_bits == 8 and gamma < 0.0:
+        return False
     return x.is_cuda and (x.dtype == torch.float32 or (saved_bits == 8 and x.dtype in _lib.DTYPE_CODES)) \
         and targets.dtype == torch.int64 and targets.device == x.device
 
@@ -421,7 +424,7 @@ class FocalLoss(torch.nn.Module):
     `forward(inputs, targets, num_boxes)` with `inputs` [B, n_cls, Q] (/root/reference/models/detr/loss.py:208-213) or
     [B, Q, n_cls] (/root/reference/models/co_detr/loss.py:272-276) -- `channels_first` says which, None tells them
     apart by their shape -- and `targets` the [B, Q] class map.  Inputs the kernel does not take (not float32, not on
-    a GPU, a layout that cannot be told) go to `fallback` when one is given.  `saved_bits` as in `focal_loss`."""
+    a GPU, a layout that cannot be told, with 8 bits a gamma below zero) go to `fallback` when one is given.  `saved_bits` as in `focal_loss`."""
 
     def __init__(self, alpha: float, gamma: float, n_cls: int, channels_first: Optional[bool] = None, fallback=None,
                  saved_bits: int = 32):
@@ -432,8 +435,10 @@ class FocalLoss(torch.nn.Module):
 
     def forward(self, inputs, targets, num_boxes):
         x = _class_last(inputs, targets, self.n_cls, self.channels_first)
-        if x is None or x.shape[-1] != self.n_cls or not _takes(x, targets, self.saved_bits):
+        if x is None or x.shape[-1] != self.n_cls or not _takes(x, targets, self.saved_bits, self.gamma):
             if self.fallback is None:
+                if self.saved_bits == 8 and self.gamma < 0.0:
+                    raise ValueError("gamma must not be below zero with saved_bits=8, got %s" % self.gamma)
                 raise RuntimeError("detr_amd.losses.FocalLoss: float32 GPU logits of [B, Q, n_cls] or [B, n_cls, Q] expected")
             return self.fallback(inputs, targets, num_boxes)
         return focal_loss(x, targets, num_boxes, self.alpha, self.gamma, saved_bits=self.saved_bits)

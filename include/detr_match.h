@@ -353,6 +353,7 @@ int dm_cross_entropy_f32(const float *logits, const int64_t *target_cls, const f
  *   codes          device, 4-byte aligned for the focal loss: rows * C bytes rounded up to 128 there, rows * C for the
  *                  cross entropy; NULL with heads / steps NULL: the loss alone
  *   grad_loss      device float: the gradient of the loss
+ *   gamma          not below zero: the clamp at +-20 stands on sigmoid^gamma falling off (DM_E_INVALID_ARG)
  *   inv_weight     device float: loss_out[1] of the forward call
  * The other arguments, the limits and the status bits are those of the calls above.
  */

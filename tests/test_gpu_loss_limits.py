@@ -44,3 +44,18 @@ def test_gradient_of_infinite_logits_with_sigmoid_scores(E, dtype, per_image):
     bound = t * p * scale + (fi.eps / 2 + 4 * U) * np.abs(want["grad"]) + fi.smallest_normal * fi.eps + 2.0 ** -126 * (1 + scale)
     off = np.abs(grad.double().cpu().numpy() - want["grad"])
     assert (off <= bound).all(), float((off / bound).max())
+
+
+def test_a_gamma_below_zero_is_refused():
+    x = torch.randn(3, 7, 5, device="cuda")
+    cls = torch.zeros(3, 7, dtype=torch.int64, device="cuda")
+    with pytest.raises(ValueError, match="gamma"):
+        losses.focal_loss(x, cls, 1.0, gamma=-0.5, saved_bits=8)
+    seen = []
+    module = losses.FocalLoss(0.25, -0.5, 5, fallback=lambda *a: seen.append(a) or "own", saved_bits=8)
+    assert module(x, cls, 1.0) == "own" and len(seen) == 1
+    with pytest.raises(ValueError, match="gamma"):
+        losses.FocalLoss(0.25, -0.5, 5, saved_bits=8)(x, cls, 1.0)
+    # (the 32-bit form has it)
+    assert losses.focal_loss(x, cls, 1.0, gamma=-0.5).isfinite()
+    assert losses.FocalLoss(0.25, -0.5, 5)(x, cls, 1.0).isfinite()

@@ -47,3 +47,29 @@ def test_tracing_the_counts_is_refused():
     for trace in (lambda: torch.jit.trace(call, (torch.zeros(2, 3, 4),), check_trace=False), lambda: make_fx(call)(torch.zeros(2, 3, 4))):
         with pytest.raises(NotImplementedError, match="trace"):
             trace()
+
+
+def test_a_gamma_below_zero_is_refused():
+    # (a call of no rows ends on the host)
+    assert lib.dm_focal_loss_from_saved(None, None, 0, None, 0, 4, 0.25, -0.5, 1.0, 0, 0, None, None, None) == _lib.E_INVALID_ARG
+    assert lib.dm_focal_loss_from_saved(None, None, 0, None, 0, 4, 0.25, 0.5, 1.0, 0, 0, None, None, None) == 0
+    with pytest.raises(ValueError, match="gamma"):
+        losses._loss_nodes().focal_losses([torch.zeros(1, 2)], [torch.zeros(1, dtype=torch.int64)], 0.25, -0.5, [1.0], None, True,
+                                          torch.zeros(1, dtype=torch.int32))
+
+
+class FocalLoss(torch.nn.Module):
+    def __init__(self):
+        super().__init__()
+        self.alpha, self.gamma, self.n_cls = 0.25, 2.0, 6
+
+    def forward(self, inputs, targets, num_boxes):
+        return "own"
+
+
+def test_a_gamma_below_zero_stays_with_the_module():
+    module = FocalLoss()
+    module.gamma = -0.5
+    criterion.fuse_cls_criterion(module, saved_bits=8)
+    assert not losses._takes(torch.zeros(2, 3, 6), torch.zeros(2, 3, dtype=torch.int64), 8, gamma=-0.5)
+    assert module(torch.zeros(2, 3, 6), torch.zeros(2, 3, dtype=torch.int64), 1) == "own"
