@@ -74,23 +74,28 @@ def fuse_cls_criterion(own, seen_devices=None, saved_bits: int = 32) -> bool:
     they keep.  The module object, its buffers and its ``state_dict`` stay as they are: the replacement is an instance
     attribute ``forward`` (removed by `unfuse_cls_criterion`), which reads the parameters from `own` at every call and
     hands anything the kernels do not take (CPU or non-float32 tensors, a [B, Q, C] / [B, C, Q] layout that cannot be told
-    because Q == C) to the module's own forward.  `saved_bits` as in `losses.focal_loss`.  Returns whether `own` was
-    recognised."""
+    because Q == C) to the module's own forward.  `saved_bits` as in `losses.focal_loss`; of a module that is fused already
+    the latest call's is in force.  Returns whether `own` was recognised (a `forward` of somebody else's in front of the
+    class's is left there, and knows of no 8 bits)."""
     from . import losses
 
     losses._check_saved_bits(saved_bits)
     if "forward" in own.__dict__:
-        return True
+        in_force = getattr(own.__dict__["forward"], "saved_bits", None)
+        if in_force is not None:
+            in_force[0] = saved_bits
+        return in_force is not None or saved_bits == 32
+    bits = [saved_bits]
     name = type(own).__name__
     own_forward = own.forward
     if name == "FocalLoss" and all(hasattr(own, a) for a in ("alpha", "gamma", "n_cls")):
         def forward(inputs, targets, num_boxes):
             x = losses._class_last(inputs, targets, own.n_cls, None)
-            if x is None or x.shape[-1] != own.n_cls or not losses._takes(x, targets, saved_bits, own.gamma):
+            if x is None or x.shape[-1] != own.n_cls or not losses._takes(x, targets, bits[0], own.gamma):
                 return own_forward(inputs, targets, num_boxes)
             if seen_devices is not None:
                 seen_devices.add(x.device)
-            return losses.focal_loss(x, targets, num_boxes, own.alpha, own.gamma, saved_bits=saved_bits)
+            return losses.focal_loss(x, targets, num_boxes, own.alpha, own.gamma, saved_bits=bits[0])
     elif name == "CrossEntropy" and isinstance(getattr(own, "criterion", None), torch.nn.CrossEntropyLoss) \
             and own.criterion.reduction == "mean" and own.criterion.label_smoothing == 0.0:
         def forward(inputs, targets, num_boxes=None):
@@ -98,13 +103,14 @@ def fuse_cls_criterion(own, seen_devices=None, saved_bits: int = 32) -> bool:
             w = inner.weight
             C = w.shape[0] if w is not None else None
             x = losses._class_last(inputs, targets, C, None) if C is not None else None
-            if x is None or not losses._takes(x, targets, saved_bits) or w.device != x.device or w.dtype != torch.float32:
+            if x is None or not losses._takes(x, targets, bits[0]) or w.device != x.device or w.dtype != torch.float32:
                 return own_forward(inputs, targets, num_boxes)
             if seen_devices is not None:
                 seen_devices.add(x.device)
-            return losses.cross_entropy(x, targets, w, inner.ignore_index, saved_bits)
+            return losses.cross_entropy(x, targets, w, inner.ignore_index, bits[0])
     else:
         return False
+    forward.saved_bits = bits
     own.forward = forward          # (an instance attribute in front of the class's method)
     return True
 
@@ -205,19 +211,31 @@ def attach(criterion: torch.nn.Module, keys: Sequence[str] = MATCHED_KEYS, aux_h
     classification losses keep of every logit for the backward pass, as in `losses.focal_loss`.
     The wrappers are instance attributes holding local functions:
     `detach` the criterion before pickling the object itself (its ``state_dict`` is not affected).  Returns the
-    matcher.  Calling it twice on one criterion is harmless."""
+    matcher.  Calling it twice on one criterion is harmless; with `fused_consumers` the second call's `saved_bits` are in force
+    from then on (8 for a criterion that was attached without them: ValueError, `detach` it first)."""
     if saved_bits not in (32, 8) or (saved_bits == 8 and not fused_consumers):
         raise ValueError("saved_bits must be 32, or 8 with fused_consumers")
+    attached = getattr(criterion, "_detr_amd_hooks", None) is not None
+    bits_in_force = getattr(criterion, "_detr_amd_saved_bits", None) if attached else None
+    if attached and bits_in_force is None and saved_bits != 32:
+        raise ValueError("saved_bits=8: the criterion is attached without fused_consumers; detach it first")
     matcher = matcher_like(criterion.matcher)
     criterion.matcher = matcher
     heads = getattr(criterion, "aux_heads", None)
     if aux_heads and isinstance(heads, dict):
         for key in list(heads):
             heads[key] = aux_head_like(heads[key])
-    if getattr(criterion, "_detr_amd_hooks", None) is not None:
+    if attached:
+        if fused_consumers and bits_in_force is not None:
+            bits_in_force[0] = saved_bits
+            fused = getattr(criterion, "cls_criterion", None)
+            if isinstance(fused, torch.nn.Module) and "forward" in fused.__dict__:
+                fuse_cls_criterion(fused, None, saved_bits)
         return matcher
     device_indices = device_indices or fused_consumers
     cls_devices = set()
+    bits = [saved_bits]
+    criterion._detr_amd_saved_bits = bits if fused_consumers else None
     if fused_consumers and isinstance(getattr(criterion, "cls_criterion", None), torch.nn.Module):
         fuse_cls_criterion(criterion.cls_criterion, cls_devices, saved_bits)
     if fused_consumers and callable(getattr(criterion, "calc_box_loss", None)):
@@ -285,7 +303,7 @@ def attach(criterion: torch.nn.Module, keys: Sequence[str] = MATCHED_KEYS, aux_h
             n_cls = criterion.n_cls
             device = logits.device
             if logits.dim() != 3 or logits.shape[-1] != n_cls \
-                    or not losses._takes(logits, torch.empty(0, dtype=torch.int64, device=device), saved_bits):
+                    or not losses._takes(logits, torch.empty(0, dtype=torch.int64, device=device), bits[0]):
                 return own_with_ignore(outputs, targets, pos_indices, neg_indices)
             n_pos = sum(int(src.shape[0]) for src, _ in pos_indices)
             target_cls = torch.full(logits.shape[:2], -1, dtype=torch.int64, device=device)
@@ -312,7 +330,7 @@ def attach(criterion: torch.nn.Module, keys: Sequence[str] = MATCHED_KEYS, aux_h
                     neg_b, neg_q = neg_b.to(device), neg_q.to(device)
                 target_cls[neg_b, neg_q] = n_cls
             cls_devices.add(device)
-            return losses.focal_loss(logits, target_cls, max(n_pos, 1), 0.25, 2.0, ignore_index=-1, saved_bits=saved_bits)
+            return losses.focal_loss(logits, target_cls, max(n_pos, 1), 0.25, 2.0, ignore_index=-1, saved_bits=bits[0])
 
         criterion.calc_cls_loss_with_ignore = calc_cls_loss_with_ignore
 
@@ -354,6 +372,7 @@ def detach(criterion: torch.nn.Module) -> None:
         for h in hooks:
             h.remove()
         criterion._detr_amd_hooks = None
+        criterion._detr_amd_saved_bits = None
         for name in ("calc_box_loss", "_get_src_permutation_idx", "calc_cls_loss", "calc_cls_loss_with_ignore"):
             if name in criterion.__dict__:
                 del criterion.__dict__[name]       # the class's own method shows again

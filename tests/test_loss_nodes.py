@@ -67,6 +67,74 @@ class FocalLoss(torch.nn.Module):
         return "own"
 
 
+class Criterion(torch.nn.Module):
+    def __init__(self):
+        super().__init__()
+        import detr_amd
+
+        self.matcher = detr_amd.HungarianMatcher()
+        self.cls_criterion = FocalLoss()
+        self.n_cls = 6
+
+    def calc_cls_loss_with_ignore(self, outputs, targets, pos_indices, neg_indices):
+        return "own"
+
+    def forward(self, outputs, targets):
+        return None
+
+
+def bits_of(monkeypatch, c):
+    """The saved_bits that the two classification losses of an attached criterion are called with."""
+    got = []
+    monkeypatch.setattr(losses, "_takes", lambda *a, **k: True)
+    monkeypatch.setattr(losses, "focal_loss", lambda *a, saved_bits=32, **k: got.append(saved_bits))
+    c.cls_criterion(torch.zeros(2, 3, 6), torch.zeros(2, 3, dtype=torch.int64), 1)
+    none = [(torch.zeros(0, dtype=torch.int64),) * 2] * 2
+    c.calc_cls_loss_with_ignore({"pred_logits": torch.zeros(2, 3, 6)}, [], none, [torch.zeros(0, dtype=torch.int64)] * 2)
+    monkeypatch.undo()
+    return got
+
+
+def test_a_second_attach_with_other_bits(monkeypatch):
+    for first, second in ((32, 8), (8, 32), (8, 8)):
+        c = Criterion()
+        criterion.attach(c, fused_consumers=True, saved_bits=first)
+        assert bits_of(monkeypatch, c) == [first, first]
+        criterion.attach(c, fused_consumers=True, saved_bits=second)
+        assert bits_of(monkeypatch, c) == [second, second]
+        criterion.attach(c)                                # (asks for nothing: nothing changes)
+        assert bits_of(monkeypatch, c) == [second, second]
+        criterion.detach(c)
+        assert c.cls_criterion(None, None, None) == "own" and c.calc_cls_loss_with_ignore(None, None, None, None) == "own"
+
+
+def test_bits_without_the_fused_consumers_are_refused():
+    c = Criterion()
+    criterion.attach(c)
+    with pytest.raises(ValueError, match="detach"):
+        criterion.attach(c, fused_consumers=True, saved_bits=8)
+    criterion.attach(c, fused_consumers=True)              # (as before: harmless)
+    criterion.detach(c)
+    criterion.attach(c, fused_consumers=True, saved_bits=8)
+    assert "forward" in c.cls_criterion.__dict__
+
+
+def test_fusing_a_module_again(monkeypatch):
+    got = []
+    module = FocalLoss()
+    for bits in (32, 8, 32):
+        assert criterion.fuse_cls_criterion(module, saved_bits=bits)
+        monkeypatch.setattr(losses, "_takes", lambda *a, **k: True)
+        monkeypatch.setattr(losses, "focal_loss", lambda *a, saved_bits=32, **k: got.append(saved_bits))
+        module(torch.zeros(2, 3, 6), torch.zeros(2, 3, dtype=torch.int64), 1)
+        monkeypatch.undo()
+    assert got == [32, 8, 32]
+    other = FocalLoss()
+    other.forward = lambda *a: "somebody else's"
+    assert criterion.fuse_cls_criterion(other)
+    assert not criterion.fuse_cls_criterion(other, saved_bits=8) and other() == "somebody else's"
+
+
 def test_a_gamma_below_zero_stays_with_the_module():
     module = FocalLoss()
     module.gamma = -0.5
