@@ -42,7 +42,7 @@ NODES_SRC = os.path.join(CSRC, "loss_nodes.cpp")
 NODES = os.path.join(PKG, "_loss_nodes.so")
 
 
-def build_helper(force=False, verbose=False, src=HELPER_SRC, out=HELPER, what="index_views", flags=()):
+def build_helper(force=False, verbose=False, src=HELPER_SRC, out=HELPER, what="index_views", flags=(), libs=()):
     """A host-side module of plain C++ against the torch headers (no GPU code): detr_amd._index_views (bulk creation of the
     per-image index views) or, through `build_nodes`, detr_amd._loss_nodes."""
     import sysconfig
@@ -64,7 +64,7 @@ def build_helper(force=False, verbose=False, src=HELPER_SRC, out=HELPER, what="i
            '-DDM_BUILT_FOR_TORCH="%s"' % torch.__version__, *flags]
     for inc in cpp_extension.include_paths() + [sysconfig.get_paths()["include"]]:
         cmd += ["-I", inc]
-    cmd += [src, "-o", out, "-L", libdir, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip",
+    cmd += [src, "-o", out, "-L", libdir, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", *libs,
             "-Wl,-rpath," + libdir]
     if verbose:
         print(" ".join(cmd))
@@ -77,7 +77,8 @@ def build_nodes(force=False, verbose=False):
     rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
     return build_helper(force, verbose, NODES_SRC, NODES, "loss_nodes",
                         ["-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_EXTENSION_NAME=_loss_nodes", "-I",
-                         os.path.join(ROOT, "include"), "-I", os.path.join(rocm, "include")])
+                         os.path.join(ROOT, "include"), "-I", os.path.join(rocm, "include")],
+                        ["-lc10_hip", "-lamdhip64"])
 
 
 DEMO_SRC = os.path.join(ROOT, "tests", "c_abi", "abi_demo.c")

@@ -10,6 +10,8 @@
 // No GPU code: the kernels are reached through the addresses of libdetr_match.so's entry points, handed over once by `bind`.
 // Built against one torch version, which the module names (`built_for_torch`); the Python code refuses it under any other.
 #include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
+#include <c10/hip/HIPGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -359,6 +361,26 @@ Tensor cross_entropies(const std::vector<Tensor> &logits, const std::vector<Tens
     return cls_losses(logits, maps, weight, ClsCall{true, 0.0, 0.0, {}, ignore_index, false}, scalar, status);
 }
 
+// ---- the status word of a call inside a capture ----
+
+// An int32 zero that is no part of the graph that the current stream captures: neither its memory nor its clearing.  From a
+// stream that captures nothing (of the pool that the capturing one may itself be of), while this thread may allocate and wait.
+Tensor zero_word_outside_capture(int64_t device_index)
+{
+    const auto index = static_cast<c10::DeviceIndex>(device_index);
+    const c10::hip::HIPGuard device(index);
+    c10::hip::HIPStreamCaptureModeGuard relaxed(hipStreamCaptureModeRelaxed);
+    for (int tries = 0; tries < 64; ++tries) {
+        const c10::hip::HIPStream stream = c10::hip::getStreamFromPool(/*isHighPriority=*/false, index);
+        const c10::hip::HIPStreamGuard on(stream);
+        if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None) continue;
+        const Tensor word = at::zeros({1}, at::TensorOptions().dtype(at::kInt).device(at::kCUDA, index));
+        stream.synchronize();
+        return word;
+    }
+    TORCH_CHECK(false, "detr_amd.losses: no stream outside the capture");
+}
+
 // ---- the balance loss of expert routers ----
 
 struct RouterCall {
@@ -600,4 +622,5 @@ PYBIND11_MODULE(_loss_nodes, m)
     m.def("cross_entropies", torch::wrap_pybind_function(&cross_entropies));
     m.def("balance_losses", torch::wrap_pybind_function(&balance_losses));
     m.def("expert_counts", torch::wrap_pybind_function(&expert_counts));
+    m.def("zero_word_outside_capture", torch::wrap_pybind_function(&zero_word_outside_capture));
 }

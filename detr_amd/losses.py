@@ -254,9 +254,12 @@ def _status_word(device):
     index = device.index if device.index is not None else torch.cuda.current_device()
     status = _cls_status.get(index)
     if status is None:
-        status = torch.zeros(1, dtype=torch.int32, device=device)
-        if not torch.cuda.is_current_stream_capturing():
-            torch.cuda.current_stream(device).synchronize()          # once: other streams' kernels write it too
+        # once, and done when this returns: other streams' kernels write it too, and a graph's replays must not clear it
+        if torch.cuda.is_current_stream_capturing():
+            status = _loss_nodes().zero_word_outside_capture(index)
+        else:
+            status = torch.zeros(1, dtype=torch.int32, device=device)
+            torch.cuda.current_stream(device).synchronize()
         _cls_status[index] = status
     return status
 

@@ -154,3 +154,45 @@ def test_forward_mode_and_tracing_are_refused(name):
         torch.jit.trace(counts, (x,), check_trace=False)
     with fw.dual_level():                # (whole numbers have no tangent)
         assert torch.equal(counts(fw.make_dual(x, torch.ones_like(x))), counts(x))
+
+
+@pytest.mark.parametrize("name", ["focal32", "focal", "balance"])
+def test_first_call_inside_a_capture(name):
+    """The word that findings are reported in is neither part of the graph nor cleared by its replays."""
+    x, cls = data()
+    fn = {"focal32": lambda: losses.focal_loss(x, cls, 3.0), "focal": lambda: losses.focal_loss(x, cls, 3.0, saved_bits=8),
+          "balance": lambda: losses.balance_losses(x, 2).balance}[name]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        want = fn().clone()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    index = torch.cuda.current_device()
+    word = losses._cls_status.pop(index)
+    try:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = fn()
+        losses.check_cls_status()
+        good = cls.clone()
+        cls[0, 0] = 99
+        losses.focal_loss(x, cls, 3.0)
+        losses.focal_loss(x, cls, 3.0, saved_bits=8)
+        cls.copy_(good)
+        for _ in range(3):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
+        with pytest.raises(RuntimeError):
+            losses.check_cls_status()
+        graph.replay()
+        losses.check_cls_status()
+        if name != "balance":            # what the graph's own kernels find is reported as well
+            cls[0, 0] = 99
+            graph.replay()
+            with pytest.raises(RuntimeError):
+                losses.check_cls_status()
+        assert losses._cls_status[index] is not word
+    finally:
+        losses._cls_status[index] = word
