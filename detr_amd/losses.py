@@ -267,6 +267,10 @@ def _status_word(device):
 def _cls_buffers(device):
     index = device.index if device.index is not None else torch.cuda.current_device()
     stream = torch.cuda.current_stream(device).cuda_stream
+    if torch.cuda.is_current_stream_capturing():
+        # (a graph's own: graphs captured on one stream may be replayed on several at once)
+        partials = torch.empty(_lib.CLS_LOSS_PARTIALS, dtype=torch.float64, device=device)
+        return partials, _status_word(device), stream
     partials = _cls_partials.get((index, stream))
     if partials is None:
         partials = _cls_partials[(index, stream)] = torch.empty(_lib.CLS_LOSS_PARTIALS, dtype=torch.float64, device=device)

@@ -196,3 +196,50 @@ def test_first_call_inside_a_capture(name):
         assert losses._cls_status[index] is not word
     finally:
         losses._cls_status[index] = word
+
+
+@pytest.mark.parametrize("kind", ["focal", "ce"])
+def test_captured_graphs_share_no_workspace(kind, monkeypatch):
+    """The 32-bit losses in two graphs that were captured on one stream: their partial sums lie apart, and apart from those of
+    eager calls, so that replays on two streams do not meet."""
+    x, cls = data(B=64, Q=900)
+    name = "dm_focal_loss_f32" if kind == "focal" else "dm_cross_entropy_f32"
+    real, used = getattr(losses.lib, name), []
+
+    class Spy:
+        def __getattr__(self, n):
+            return getattr(lib, n)
+
+    def spy(*args):
+        used.append(args[-3])
+        return real(*args)
+
+    lib = losses.lib
+    setattr(Spy, name, staticmethod(spy))
+    monkeypatch.setattr(losses, "lib", Spy())
+    xs = [x.clone(), x.clone() * 0.5]
+
+    def fn(x):
+        return losses.focal_loss(x, cls, 3.0) if kind == "focal" else losses.cross_entropy(x, cls)
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        want = [fn(x).clone() for x in xs]
+    torch.cuda.synchronize()
+    del used[:]
+    graphs, outs = [], []
+    for x in xs:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            outs.append(fn(x))
+        graphs.append(graph)
+    assert len(set(used)) == 2 and not set(used) & {p.data_ptr() for p in losses._cls_partials.values()}
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(5):
+        for graph, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for got, value in zip(outs, want):
+            assert torch.equal(got, value)
