@@ -194,7 +194,7 @@ __global__ __launch_bounds__(CLS_THREADS) void focal_saved_kernel(const T *__res
     const unsigned blocks = n / BLOCK, stride = gridDim.x * BLOCKS_AT_A_TIME;      // whole blocks
     const unsigned sub = threadIdx.x & (LANES - 1), lane = threadIdx.x & 63;
     const float alpha1 = fp.alpha >= 0.0f ? fp.alpha : 1.0f, alpha0 = fp.alpha >= 0.0f ? 1.0f - fp.alpha : 1.0f;
-    float acc = 0.0f;
+    double acc = 0.0;                // (in 64 bits from block to block: a lane may walk hundreds of equal ones)
     bool bad = false;
 
     // a block with its logits and rows; whole: all 128 are there
@@ -233,7 +233,7 @@ __global__ __launch_bounds__(CLS_THREADS) void focal_saved_kernel(const T *__res
             high = dm::max3(dm::max3(high, c[4 * q], c[4 * q + 1]), c[4 * q + 2], c[4 * q + 3]);
             sum += (term[0] + term[1]) + (term[2] + term[3]);
         }
-        acc += sum;
+        acc += (double)sum;
         if (!codes) return;
         if (dropped) {
             low = FOCAL_CLAMP;
@@ -300,7 +300,7 @@ __global__ __launch_bounds__(CLS_THREADS) void focal_saved_kernel(const T *__res
         work(blocks, v, rows_of, false);
     }
     if (bad) dm::raise_status(status, DM_ST_LABEL_RANGE);
-    const double total = block_sum((double)acc, lds);
+    const double total = block_sum(acc, lds);
     if (threadIdx.x == 0) {
         if (gridDim.x == 1) loss_out[0] = (float)(total * (double)fp.scale);
         else partials[blockIdx.x] = total;
@@ -417,7 +417,7 @@ __global__ __launch_bounds__(CLS_THREADS) void ce_saved_kernel(const void *__res
     constexpr unsigned ROWS = CLS_THREADS / L;
     const unsigned stride = gridDim.x * ROWS;
     const float inf = __builtin_huge_valf();
-    float num = 0.0f, den = 0.0f;
+    double num = 0.0, den = 0.0;     // (a lane may walk thousands of rows, and equal ones round to the same side)
     bool bad = false;
     dm::RawRow<NQ, WIDE> next;
     int64_t next_y = 0;
@@ -457,8 +457,8 @@ __global__ __launch_bounds__(CLS_THREADS) void ce_saved_kernel(const void *__res
         for (int j = 0; j < N; ++j) sum += __builtin_amdgcn_exp2f((v[j] - mx) * LOG2E);      // (past the row: exp2(-inf) = 0)
         sum = dm::over_group<L>(sum, dm::Add());
         if (sub == 0 && w != 0.0f) {
-            num += w * ((mx + __builtin_amdgcn_logf(sum) * LN2) - own);
-            den += w;
+            num += (double)(w * ((mx + __builtin_amdgcn_logf(sum) * LN2) - own));
+            den += (double)w;
         }
         if (!codes) continue;
         const float high = __builtin_amdgcn_fmed3f(mx, -CE_CLAMP, CE_CLAMP);
@@ -483,8 +483,8 @@ __global__ __launch_bounds__(CLS_THREADS) void ce_saved_kernel(const void *__res
         if (sub == 0 && live) steps[row] = (int8_t)(sum == sum ? e : NOT_A_NUMBER);
     }
     if (bad) dm::raise_status(status, DM_ST_LABEL_RANGE);
-    const double a = block_sum((double)num, lds);
-    const double b = block_sum((double)den, lds);
+    const double a = block_sum(num, lds);
+    const double b = block_sum(den, lds);
     if (threadIdx.x == 0) ce_sums(a, b, partials, loss_out);
 }
 

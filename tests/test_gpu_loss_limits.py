@@ -46,6 +46,37 @@ def test_gradient_of_infinite_logits_with_sigmoid_scores(E, dtype, per_image):
     assert (off <= bound).all(), float((off / bound).max())
 
 
+def test_sums_of_very_many_equal_rows_cross_entropy():
+    """2730 rows a lane, all of weight 0.1: added up in float32 they would be off by 450 u, each rounding to the same side.
+    A row's loss is log 2: the constant, the product with the weight and three roundings of the sums' ends, and the hardware's
+    logarithm to a step: 16 u; the sum of the weights three roundings."""
+    rows = 1536 * 256 * 2730
+    assert 2 * rows < 1 << 31
+    x = torch.zeros(rows, 2, dtype=torch.bfloat16, device="cuda")
+    cls = torch.zeros(rows, dtype=torch.int64, device="cuda")
+    weight = torch.full((2,), 0.1, device="cuda")
+    out = torch.zeros(2, device="cuda")
+    partials = torch.empty(_lib.CLS_LOSS_PARTIALS, dtype=torch.float64, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    rc = lib.dm_cross_entropy_saved(x.data_ptr(), 1, cls.data_ptr(), weight.data_ptr(), rows, 2, -100, out.data_ptr(), None, None,
+                                    partials.data_ptr(), status.data_ptr(), torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    loss, inverse = out.tolist()
+    assert abs(inverse * rows * float(np.float32(0.1)) - 1) <= 4 * U
+    assert abs(loss / math.log(2) - 1) <= 16 * U
+
+
+def test_sums_of_very_many_equal_logits_focal():
+    """341 times 16 logits a lane, all 0: each is 0.75 log 2 / 4 (1/x and the logarithm to a step, six products), a lane's 16 are
+    added in float32 (at most six roundings), the rest in 64 bits: 16 u, where a float32 sum would be off by 43 u."""
+    n = 1534 * 4096 * 341
+    assert n < 1 << 31
+    x = torch.zeros(n // 2, 2, dtype=torch.bfloat16, device="cuda")
+    cls = torch.full((n // 2,), 2, dtype=torch.int64, device="cuda")
+    loss = losses.focal_loss(x, cls, float(n), saved_bits=8).item()
+    assert abs(loss / (0.75 * math.log(2) / 4) - 1) <= 20 * U
+
+
 def test_a_gamma_below_zero_is_refused():
     x = torch.randn(3, 7, 5, device="cuda")
     cls = torch.zeros(3, 7, dtype=torch.int64, device="cuda")
