@@ -8,7 +8,8 @@
 // stored less one (the p of a row sum to one, so a constant drops out): near balance f_e - sum f p would lose its digits.
 //
 // Forward: workgroups walk chunks of an image's rows, a group of lanes per row; sums over rows stay in registers of the
-// lane that owns the expert, and leave once per workgroup, into a slot of the workspace.  A second kernel adds the slots in
+// lane that owns the expert (in float32 for RUN rows, then they go to 64 bits in shared memory), and leave once per workgroup,
+// into a slot of the workspace.  A second kernel adds the slots in
 // index order in 64 bits: no float atomics, the same bits every run.  A group that one workgroup walks needs no second kernel.
 //
 // What bounds it, as measured (a copy of a GiB runs at 5.1 TB/s, a kernel of a few workgroups takes 4 us among others):
@@ -30,6 +31,7 @@ namespace {
 constexpr int RT_THREADS = 256;
 constexpr int RT_WAVES = RT_THREADS / 64;
 constexpr int RT_MAX_EXPERTS = 1024;
+constexpr unsigned RUN = 64;         // rows whose scores a lane adds in float32: equal ones round to the same side
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 // One set as the kernels see it: `images` images of Q rows (a contiguous set asked for as one group is one image of B * Q
@@ -286,13 +288,15 @@ __global__ __launch_bounds__(RT_THREADS) void router_forward_kernel(const Router
     constexpr int PARTS = L <= 16 ? 4 : 64 / L;                // partial sums of p that a wave leaves
     constexpr unsigned WIDTH = N * L;                          // E, rounded up to what the lanes hold
     __shared__ unsigned hist[WIDTH];
-    __shared__ float psum_lds[COUNT_ONLY ? 1 : RT_WAVES * PARTS][COUNT_ONLY ? 1 : WIDTH];
+    __shared__ double psum_lds[COUNT_ONLY ? 1 : RT_WAVES * PARTS][COUNT_ONLY ? 1 : WIDTH];
     __shared__ double z_lds[RT_WAVES];
     __shared__ unsigned n_lds[RT_WAVES];
     __shared__ LossSums loss_lds;
     const unsigned E = a.E, k = a.k;
     const float ninf = -__builtin_huge_valf();
     for (unsigned e = threadIdx.x; e < WIDTH; e += RT_THREADS) hist[e] = 0;
+    if constexpr (!COUNT_ONLY)
+        for (unsigned i = threadIdx.x; i < RT_WAVES * PARTS * WIDTH; i += RT_THREADS) psum_lds[0][i] = 0.0;
     __syncthreads();
 
     const Place at = place_of(a, blockIdx.x);
@@ -304,7 +308,7 @@ __global__ __launch_bounds__(RT_THREADS) void router_forward_kernel(const Router
     constexpr unsigned ROWS = RT_THREADS / L;                  // rows of the workgroup at a time
     float psum[N] = {};
     unsigned cnt[N] = {};
-    float z = 0.0f;
+    double z = 0.0;
     unsigned n = 0;
     bool bad = false;
 
@@ -318,150 +322,164 @@ __global__ __launch_bounds__(RT_THREADS) void router_forward_kernel(const Router
         if (set.mask) next_counts = set.mask[image_row + row];
     };
     if (at.rows) fetch(local);
-    for (unsigned r0 = 0; r0 < at.rows; r0 += ROWS) {
-        const unsigned r = r0 + local;
-        const bool there = r < at.rows;
-        const size_t row = (size_t)at.row0 + (there ? r : 0);
-        dm::RawRow<NQ, WIDE> raw = next;
-        const bool counts = there && next_counts != 0;
-        if (r0 + ROWS < at.rows) fetch(r + ROWS);
-        typedef Order<WIDE> O;
-        typename O::Type y[N];
-        bool nan;
-        in_order<NQ, L>(raw, dtype, sub, E, counts, y, &nan);
-        constexpr int PLACES = K < N ? K : N;
-        typename O::Type list[PLACES];
+    unsigned r0 = 0, run = 0;
+    do {
+        run = COUNT_ONLY ? at.rows : min(at.rows, r0 + RUN * ROWS);
+        for (; r0 < run; r0 += ROWS) {
+            const unsigned r = r0 + local;
+            const bool there = r < at.rows;
+            const size_t row = (size_t)at.row0 + (there ? r : 0);
+            dm::RawRow<NQ, WIDE> raw = next;
+            const bool counts = there && next_counts != 0;
+            if (r0 + ROWS < at.rows) fetch(r + ROWS);
+            typedef Order<WIDE> O;
+            typename O::Type y[N];
+            bool nan;
+            in_order<NQ, L>(raw, dtype, sub, E, counts, y, &nan);
+            constexpr int PLACES = K < N ? K : N;
+            typename O::Type list[PLACES];
 #pragma unroll
-        for (int i = 0; i < PLACES; ++i) list[i] = O::never();
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-#pragma unroll
-            for (int i = PLACES - 1; i >= 1; --i)
-                if (i <= j) list[i] = dm::median(list[i - 1], list[i], y[j]);      // (place j is empty before the j-th)
-            list[0] = j ? dm::median(list[0], y[j], O::above_all()) : y[0];
-        }
-        const typename O::Type top = dm::largest<L>(list[0]);
-        if (COUNT_ONLY || !set.experts) {
-            typename O::Type last = O::never();
-            if (L == 1) {
-#pragma unroll
-                for (int i = 0; i < PLACES; ++i) last = i + 1 == (int)k ? list[i] : last;
-            } else {
-                last = top;
-                // the heads that equal `last` off their lists, as far as `places`, and the largest head that is left (the median of a
-                // place, the next and the least is the next, of the largest the place itself)
-                auto next_largest = [&](int places) {
-                    const typename O::Type gone = list[0] == last ? O::never() : O::above_all();
-#pragma unroll
-                    for (int j = 0; j < PLACES; ++j)
-                        if (j < places) list[j] = dm::median(list[j], j + 1 < PLACES ? list[j + 1] : O::never(), gone);
-                    last = dm::largest<L>(list[0]);
-                };
-                if (K == 16 && k > 16) {
-                    for (unsigned i = 1; i < k; ++i) next_largest(PLACES);
-                } else {
-#pragma unroll
-                    for (int i = 1; i < K; ++i)
-                        if (i < (int)k) next_largest(K - i);       // (what could come up after the k-th is not moved any more)
-                }
-            }
-            last = max(last, O::least(dtype));                 // (fewer than k: all that can be)
-            unsigned chosen = 0;
+            for (int i = 0; i < PLACES; ++i) list[i] = O::never();
 #pragma unroll
             for (int j = 0; j < N; ++j) {
-                const unsigned one = y[j] >= last ? 1u : 0u;
-                cnt[j] += one;
-                if (WIDE) chosen += one;
+#pragma unroll
+                for (int i = PLACES - 1; i >= 1; --i)
+                    if (i <= j) list[i] = dm::median(list[i - 1], list[i], y[j]);      // (place j is empty before the j-th)
+                list[0] = j ? dm::median(list[0], y[j], O::above_all()) : y[0];
             }
-            if (WIDE) chosen = dm::over_group<L>(chosen, dm::Add());
-            if (WIDE && __any(chosen > k)) {
+            const typename O::Type top = dm::largest<L>(list[0]);
+            if (COUNT_ONLY || !set.experts) {
+                typename O::Type last = O::never();
+                if (L == 1) {
 #pragma unroll
-                for (int j = 0; j < N; ++j) cnt[j] -= y[j] >= last ? 1u : 0u;
-                // k times the largest that is left, of the lowest expert that has it
-                typename O::Type left[N];
+                    for (int i = 0; i < PLACES; ++i) last = i + 1 == (int)k ? list[i] : last;
+                } else {
+                    last = top;
+                    // the heads that equal `last` off their lists, as far as `places`, and the largest head that is left (the median of a
+                    // place, the next and the least is the next, of the largest the place itself)
+                    auto next_largest = [&](int places) {
+                        const typename O::Type gone = list[0] == last ? O::never() : O::above_all();
 #pragma unroll
-                for (int j = 0; j < N; ++j) left[j] = y[j];
-                for (unsigned i = 0; i < k; ++i) {
-                    typename O::Type best = O::never();
+                        for (int j = 0; j < PLACES; ++j)
+                            if (j < places) list[j] = dm::median(list[j], j + 1 < PLACES ? list[j + 1] : O::never(), gone);
+                        last = dm::largest<L>(list[0]);
+                    };
+                    if (K == 16 && k > 16) {
+                        for (unsigned i = 1; i < k; ++i) next_largest(PLACES);
+                    } else {
 #pragma unroll
-                    for (int j = 0; j < N; ++j) best = dm::median(best, left[j], O::above_all());
-                    best = dm::largest<L>(best);
-                    unsigned first = 0xFFFFFFFFu;
+                        for (int i = 1; i < K; ++i)
+                            if (i < (int)k) next_largest(K - i);       // (what could come up after the k-th is not moved any more)
+                    }
+                }
+                last = max(last, O::least(dtype));                 // (fewer than k: all that can be)
+                unsigned chosen = 0;
 #pragma unroll
-                    for (int j = N - 1; j >= 0; --j)
-                        if (left[j] == best) first = (unsigned)(4 * ((j >> 2) * L + sub) + (j & 3));
-                    first = dm::over_group<L>(first, dm::Min());
-                    if (best < O::least(dtype)) first = 0xFFFFFFFFu;
+                for (int j = 0; j < N; ++j) {
+                    const unsigned one = y[j] >= last ? 1u : 0u;
+                    cnt[j] += one;
+                    if (WIDE) chosen += one;
+                }
+                if (WIDE) chosen = dm::over_group<L>(chosen, dm::Add());
+                if (WIDE && __any(chosen > k)) {
 #pragma unroll
-                    for (int j = 0; j < N; ++j) {
-                        const bool hit = first == (unsigned)(4 * ((j >> 2) * L + sub) + (j & 3));
-                        cnt[j] += hit ? 1u : 0u;
-                        left[j] = hit ? O::never() : left[j];
+                    for (int j = 0; j < N; ++j) cnt[j] -= y[j] >= last ? 1u : 0u;
+                    // k times the largest that is left, of the lowest expert that has it
+                    typename O::Type left[N];
+#pragma unroll
+                    for (int j = 0; j < N; ++j) left[j] = y[j];
+                    for (unsigned i = 0; i < k; ++i) {
+                        typename O::Type best = O::never();
+#pragma unroll
+                        for (int j = 0; j < N; ++j) best = dm::median(best, left[j], O::above_all());
+                        best = dm::largest<L>(best);
+                        unsigned first = 0xFFFFFFFFu;
+#pragma unroll
+                        for (int j = N - 1; j >= 0; --j)
+                            if (left[j] == best) first = (unsigned)(4 * ((j >> 2) * L + sub) + (j & 3));
+                        first = dm::over_group<L>(first, dm::Min());
+                        if (best < O::least(dtype)) first = 0xFFFFFFFFu;
+#pragma unroll
+                        for (int j = 0; j < N; ++j) {
+                            const bool hit = first == (unsigned)(4 * ((j >> 2) * L + sub) + (j & 3));
+                            cnt[j] += hit ? 1u : 0u;
+                            left[j] = hit ? O::never() : left[j];
+                        }
                     }
                 }
             }
+            if constexpr (!COUNT_ONLY) {
+                // the scores, of the logits as they came
+                const float mx = top < O::least(dtype) ? 0.0f : O::logit(top, dtype);
+                float x[N];
+                if constexpr (WIDE) {
+#pragma unroll
+                    for (int j = 0; j < N; ++j) x[j] = y[j];
+                } else {
+                    dm::raw_values<NQ, WIDE>(raw, dtype, x);
+                }
+                float sum = nan ? __builtin_nanf("") : 0.0f;
+                if (sigmoid) {
+                    float none[1];
+                    sigmoid_weights<N, false>(x, mx, none);
+                } else {
+                    softmax_weights(x, mx);
+                }
+#pragma unroll
+                for (int j = 0; j < N; ++j) sum += x[j];
+                sum = dm::over_group<L>(sum, dm::Add());
+                const bool live = sum != 0.0f;                     // (a NaN makes it NaN)
+                const float inv = live ? __builtin_amdgcn_rcpf(sum) : 0.0f;
+#pragma unroll
+                for (int j = 0; j < N; ++j) psum[j] = __builtin_fmaf(x[j], inv, psum[j]);
+                if (live && sub == 0) {
+                    const float lse = mx + __builtin_amdgcn_logf(sum) * LN2;
+                    z += (double)lse * (double)lse;
+                    ++n;
+                }
+                if (set.experts && live)
+                    for (unsigned j = sub; j < k; j += L) {
+                        const int64_t e = set.experts[(image_row + row) * k + j];
+                        if (e >= 0 && e < (int64_t)E) atomicAdd(&hist[(unsigned)e], 1u);
+                        else bad |= e != -1;
+                    }
+            }
         }
         if constexpr (!COUNT_ONLY) {
-            // the scores, of the logits as they came
-            const float mx = top < O::least(dtype) ? 0.0f : O::logit(top, dtype);
-            float x[N];
-            if constexpr (WIDE) {
+            // the run's sums of p into the workgroup's: the rows of a wave whose lanes are 16 apart or more have a part each, and every
+            // place of it one lane that writes it
+            unsigned thread = threadIdx.x;
+            asm("" : "+v"(thread));                                // (or places are worked out before the walk, and kept in registers)
+            double *part = psum_lds[thread / (L <= 16 ? 16 : L)] + 4 * (thread & (L - 1));
 #pragma unroll
-                for (int j = 0; j < N; ++j) x[j] = y[j];
-            } else {
-                dm::raw_values<NQ, WIDE>(raw, dtype, x);
+            for (int j = 0; j < N; ++j) {
+                if (L <= 16) psum[j] = dm::over_row16<L>(psum[j]);
             }
-            float sum = nan ? __builtin_nanf("") : 0.0f;
-            if (sigmoid) {
-                float none[1];
-                sigmoid_weights<N, false>(x, mx, none);
-            } else {
-                softmax_weights(x, mx);
+            if ((thread & 15) < L || L > 16) {
+                // (one instruction without an answer to wait for; nobody else adds to the place)
+#pragma unroll
+                for (int j = 0; j < N; ++j)
+                    __hip_atomic_fetch_add(part + 4 * (j >> 2) * L + (j & 3), (double)psum[j], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
             }
 #pragma unroll
-            for (int j = 0; j < N; ++j) sum += x[j];
-            sum = dm::over_group<L>(sum, dm::Add());
-            const bool live = sum != 0.0f;                     // (a NaN makes it NaN)
-            const float inv = live ? __builtin_amdgcn_rcpf(sum) : 0.0f;
-#pragma unroll
-            for (int j = 0; j < N; ++j) psum[j] = __builtin_fmaf(x[j], inv, psum[j]);
-            if (live && sub == 0) {
-                const float lse = mx + __builtin_amdgcn_logf(sum) * LN2;
-                z += lse * lse;
-                ++n;
-            }
-            if (set.experts && live)
-                for (unsigned j = sub; j < k; j += L) {
-                    const int64_t e = set.experts[(image_row + row) * k + j];
-                    if (e >= 0 && e < (int64_t)E) atomicAdd(&hist[(unsigned)e], 1u);
-                    else bad |= e != -1;
-                }
+            for (int j = 0; j < N; ++j) psum[j] = 0.0f;
         }
-    }
+    } while (r0 < at.rows);
     if (bad) dm::raise_status(status, DM_ST_LABEL_RANGE);
 
-    // the rows of a wave whose lanes are 16 apart or more leave a part each; the parts are added in order
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-        const unsigned e = 4 * ((j >> 2) * L + sub) + (j & 3);
-        if (L <= 16) {
-            cnt[j] = dm::over_row16<L>(cnt[j]);
-            if (!COUNT_ONLY) psum[j] = dm::over_row16<L>(psum[j]);
-        }
-        if ((lane & 15) < L || L > 16) {
-            if (!COUNT_ONLY) psum_lds[wave * PARTS + lane / (L <= 16 ? 16 : L)][e] = psum[j];
-            if (cnt[j]) atomicAdd(&hist[e], cnt[j]);
-        }
+        if (L <= 16) cnt[j] = dm::over_row16<L>(cnt[j]);
+        if (((lane & 15) < L || L > 16) && cnt[j]) atomicAdd(&hist[4 * ((j >> 2) * L + sub) + (j & 3)], cnt[j]);
     }
-    double zd = z;
     if (!COUNT_ONLY) {
 #pragma unroll
         for (int off = 32; off >= 1; off >>= 1) {
-            zd += __shfl_xor(zd, off);
+            z += __shfl_xor(z, off);
             n += __shfl_xor(n, off);
         }
         if (lane == 0) {
-            z_lds[wave] = zd;
+            z_lds[wave] = z;
             n_lds[wave] = n;
         }
     }
@@ -480,10 +498,10 @@ __global__ __launch_bounds__(RT_THREADS) void router_forward_kernel(const Router
                 counts[j] = (long long)hist[e];
                 out.counts[group * E + e] = counts[j];
                 if (!COUNT_ONLY) {
-                    float s = psum_lds[0][e];
+                    double s = psum_lds[0][e];      // (the parts in order)
 #pragma unroll
                     for (int w = 1; w < RT_WAVES * PARTS; ++w) s += psum_lds[w][e];
-                    sums[j] = (double)s;
+                    sums[j] = s;
                     if (out.given_counts) counts[j] = out.given_counts[group * E + e];
                 }
             }
@@ -497,10 +515,10 @@ __global__ __launch_bounds__(RT_THREADS) void router_forward_kernel(const Router
     unsigned *slot = slots + (size_t)blockIdx.x * slot_words(E);
     for (unsigned e = threadIdx.x; e < E; e += RT_THREADS) {
         if (!COUNT_ONLY) {
-            float s = psum_lds[0][e];
+            double s = psum_lds[0][e];
 #pragma unroll
             for (int w = 1; w < RT_WAVES * PARTS; ++w) s += psum_lds[w][e];
-            slot[e] = __float_as_uint(s);
+            slot[e] = __float_as_uint((float)s);
         }
         slot[E + e] = hist[e];
     }

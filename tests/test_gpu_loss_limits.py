@@ -77,6 +77,37 @@ def test_sums_of_very_many_equal_logits_focal():
     assert abs(loss / (0.75 * math.log(2) / 4) - 1) <= 20 * U
 
 
+def test_sums_of_very_many_equal_rows_balance():
+    """2731 rows a lane, the same row: a lane's float32 runs are 64 rows long, beyond that sums are of 64 bits.  A score 1/10 is
+    good to a step and the product's rounding, so balance = 1 to (64 + 8) u; log 10 to 5 u (its logarithm to a step, constant,
+    product, sum), twice in the square: 12 u.  In float32 throughout both were off by 450 u."""
+    B, Q, E = 48, 256 * 2731, 10
+    long = torch.zeros(B, Q, E, dtype=torch.bfloat16, device="cuda")
+    short = torch.zeros(B, 1, E, dtype=torch.bfloat16, device="cuda")
+    out = losses.balance_losses([short] * 7 + [long] + [short] * 8, 2, per_image=True)
+    for s in (7, 0):
+        assert float((out.balance[s].double() - 1).abs().max()) <= 72 * U
+        assert float((out.z[s].double() / math.log(10) ** 2 - 1).abs().max()) <= 14 * U
+    assert out.counts[7].unique().tolist() == [0, Q] and out.counts[7].sum().item() == 2 * B * Q
+
+
+@pytest.mark.parametrize("E", [9, 30, 100, 300, 600])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_runs_of_rows_in_a_lane(E, dtype):
+    """Rows beyond one float32 run of a lane (64), and a run that ends with the rows: with so many images a workgroup each."""
+    lanes = 1 if E <= 16 else 2 if E <= 32 else 8 if E <= 128 else 32 if E <= 512 else 64
+    trip = 256 // lanes
+    for Q in (64 * trip, 64 * trip + 1, 131 * trip - 1):
+        gen = torch.Generator().manual_seed(E + Q)
+        x = torch.randn(1, Q, E, generator=gen).to(DTYPES[dtype])
+        long = torch.zeros(48, Q, E, dtype=x.dtype, device="cuda")
+        long[5] = x[0].cuda()
+        short = torch.zeros(48, 1, E, dtype=x.dtype, device="cuda")
+        out = losses.balance_losses([long] + [short] * 15, 2, per_image=True)
+        want = oracle.balance_losses(x.double().numpy(), 2, per_image=True)
+        check_set(x, want, out.balance[0, 5:6], out.z[0, 5:6], out.counts[0, 5:6], None)
+
+
 def test_a_gamma_below_zero_is_refused():
     x = torch.randn(3, 7, 5, device="cuda")
     cls = torch.zeros(3, 7, dtype=torch.int64, device="cuda")
