@@ -492,6 +492,7 @@ struct BalanceNode : LossNode {
         variable_list saved(2 * S + 1);
         if (!any(grads)) return saved;
         for (size_t i = 0; i < S; ++i) {
+            if (!task_should_compute_output(i)) continue;
             saved[2 * i] = logits[i].unpack();
             if (masked[i]) saved[2 * i + 1] = masks[i].unpack();
         }
@@ -511,19 +512,26 @@ struct BalanceNode : LossNode {
         std::vector<Tensor> held(2 * S);
         for (size_t i = 0; i < S; ++i) {
             const Tensor &x = saved[2 * i];
+            if (!x.defined()) continue;
             held[2 * i] = image_stride(x) >= 0 ? x : x.contiguous();
             if (masked[i]) held[2 * i + 1] = saved[2 * i + 1].contiguous();
             result[i] = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
             describe(sets, i, held[2 * i], held[2 * i + 1], Tensor(), &result[i]);
         }
         const float *slope = shares.const_data_ptr<float>();
-        check(g.balance_backward(sets.data(), static_cast<int>(S), static_cast<int>(call.B), static_cast<int>(call.E), call.dtype,
-                                 call.sigmoid, call.per_image, slope, slope + call.groups() * call.E,
-                                 gb.defined() ? gb.const_data_ptr<float>() : nullptr, gz.defined() ? gz.const_data_ptr<float>() : nullptr,
-                                 current_stream(shares.device())),
-              "dm_balance_backward");
-        for (size_t i = 0; i < S; ++i)
-            if (!task_should_compute_output(i)) result[i].reset();
+        const float *inv_rows = slope + call.groups() * call.E;
+        const size_t groups = call.per_image ? call.B : 1;      // of a set
+        // (a call for each run of sets that need a gradient: one, unless some in between need none)
+        for (size_t i = 0, end; i < S; i = end) {
+            end = i + 1;
+            if (!result[i].defined()) continue;
+            while (end < S && result[end].defined()) ++end;
+            check(g.balance_backward(sets.data() + i, static_cast<int>(end - i), static_cast<int>(call.B), static_cast<int>(call.E),
+                                     call.dtype, call.sigmoid, call.per_image, slope + i * groups * call.E, inv_rows + i * groups,
+                                     gb.defined() ? gb.const_data_ptr<float>() + i * groups : nullptr,
+                                     gz.defined() ? gz.const_data_ptr<float>() + i * groups : nullptr, current_stream(shares.device())),
+                  "dm_balance_backward");
+        }
         return result;
     }
 };

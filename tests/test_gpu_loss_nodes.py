@@ -243,3 +243,39 @@ def test_captured_graphs_share_no_workspace(kind, monkeypatch):
         torch.cuda.synchronize()
         for got, value in zip(outs, want):
             assert torch.equal(got, value)
+
+
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("per_image", [False, True])
+def test_routers_that_need_no_gradient_are_left_out(scores, per_image):
+    """The gradients of the others are the same, and nothing is allocated for a set that needs none."""
+    sets, B, Q, E = 6, 8, 4096, 32
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    xs = [torch.randn(B, Q + 8 * s, E, device="cuda", generator=gen, requires_grad=True) for s in range(sets)]
+    groups = (sets, B) if per_image else (sets,)
+    upstream = torch.rand(groups, device="cuda", generator=gen)
+
+    def value():
+        out = losses.balance_losses(xs, 2, scores=scores, per_image=per_image)
+        return (out.balance * upstream).sum() if out.z is None else (out.balance * upstream).sum() + (out.z * upstream).sum()
+
+    want = torch.autograd.grad(value(), xs)
+    for wanted in ([0], [5], [2, 3], [0, 2, 5], [1, 2, 4]):
+        loss = value()
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        got = torch.autograd.grad(loss, [xs[i] for i in wanted])
+        torch.cuda.synchronize()
+        most = sum(xs[i].numel() * 4 for i in wanted) + (1 << 21)
+        assert torch.cuda.max_memory_allocated() - before <= most
+        for i, g in zip(wanted, got):
+            assert torch.equal(g, want[i])
+        del loss, got
+    # one that is not a leaf's, one that is frozen
+    mixed = [xs[0], xs[1].detach(), xs[2]]
+    out = losses.balance_losses(mixed, 2, scores=scores, per_image=per_image)
+    got = torch.autograd.grad((out.balance * upstream[:3]).sum(), [xs[0], xs[2]])
+    out = losses.balance_losses(xs[:3], 2, scores=scores, per_image=per_image)
+    both = torch.autograd.grad((out.balance * upstream[:3]).sum(), xs[:3])
+    assert torch.equal(got[0], both[0]) and torch.equal(got[1], both[2])
