@@ -148,8 +148,10 @@ struct BlockRows {
                 const unsigned low = (unsigned)label[q][k];
                 high |= (unsigned)((uint64_t)label[q][k] >> 32);
                 largest = max(largest, low);
-                // (a class that is none is nowhere: its row's neighbours in the quad are others')
-                hot[q][k] = (low < C ? (int)low : INT_MIN / 2) + (ONE_CLASS ? (int)k : k ? (int)(C - col[q]) : -(int)col[q]);
+                // (a class that is none is nowhere: its row's neighbours in the quad are others'.  Modulo 2^32, where no other place
+                // comes round to 0 to 3 again: low - col lies between -2^31 and 2^31, low + C - col below 2^32)
+                const unsigned place = low + (ONE_CLASS ? k : k ? C - col[q] : 0u - col[q]);
+                hot[q][k] = low < C ? (int)place : INT_MIN;
             }
         skipped = high != 0 || largest > C;
         if (fp.use_ignore && (uint64_t)fp.ignore_index <= C) {

@@ -108,6 +108,18 @@ def test_runs_of_rows_in_a_lane(E, dtype):
         check_set(x, want, out.balance[0, 5:6], out.z[0, 5:6], out.counts[0, 5:6], None)
 
 
+def test_a_row_of_more_than_2_30_classes():
+    """No class is the row's: every logit is a negative one, its gradient positive."""
+    C = (1 << 30) + 1000
+    x = torch.zeros(1, C, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    for label, hot in ((C, None), (C - 1, C - 1), (5, 5)):
+        cls = torch.full((1,), label, dtype=torch.int64, device="cuda")
+        (grad,) = torch.autograd.grad(losses.focal_loss(x, cls, 1.0, saved_bits=8), x)
+        negative = (grad[0] <= 0).nonzero().flatten().tolist()
+        assert negative == ([] if hot is None else [hot])
+        del grad
+
+
 def test_a_gamma_below_zero_is_refused():
     x = torch.randn(3, 7, 5, device="cuda")
     cls = torch.zeros(3, 7, dtype=torch.int64, device="cuda")
