@@ -623,7 +623,9 @@ def set_loss_total(matcher, outputs_list, targets, n_cls: int, cls_loss: str = "
                    giou_weight: float = 1.0, cls_weight: float = 1.0, focal_alpha: float = 0.25, focal_gamma: float = 2.0,
                    class_weight: Optional[torch.Tensor] = None, reduction: str = "mean", saved_bits: int = 32,
                    router_logits: Optional[Sequence[torch.Tensor]] = None, router_top_k: int = 1, router_mask=None,
-                   balance_weight: float = 0.01, router_z_weight: float = 0.0) -> torch.Tensor:
+                   balance_weight: float = 0.01, router_z_weight: float = 0.0, router_experts=None,
+                   router_counts: Optional[torch.Tensor] = None, router_scores: str = "softmax",
+                   router_per_image: bool = False) -> torch.Tensor:
     """`l1_weight * l1 + giou_weight * giou + cls_weight * cls` over the Hungarian-matched output sets of ONE output group
     as one scalar -- with reduction='mean' what the reference's `calc_total_loss` makes of the group's per-layer losses
     (/root/reference/models/detr/loss.py:135-158: the mean of each kind over the layers, weighted and summed) -- with
@@ -631,7 +633,8 @@ def set_loss_total(matcher, outputs_list, targets, n_cls: int, cls_loss: str = "
     is no longer bound by the host's walk through tiny tensor operations.  `saved_bits`: as in `focal_loss`.
 
     `router_logits`: for a model whose decoder layers have expert blocks, the [B, Q, E] logits of their routers; the
-    `balance_loss_total` of them (`router_top_k`, `router_mask`, `balance_weight`, `router_z_weight`, the group's
+    `balance_loss_total` of them (`router_top_k`, `router_mask`, `balance_weight`, `router_z_weight`, `router_experts`: what
+    the model's own routers chose, `router_counts`: those of all ranks, `router_scores`, `router_per_image`, the group's
     `reduction` over the layers) is added."""
     if reduction not in ("mean", "sum"):
         raise ValueError("reduction must be 'mean' or 'sum'")
@@ -657,5 +660,6 @@ def set_loss_total(matcher, outputs_list, targets, n_cls: int, cls_loss: str = "
     total = box + cls.sum() * (share * cls_weight)
     if router_logits is not None:
         total = total + balance_loss_total(router_logits, router_top_k, balance_weight, router_z_weight, mask=router_mask,
-                                           reduction=reduction)
+                                           experts=router_experts, counts=router_counts, scores=router_scores,
+                                           per_image=router_per_image, reduction=reduction)
     return total

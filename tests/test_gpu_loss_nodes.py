@@ -279,3 +279,25 @@ def test_routers_that_need_no_gradient_are_left_out(scores, per_image):
     out = losses.balance_losses(xs[:3], 2, scores=scores, per_image=per_image)
     both = torch.autograd.grad((out.balance * upstream[:3]).sum(), xs[:3])
     assert torch.equal(got[0], both[0]) and torch.equal(got[1], both[2])
+
+
+def test_what_a_total_takes_of_the_routers():
+    """set_loss_total hands the model's own choice, the counts of all ranks, the scores and the images on to the balance loss."""
+    import detr_amd
+    from detr_amd import synth
+
+    wl, sets, targets = synth.make_workload("cfg2", device="cuda", batch=4)
+    matcher = detr_amd.HungarianMatcher(**wl.matcher_kwargs)
+    gen = torch.Generator().manual_seed(6)
+    Q = sets[0]["pred_logits"].shape[1]
+    routers = [torch.randn(4, Q, 8, generator=gen).cuda() for _ in sets]
+    chosen = [torch.randint(-1, 8, (4, Q, 2), generator=gen).cuda() for _ in sets]
+    plain = losses.set_loss_total(matcher, sets, targets, wl.n_label_classes)
+    for extra in (dict(experts=chosen), dict(counts=torch.randint(1, 50, (len(sets), 8), generator=gen).cuda()),
+                  dict(scores="sigmoid"), dict(per_image=True), dict(per_image=True, scores="sigmoid", experts=chosen)):
+        total = losses.set_loss_total(matcher, sets, targets, wl.n_label_classes, router_logits=routers, router_top_k=2,
+                                      balance_weight=0.5, **{"router_" + k: v for k, v in extra.items()})
+        part = losses.balance_loss_total(routers, 2, 0.5, **extra)
+        # (the sum of the two, rounded once)
+        torch.testing.assert_close(total, plain + part, rtol=2.0 ** -23, atol=0)
+        assert not torch.equal(part, losses.balance_loss_total(routers, 2, 0.5))
