@@ -433,6 +433,8 @@ class FocalLoss(torch.nn.Module):
     apart by their shape -- and `targets` the [B, Q] class map.  Inputs the kernel does not take (not float32, not on
     a GPU, a layout that cannot be told, with 8 bits a gamma below zero) go to `fallback` when one is given.  `saved_bits` as in `focal_loss`."""
 
+    saved_bits = 32        # (of modules that were saved before there was a choice)
+
     def __init__(self, alpha: float, gamma: float, n_cls: int, channels_first: Optional[bool] = None, fallback=None,
                  saved_bits: int = 32):
         super().__init__()
@@ -454,6 +456,8 @@ class FocalLoss(torch.nn.Module):
 class CrossEntropy(torch.nn.Module):
     """Takes the place of the reference's `CrossEntropy(weight)` (/root/reference/models/detr/loss.py:185-195, input
     [B, C, Q]; /root/reference/models/co_detr/loss.py:249-259, input [B, Q, C]).  `saved_bits` as in `cross_entropy`."""
+
+    saved_bits = 32        # (as above)
 
     def __init__(self, weight: Optional[torch.Tensor] = None, channels_first: Optional[bool] = None,
                  ignore_index: int = -100, fallback=None, saved_bits: int = 32):

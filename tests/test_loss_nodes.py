@@ -141,3 +141,11 @@ def test_a_gamma_below_zero_stays_with_the_module():
     criterion.fuse_cls_criterion(module, saved_bits=8)
     assert not losses._takes(torch.zeros(2, 3, 6), torch.zeros(2, 3, dtype=torch.int64), 8, gamma=-0.5)
     assert module(torch.zeros(2, 3, 6), torch.zeros(2, 3, dtype=torch.int64), 1) == "own"
+
+
+def test_modules_saved_before_there_was_a_choice():
+    for module in (losses.FocalLoss(0.25, 2.0, 6, fallback=print), losses.CrossEntropy(torch.ones(6), fallback=print)):
+        del module.__dict__["saved_bits"]
+        again = pickle.loads(pickle.dumps(module))
+        assert again.saved_bits == 32
+        again(torch.zeros(2, 3, 6), torch.zeros(2, 3, dtype=torch.int64), 1)          # (CPU: the fallback)
