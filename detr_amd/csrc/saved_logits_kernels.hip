@@ -10,7 +10,8 @@
 //   focal           blocks of 128 consecutive logits of the flat array, clamped to +-20 first: sigmoid(-20) = 2e-9 is below
 //                   the rounding of a float32 gradient of order one, and one masked logit does not take the block's
 //                   resolution away.  The span is 40 at most, so 2^-2 always suffices and no byte is cut off at 255.
-//                   Logits of rows that do not count take no part: a padded row may hold anything.
+//                   Rows that do not count are part of the array, and so of the ranges, but a padded row may hold anything:
+//                   what lies beyond +-20 there, or is no number, counts as 0.
 //                   A head per block, 32 bits: largest whole number << 8 | e.  With a gamma below zero none of this would hold
 //                   (a slope falls off like exp((1 + gamma) z) only): refused.
 //   cross entropy   a block is a row: the softmax does not change when a row's largest logit is taken off, so e is all that
@@ -203,18 +204,25 @@ __global__ __launch_bounds__(CLS_THREADS) void focal_saved_kernel(const T *__res
     auto work = [&](unsigned block, float (&v)[4 * QUADS], BlockRows<ONE_CLASS> &rows_of, bool whole) {
         const unsigned first = block * BLOCK + 4 * sub;
         rows_of.settle(C, fp);
-        // logits of rows that do not count, or behind the last one, take no part, whatever they hold: at an infinity on their
-        // class's side their loss is 0
-        unsigned dropped = 0;
+        // logits of rows that do not count, or behind the last one, add no loss, whatever they hold: at an infinity on their class's
+        // side it is 0.  The former have their place in the block's range, as 0 what lies beyond the clamp.  (Their bytes, which
+        // saturate, are not asked for.)
+        bool some_out = false;
+        float low_before = FOCAL_CLAMP, high_before = -FOCAL_CLAMP;
         if (rows_of.skipped || !whole) {
+            some_out = true;
 #pragma unroll
             for (unsigned q = 0; q < QUADS; ++q) {
                 const unsigned at = first + 4 * LANES * q, there = whole ? 4u : at < n ? min(n - at, 4u) : 0u;
-                const unsigned out = (rows_of.dropped(q, C, fp, &bad) | (15u << there)) & 15u;
+                const unsigned none = rows_of.dropped(q, C, fp, &bad), out = none | (15u << there);
 #pragma unroll
-                for (unsigned k = 0; k < 4; ++k)
+                for (unsigned k = 0; k < 4; ++k) {
+                    const float x = v[4 * q + k], clamped = __builtin_amdgcn_fmed3f(x, -FOCAL_CLAMP, FOCAL_CLAMP);
+                    const float held = none >> k & 1 && clamped != x ? 0.0f : clamped;
+                    low_before = k < there ? dm::min3(low_before, held, held) : low_before;
+                    high_before = k < there ? dm::max3(high_before, held, held) : high_before;
                     if (out >> k & 1) v[4 * q + k] = rows_of.positive(q, k) ? __builtin_huge_valf() : -__builtin_huge_valf();
-                dropped |= out << (4 * q);
+                }
             }
         }
         float c[4 * QUADS], high = -FOCAL_CLAMP, low = FOCAL_CLAMP, sum = 0.0f;
@@ -237,26 +245,14 @@ __global__ __launch_bounds__(CLS_THREADS) void focal_saved_kernel(const T *__res
         }
         acc += (double)sum;
         if (!codes) return;
-        if (dropped) {
-            low = FOCAL_CLAMP;
-            high = -FOCAL_CLAMP;
-#pragma unroll
-            for (unsigned j = 0; j < 4 * QUADS; ++j) {
-                low = dropped >> j & 1 ? low : dm::min3(low, c[j], c[j]);
-                high = dropped >> j & 1 ? high : dm::max3(high, c[j], c[j]);
-            }
-        }
+        low = some_out ? low_before : low;
+        high = some_out ? high_before : high;
         high = dm::largest<LANES>(high);
         low = -dm::largest<LANES>(-low);
         const bool block_nan = ((__ballot(nan) >> (lane & ~(LANES - 1))) & ((1u << LANES) - 1)) != 0;
         const int e = step_exponent(high, low, FOCAL_COARSEST);
         const float inverse = power_of_two(-e);
         const float top = __builtin_rintf(high * inverse);
-        if (dropped) {
-#pragma unroll
-            for (unsigned j = 0; j < 4 * QUADS; ++j)
-                if (dropped >> j & 1) c[j] = high;             // (the byte 0)
-        }
 #pragma unroll
         for (unsigned q = 0; q < QUADS; ++q) {
             unsigned packed = 0;

@@ -344,9 +344,9 @@ int dm_cross_entropy_f32(const float *logits, const int64_t *target_cls, const f
  * e >= -16 for which the whole numbers q(x) = rint(x 2^-e) of the block span at most 255; a byte is
  * min(max q - q(x), 255).  All of it is exact in float32: the bytes follow from this definition alone.
  *   focal          blocks of 128 consecutive logits of the flat array (the last one may be shorter), clamped to +-20 first;
- *                  e <= -2; heads[block] = max q << 8 | (e & 255); the logit is (max q - byte) 2^e.  Logits of rows that do
- *                  not count (ignored, or of a class that is none) take no part and get the byte 0; a block of such alone
- *                  has any head but that of a NaN
+ *                  e <= -2; heads[block] = max q << 8 | (e & 255); the logit is (max q - byte) 2^e.  In rows that do not
+ *                  count (ignored, or of a class that is none) a logit beyond +-20 or NaN counts as 0,
+ *                  and the bytes mean nothing
  *   cross entropy  a block is a row, clamped to +-2^20 first; e <= -3; steps[row] = e; the logit is -byte 2^e, but for a
  *                  constant of the row (the byte 255 stands for anything further below the largest than 31.9)
  * e = -128: the block holds a NaN (cross entropy: the row's softmax is NaN); its gradient is NaN.

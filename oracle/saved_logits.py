@@ -18,27 +18,24 @@ def step_exponent(block, coarsest):
 
 def focal_codes(x, keep=True):
     """(bytes [n], heads [blocks], decoded logits like x) of the flat array; the heads as signed 32-bit words.  keep: whether a
-    logit's row counts; the others take no part (they decode to 0 here, a block of them alone has the head 0).
+    logit's row counts; of the others what lies beyond the clamp, or is NaN, counts as 0.
     """
     flat = np.asarray(x, dtype=np.float64).reshape(-1)
     keep = np.broadcast_to(keep, np.shape(x)).reshape(-1)
     codes, heads, decoded = np.zeros(flat.size, np.uint8), [], np.empty(flat.size)
     for i in range(0, flat.size, 128):
-        kept = np.flatnonzero(keep[i:i + 128]) + i
-        decoded[i:i + 128] = 0.0
-        if not kept.size:
-            heads.append(0)
-            continue
-        block = np.clip(flat[kept], -FOCAL_CLAMP, FOCAL_CLAMP)
+        kept = keep[i:i + 128]
+        block = flat[i:i + 128]
+        block = np.where(kept, np.clip(block, -FOCAL_CLAMP, FOCAL_CLAMP), np.where(np.abs(block) <= FOCAL_CLAMP, block, 0.0))
         if np.isnan(block).any():
             heads.append(NOT_A_NUMBER & 255)
-            decoded[kept] = np.nan
+            decoded[i:i + 128] = np.nan
             continue
         e = step_exponent(block, FOCAL_COARSEST)
         q = np.rint(block * 2.0 ** -e)
-        codes[kept] = q.max() - q
+        codes[i:i + 128] = q.max() - q
         heads.append(int(q.max()) * 256 + (e & 255))
-        decoded[kept] = q * 2.0 ** e
+        decoded[i:i + 128] = q * 2.0 ** e
     return codes, np.array(heads, dtype=np.int64).astype(np.int32), decoded.reshape(np.shape(x))
 
 

@@ -10,6 +10,7 @@ from detr_amd import _lib, losses
 from detr_amd._lib import lib
 from oracle import balance_loss as oracle
 from test_gpu_balance_loss import check_set
+from test_gpu_saved_logits import check_focal
 
 pytestmark = pytest.mark.gpu
 
@@ -118,6 +119,37 @@ def test_a_row_of_more_than_2_30_classes():
         negative = (grad[0] <= 0).nonzero().flatten().tolist()
         assert negative == ([] if hot is None else [hot])
         del grad
+
+
+@pytest.mark.parametrize("C", [1, 2, 3, 11, 91, 128, 130, 300, 1203])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_rows_that_do_not_count_are_part_of_the_ranges(C, dtype):
+    """They widen a block's step with what they hold within +-20; what lies beyond, infinities and NaN count as 0."""
+    gen = torch.Generator().manual_seed(C)
+    Q = 37 if C < 1000 else 5
+    x = torch.randn(5, Q, C, generator=gen)
+    cls = torch.where(torch.rand(5, Q, generator=gen) < 0.2, torch.randint(0, C, (5, Q), generator=gen), C)
+    ignored = torch.rand(5, Q, generator=gen) < 0.4
+    ignored[1] = True
+    ignored[4, Q - 1] = C % 2 == 0
+    cls[ignored] = -1
+    x[ignored] *= 8
+    x = x.clamp(-20, 20).to(DTYPES[dtype])
+    check_focal(x, cls, ignore_index=-1)
+    held = torch.rand(x.shape, generator=gen)
+    for value, low in ((20.0, 0.9), (-20.0, 0.8), (math.inf, 0.7), (-math.inf, 0.6), (math.nan, 0.5), (25.0, 0.4), (-30000.0, 0.3)):
+        x[ignored[..., None] & (held > low) & (held < low + 0.1)] = value
+    dev = x.cuda().requires_grad_(True)
+    loss = losses.focal_loss(dev, cls.cuda(), 3.0, ignore_index=-1, saved_bits=8)
+    (grad,) = torch.autograd.grad(loss, dev)
+    y = torch.where(ignored[..., None] & ~(x.abs() <= 20), torch.zeros_like(x), x)
+    dev = y.cuda().requires_grad_(True)
+    same = losses.focal_loss(dev, cls.cuda(), 3.0, ignore_index=-1, saved_bits=8)
+    assert torch.equal(loss, same) and torch.equal(grad, torch.autograd.grad(same, dev)[0])
+    check_focal(y, cls, ignore_index=-1)
+    # (the last logit is a live one beyond the clamp: what is behind it in the block adds nothing)
+    cls[4, Q - 1], y[4, Q - 1] = C, 40.0
+    check_focal(y, cls, ignore_index=-1)
 
 
 def test_a_gamma_below_zero_is_refused():
