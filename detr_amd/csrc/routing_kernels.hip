@@ -9,18 +9,20 @@
 //
 // Forward: workgroups walk chunks of an image's rows, a group of lanes per row; sums over rows stay in registers of the
 // lane that owns the expert (in float32 for RUN rows, then they go to 64 bits in shared memory), and leave once per workgroup,
-// into a slot of the workspace.  A second kernel adds the slots in
-// index order in 64 bits: no float atomics, the same bits every run.  A group that one workgroup walks needs no second kernel.
+// into a slot of the workspace.  A second kernel adds the slots in index order in 64 bits: no two lanes add to one place, the
+// same bits every run.  A group that one workgroup walks needs no second kernel.
 //
 // What bounds it, as measured (a copy of a GiB runs at 5.1 TB/s, a kernel of a few workgroups takes 4 us among others):
 //   memory          6 x 256 x 900 x 64 float32, top 4 (354 MB): forward 107 us, sums and loss 5 each, backward 123 (708 MB at
 //                   5.8 TB/s).  Forward, sums and loss by themselves, over and over, take 75 (4.7 TB/s); in a step they wait for the
 //                   gradients of the one before, of which the caches hold up to 256 MB, to be written.
-//   instructions    16-bit logits with many choices: 2 x 64 x 1050 x 160 bfloat16, sigmoid scores, top 8 (43 MB): forward 35 us,
-//                   sums and loss 7, backward 27; counts alone of 256 x 900 x 256, top 8 (118 MB): 44 us, the vector units
-//                   busy four fifths of it, 20 instructions per logit of which 6 keep the list and 3 make the order.
-//   the launches    6 x 64 x 600 x 16 float32 (15 MB): 10.5, 5.5 and 8.6 us; 1 x 300 x 8, where one workgroup makes the loss as well:
-//                   6.0 and 2.8.
+//   instructions    16-bit logits with many choices: 2 x 64 x 1050 x 160 bfloat16, sigmoid scores, top 8 (43 MB): forward 36 us,
+//                   sums and loss 7, backward 27; 6 x 256 x 900 x 64 bfloat16, softmax, top 4 (177 MB): 70, 9 and 89; counts alone
+//                   of 256 x 900 x 256, top 8 (118 MB): 44 us, the vector units busy four fifths of it.  Of the 20 instructions per
+//                   logit 6 keep the list and 3 make the order; taking the heads off the lists (for the top 8 seven rounds that
+//                   wait for one another) costs a lane about a hundred a row, however few logits it holds.
+//   the launches    6 x 64 x 600 x 16 float32 (15 MB): 11.2, 5.4 and 8.6 us; 1 x 300 x 8, where one workgroup makes the loss as
+//                   well: 6.1 and 2.8.
 #include <algorithm>
 #include <climits>
 
@@ -751,7 +753,7 @@ int check_shape(const DmRouterSet *sets, int S, int B, int E, int per_image, Sha
 // Quads of four logits per lane, and lanes per row.
 //   Forward: as few lanes as can hold the row with sixteen logits each.  Every reduction over lanes is paid per row, every
 //   lane behind the row's end as well: 354 MB of float32 logits of 16, 48, 64 and 96 experts (top 2, 4, 4, 4) take 79, 79, 79 and
-//   80 us, with half as many logits per lane 105, 101, 89 and 117 us.
+//   80 us, with half as many logits per lane 105, 101, 89 and 117 us.  (More than sixteen have not been measured.)
 //   Backward, float32: four logits per lane and up to sixteen lanes, whose store is a run of memory; in the forward pass's
 //   forms 12, 24 and 48 experts take 171, 169 and 157 us for 354 MB read and written instead of 152, 149 and 149.
 //   Backward, 16 bits: bound by instructions, not memory, where lanes lie behind the row's end: 12, 20, 33 and 96 experts take
@@ -917,7 +919,8 @@ struct Workspace {
 };
 Workspace workspace_of(const DmRouterSet *sets, const Shape &sh)
 {
-    return Workspace{most_blocks(sets, sh, forward_pass(sets, sh)), (unsigned long long)std::min(sh.S, DM_MAX_SETS_PER_LAUNCH) * (sh.per_image ? (unsigned long long)sh.B : 1ull)};
+    const unsigned long long groups = sh.per_image ? (unsigned long long)sh.B : 1ull;      // of a set
+    return Workspace{most_blocks(sets, sh, forward_pass(sets, sh)), (unsigned long long)std::min(sh.S, DM_MAX_SETS_PER_LAUNCH) * groups};
 }
 
 int forward(const DmRouterSet *sets, int S, int B, int E, int top_k, int dtype, int scores, int per_image,
@@ -1031,9 +1034,9 @@ extern "C" int dm_balance_backward(const DmRouterSet *sets, int S, int B, int E,
         const int n = std::min(S - first, DM_MAX_SETS_PER_LAUNCH);
         const unsigned blocks = (unsigned)describe(sets, first, n, sh, 0, backward_pass(sh, dtype == DM_F32), &a);
         const size_t g0 = (size_t)first * (per_image ? (size_t)B : 1);
-        hipLaunchKernelGGL(dtype == DM_F32 ? backward_for<true>((unsigned)E) : backward_for<false>((unsigned)E), dim3(blocks), dim3(RT_THREADS), 0, st, a, dtype, scores == DM_SCORES_SIGMOID ? 1 : 0,
-                           slope + g0 * E, inv_rows + g0, grad_balance ? grad_balance + g0 : nullptr,
-                           grad_z ? grad_z + g0 : nullptr);
+        hipLaunchKernelGGL(dtype == DM_F32 ? backward_for<true>((unsigned)E) : backward_for<false>((unsigned)E), dim3(blocks),
+                           dim3(RT_THREADS), 0, st, a, dtype, scores == DM_SCORES_SIGMOID ? 1 : 0, slope + g0 * E, inv_rows + g0,
+                           grad_balance ? grad_balance + g0 : nullptr, grad_z ? grad_z + g0 : nullptr);
         rc = dm::check_hip(hipGetLastError(), "router_backward_kernel launch");
         if (rc != DM_OK) return rc;
     }

@@ -21,14 +21,15 @@
 //
 // The gradient is that of the loss at the decoded logits; the loss itself is of the logits as they came.
 //
-// Measured (a copy of a GiB runs at 5.1 TB/s, a kernel of a few workgroups takes 4 us among others), forward and backward:
-//   focal           256 x 900 x 91 float32 (84 MB of logits, 21 of bytes): 27 and 25 us, 4 TB/s, bound by 50 and 35 vector
-//                   instructions per logit, an exponential, a logarithm and a reciprocal among them; 4 x 300 x 1203 bfloat16: 7.6 and 6.1;
-//                   64 x 600 x 2 float32: 4.6 and 4.3
-//   cross entropy   256 x 900 x 92 float32 (85 MB, 21 MB): 22.4 and 18.7 us, 4.7 and 5.7 TB/s, at the rate of a copy;
-//                   16 x 301 x 1205 float16 (12 MB, 6 MB): 10.9 and 8.4
-// The sums of the workgroups' partial sums take 2 to 4 us more; one workgroup by itself makes the loss as well.  The host's part of a call and its backward pass, about 45 us,
-// most of it the autograd engine's, covers all of these.
+// Measured in a step (a copy of a GiB runs at 5.1 TB/s, a kernel of a few workgroups takes 4 us among others), forward and backward:
+//   focal           256 x 900 x 91 float32 (84 MB of logits, 21 of bytes): 27.5 and 25.6 us, 4 TB/s, bound by 50 and 35 vector
+//                   instructions per logit, an exponential, a logarithm and a reciprocal among them; the same of bfloat16: 26.9 and
+//                   25.5; with a fifth of the rows ignored: 34.3 and 28.4 (what does not count is asked of each quad of a wave that
+//                   meets such a row); 4 x 300 x 1203 bfloat16: 7.8 and 5.9; 64 x 600 x 2 float32: 4.6 and 4.2
+//   cross entropy   256 x 900 x 92 float32 (85 MB, 21 MB): 22.5 and 19.1 us, 4.7 and 5.6 TB/s, at the rate of a copy; of bfloat16
+//                   20.9 and 16.4; 16 x 301 x 1205 float16 (12 MB, 6 MB): 10.3 and 8.3
+// The sums of the workgroups' partial sums take 2 to 4 us more; one workgroup by itself makes the loss as well.  The host's part of
+// a call and its backward pass, about 45 us, most of it the autograd engine's, covers all of these.
 #include <algorithm>
 #include <climits>
 
@@ -554,8 +555,8 @@ __global__ __launch_bounds__(CLS_THREADS) void ce_from_saved_kernel(const uint8_
 }
 
 // Rows too long for a wavefront's registers: a workgroup per row, which it walks twice (forward: largest, smallest and sum
-// of exponentials in one pass, the bytes in the second, out of the cache; backward: the sum, then the gradient).  354 MB of float32
-// logits of 4096 classes take 127 and 161 us, of 2048 classes in registers 95 and 89.
+// of exponentials in one pass, the bytes in the second, out of the cache; backward: the sum, then the gradient).  In a step 354 MB of
+// float32 logits of 4096 classes take 144 and 155 us, of 2048 classes in registers 120 and 76: every exponential is taken twice.
 constexpr int WIDE_WAVES = CLS_THREADS / 64;
 
 struct RowStats {
@@ -738,7 +739,8 @@ constexpr unsigned WIDEST = 2048;      // logits of a row that a wavefront keeps
 // Quads of four logits per lane, and lanes per row.  Two quads and twice the lanes make longer runs of stores: the backward pass
 // takes 118, 119 and 88 us for 354 MB of float32 gradients of 24, 32 and 64 classes, with twelve or sixteen logits per lane 153, 179
 // and 126.  The forward pass of 16-bit logits is bound by instructions, and lanes behind the row's end are wasted ones: 12, 24
-// and 48 classes take 79, 73 and 67 us for 177 MB with twelve logits per lane, 94, 95 and 94 with eight.
+// and 48 classes take 79, 73 and 67 us for 177 MB with twelve logits per lane, 94, 95 and 94 with eight.  (1537 to 1792 classes take
+// the form of 2048, an eighth of its quads empty: one of seven quads has not been built.)
 struct Form {
     int NQ, L;
 };
