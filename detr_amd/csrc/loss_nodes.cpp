@@ -5,7 +5,8 @@
 // As Python functions the same nodes cost more than their kernels at the criterion's ordinary sizes: the backward pass runs in
 // the autograd engine's thread, which has to take the interpreter lock from the caller's and hand it back.  Host time of
 // forward and backward of a focal loss of 4 x 300 x 91 logits: 117 us as Python nodes, 55 us as these (of which the engine
-// itself takes some 40); of the balance loss of 1 x 300 x 8: 141 us and 63 us.  Nothing here holds the lock in the backward pass.
+// itself takes some 40); of the balance loss of 1 x 300 x 8: 141 us and 63 us.  Nothing here holds the lock in the backward
+// pass (but for hooks of Python on saved tensors).
 //
 // No GPU code: the kernels are reached through the addresses of libdetr_match.so's entry points, handed over once by `bind`.
 // Built against one torch version, which the module names (`built_for_torch`); the Python code refuses it under any other.
@@ -139,7 +140,8 @@ struct Saved {
     at::DimVector sizes;
 
     Saved() = default;
-    explicit Saved(const Tensor &t) : variable(t, false), device(t.device()), type(t.scalar_type()), sizes(t.sizes()) {}
+    // (a tensor of inference mode cannot be saved as it is)
+    explicit Saved(const Tensor &t) : variable(t.is_inference() ? t.clone() : t, false), device(t.device()), type(t.scalar_type()), sizes(t.sizes()) {}
     Tensor unpack() const
     {
         const Tensor t = variable.unpack();
@@ -474,7 +476,7 @@ Tensor workspace_for(const std::vector<DmRouterSet> &sets, const RouterCall &c, 
 
 struct BalanceNode : LossNode {
     RouterCall call;
-    std::vector<Saved> logits, masks;
+    std::vector<Saved> logits, masks;      // (of the sets that need a gradient)
     std::vector<char> masked;
     Saved kept;       // slope [groups, E], then 1 / n [groups]
 
@@ -583,10 +585,12 @@ std::tuple<Tensor, std::optional<Tensor>, Tensor> balance_losses(const std::vect
         below.reset();                                 // (saving may run hooks)
         node->call = c;
         node->kept = Saved(kept);
+        node->logits.resize(in.size());
         node->masked.resize(in.size());
         node->masks.resize(in.size());
         for (size_t i = 0; i < in.size(); ++i) {
-            node->logits.emplace_back(r.logits[i]);
+            if (!in[i].requires_grad()) continue;
+            node->logits[i] = Saved(r.logits[i]);
             node->masked[i] = r.masks[i].defined();
             if (node->masked[i]) node->masks[i] = Saved(r.masks[i]);
         }

@@ -138,6 +138,29 @@ def test_the_loss_may_be_changed_in_place():
 
 
 @pytest.mark.parametrize("name", NAMES)
+def test_class_maps_and_masks_of_inference_mode(name):
+    """What a data pipeline made in inference mode cannot be saved as it is: it is copied."""
+    x, cls = data()
+    mask = torch.rand(cls.shape, generator=torch.Generator().manual_seed(1)).cuda() < 0.8
+    results = []
+    for made in (lambda t: t, lambda t: t.clone()):
+        with torch.inference_mode():
+            c, m = made(cls), made(mask)
+        leaf = x.clone().requires_grad_(True)
+        (grad,) = torch.autograd.grad(calls(c, m)[name][0](leaf), leaf)
+        results.append(grad)
+    assert c.is_inference() and m.is_inference() and torch.equal(*results)
+    if name in ("balance", "sigmoid"):        # logits of a frozen router
+        with torch.inference_mode():
+            frozen = x.clone()
+        scores = "softmax" if name == "balance" else name
+        leaf = x.clone().requires_grad_(True)
+        (grad,) = torch.autograd.grad(losses.balance_losses([frozen, leaf], 3, scores=scores).balance[1], leaf)
+        (want,) = torch.autograd.grad(losses.balance_losses([x, leaf], 3, scores=scores).balance[1], leaf)
+        assert torch.equal(grad, want)
+
+
+@pytest.mark.parametrize("name", NAMES)
 def test_forward_mode_and_tracing_are_refused(name):
     import torch.autograd.forward_ad as fw
 
